@@ -135,7 +135,9 @@ mi_status mi_context_synchronize(mi_context* ctx);
 /* Synchronizes, then reports (and clears) the code of a bounded device wait
  * that expired since the last call: 0 = none; otherwise MI_ERR_TIMEOUT is
  * returned and *code names the wait (tensor-core GEMM pipeline: 1 producer,
- * 2 MMA issuer, 3 epilogue, 4 drain). No reference counterpart: Metal
+ * 2 MMA issuer, 3 epilogue, 4 drain). Returns MI_ERR_INVALID_ARGUMENT or
+ * MI_ERR_CONFIG when a kernel of this context refused a device-side argument
+ * since then (see the ragged batches below). No reference counterpart: Metal
  * command-buffer errors (context.rs:1058-1063) have no device-side waits. */
 mi_status mi_context_kernel_status(mi_context* ctx, uint32_t* code);
 /* The context's CUDA stream (cudaStream_t) for interop. */
@@ -201,7 +203,8 @@ mi_status mi_batch_finish(mi_batch* b, mi_dispatch_stats* stats);
 void mi_batch_abandon(mi_batch* b);
 /* PendingBatch::wait: consumes the pending handle; stats may be NULL.
  * Returns MI_ERR_TIMEOUT when a kernel's bounded device wait expired (its
- * outputs are not valid), as mi_context_kernel_status reports it. */
+ * outputs are not valid), MI_ERR_INVALID_ARGUMENT or MI_ERR_CONFIG when one
+ * refused a device-side argument, as mi_context_kernel_status reports it. */
 mi_status mi_pending_wait(mi_pending* p, mi_dispatch_stats* stats);
 /* Non-consuming completion query: 1 done, 0 running. */
 int mi_pending_is_complete(const mi_pending* p);
@@ -270,6 +273,82 @@ mi_status mi_batch_attention_flash_decode_with_configuration(
 /* ops.rs:1249-1285 */
 mi_status mi_batch_copy_into_cache(mi_batch* b, const mi_tensor* source, mi_tensor* cache,
                                    size_t offset);
+
+/* ---- ragged batches --------------------------------------------------------
+ * A step of several requests at once. No counterpart in the reference, which
+ * serves one sequence: these ops stand beside qk_norm_rope_cache,
+ * copy_into_cache, attention and mi_sample_logits for callers that batch.
+ *
+ * A paged cache is a tensor [pages, page_size, kv_heads, head_dim] (any page
+ * size; a layer's contiguous cache reshaped into pages is one). Position p of
+ * sequence s is row p % page_size of page table[s][p / page_size]; `table` is
+ * u32 [sequences, width], `lengths` u32 [sequences]. Packed tensors hold the
+ * sequences' tokens end to end: sequence s is rows [starts[s], starts[s + 1])
+ * of `starts`, u32 [sequences + 1], rising, its last value at most the rows.
+ * Rows before the first start and behind the last are left as they were.
+ *
+ * All outputs are written into tensors of the caller, so that a captured step
+ * replays on the same addresses; starts, lengths, tables and options are read
+ * on the device at run time. A start, length, page id or option outside of
+ * its range is left out by the kernel (its rows' values are then unspecified,
+ * nothing outside of the tensors is touched) and the next mi_pending_wait or
+ * mi_context_kernel_status of the context returns MI_ERR_INVALID_ARGUMENT
+ * (MI_ERR_CONFIG for sampling options).
+ *
+ * Every tensor must belong to the batch's context; data tensors start on a
+ * 16-byte boundary; outputs do not overlap inputs (paged_append may rotate
+ * queries in place). head_dim is 64 or 128, query_heads a multiple of
+ * kv_heads. Calls may be captured into CUDA graphs; a captured call has
+ * scratch of its own. */
+
+/* RoPE (and RMSNorm) of a paged append. */
+typedef struct mi_paged_rope {
+  float theta;
+  float epsilon;
+} mi_paged_rope;
+
+/* qk_norm_rope_cache + copy_into_cache for a ragged batch: sequence s appends
+ * tokens [starts[s], starts[s + 1]) at its positions lengths[s] - n ...
+ * lengths[s] - 1 (`lengths` counts the new tokens). Keys get per-head RMSNorm
+ * (with key_weight; NULL leaves it out, and then RoPE alone, as mi_batch_rope)
+ * and RoPE, values are copied; queries are transformed the same way into
+ * query_out (query, query_weight and query_out NULL: no queries). Same bits
+ * as mi_batch_qk_norm_rope_cache / mi_batch_rope. Sequences must not share a
+ * slot that is written. */
+mi_status mi_batch_paged_append(mi_batch* b, const mi_tensor* query, const mi_tensor* key,
+                                const mi_tensor* value, const mi_tensor* query_weight,
+                                const mi_tensor* key_weight, const mi_tensor* starts,
+                                const mi_tensor* lengths, const mi_tensor* table,
+                                mi_tensor* key_cache, mi_tensor* value_cache,
+                                mi_tensor* query_out, mi_paged_rope config);
+/* Attention of one new token per sequence: query and out [sequences,
+ * query_heads, head_dim]; token s sees positions [0, lengths[s]). A sequence of
+ * length 0 gives zeros. Results do not depend on timing. */
+mi_status mi_batch_paged_attention(mi_batch* b, const mi_tensor* query,
+                                   const mi_tensor* key_cache, const mi_tensor* value_cache,
+                                   const mi_tensor* lengths, const mi_tensor* table,
+                                   mi_tensor* out);
+/* Attention over packed prompts: queries [query_starts[s], ...) of sequence s
+ * see keys [key_starts[s], ...) of the same sequence. With `causal` the last
+ * query sees the last key, the one before it one key less: equal lengths are
+ * the usual causal prompt, more keys than queries a prompt whose beginning was
+ * computed before. Queries that see no key give zeros. */
+mi_status mi_batch_packed_attention(mi_batch* b, const mi_tensor* query, const mi_tensor* key,
+                                    const mi_tensor* value, const mi_tensor* query_starts,
+                                    const mi_tensor* key_starts, int causal, mi_tensor* out);
+/* One token per row of logits [rows, vocab] (vocab up to 524224): temperature,
+ * top_p, min_p and uniform F32 [rows], top_k U32 [rows] (0: all). Candidates
+ * are the finite logits, ordered as in mi_sample_logits. top_k keeps the
+ * first; over their exp((v - max) / temperature), in FP64, top_p keeps the
+ * candidates with less than top_p of the sum before them (1: all) and min_p
+ * those of weight >= min_p; the first always stays. The token is the first
+ * kept candidate whose running sum exceeds uniform (in [0, 1)) times the kept
+ * sum. Temperature 0 takes the first candidate, of equal ones the lowest index
+ * (mi_batch_argmax takes the highest). Writes 0xFFFFFFFF where no logit is
+ * finite. tokens: U32 [rows]. */
+mi_status mi_batch_sample(mi_batch* b, const mi_tensor* logits, const mi_tensor* temperature,
+                          const mi_tensor* top_k, const mi_tensor* top_p, const mi_tensor* min_p,
+                          const mi_tensor* uniform, mi_tensor* tokens);
 
 /* One-query flash decode that allocates nothing. No counterpart in the
  * reference: it serves callers that cannot allocate device memory at the

@@ -145,6 +145,13 @@ __device__ __forceinline__ void hist_add_rows(const uint16_t* logits, int first,
   __syncthreads();
 }
 
+// Says in a context's fault word (mapped host memory) that a device-side
+// argument was refused; the host reads it after a synchronization.
+__device__ __forceinline__ void report_fault(uint32_t* fault, uint32_t code) {
+  *reinterpret_cast<volatile uint32_t*>(fault) = code;
+  __threadfence_system();
+}
+
 __device__ __forceinline__ uint32_t pos_of(const Pos& p) {
   return p.dev ? (*p.dev + p.base) : p.base;
 }

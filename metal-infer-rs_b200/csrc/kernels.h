@@ -218,6 +218,67 @@ constexpr int kMmaPrefillMinTokens = 512;
 // The tensor-core prefill attention; false when the problem does not fit it.
 bool attention_prefill_mma(const Launch& l, const AttnProblem& p);
 
+// ---- ragged batches --------------------------------------------------------------
+// Device-side arguments that a kernel refused (mi_context::fault).
+enum Fault : uint32_t {
+  kFaultStarts = 1,   // starts that do not rise, or leave the rows
+  kFaultLength = 2,   // a length its page table cannot hold, or below the appended tokens
+  kFaultPage = 3,     // a page id outside of the cache
+  kFaultSampling = 4  // sampling options outside of their ranges
+};
+// Q/K norm (with weights), RoPE and the append to pages of a packed batch:
+// sequence s holds tokens [starts[s], starts[s + 1]), the last of them at
+// position lengths[s] - 1. q / q_out may be null (no query).
+struct PagedAppend {
+  const __half *q = nullptr, *k = nullptr, *v = nullptr;  // [tokens, heads, hd]
+  const __half *qw = nullptr, *kw = nullptr;              // [hd] or null
+  __half* q_out = nullptr;
+  __half *key_cache = nullptr, *value_cache = nullptr;    // [pages, page, kvh, hd]
+  const uint32_t *starts = nullptr, *lengths = nullptr, *table = nullptr;
+  uint32_t* fault = nullptr;
+  int tokens = 0, sequences = 0, qh = 0, kvh = 1, hd = 128, table_width = 0, page = 1;
+  uint32_t pages = 0;
+  float theta = 1e6f, eps = 1e-6f;
+};
+void paged_append(const Launch& l, const PagedAppend& p);
+// Attention of one new token per sequence over its pages.
+struct PagedAttention {
+  const __half* q = nullptr;  // [sequences, qh, hd]
+  const __half *key_cache = nullptr, *value_cache = nullptr;
+  __half* out = nullptr;
+  const uint32_t *lengths = nullptr, *table = nullptr;
+  uint32_t* fault = nullptr;
+  int sequences = 0, qh = 1, kvh = 1, hd = 128, table_width = 0, page = 1;
+  uint32_t pages = 0;
+};
+// Bytes of device scratch of a paged_attention launch (nothing is kept in it
+// from one launch to the next).
+size_t paged_attention_workspace(int sm_count, int hd);
+void paged_attention(const Launch& l, const PagedAttention& p, void* workspace);
+// Attention over packed sequences: queries [query_starts[s],
+// query_starts[s + 1]) see keys of [key_starts[s], key_starts[s + 1]); with
+// `causal` the last query sees the last key, the one before it one key less.
+struct PackedAttention {
+  const __half *q = nullptr, *k = nullptr, *v = nullptr;
+  __half* out = nullptr;
+  const uint32_t *query_starts = nullptr, *key_starts = nullptr;
+  uint32_t* fault = nullptr;
+  int tokens = 0, keys = 0, sequences = 0, qh = 1, kvh = 1, hd = 128, causal = 1;
+};
+void packed_attention(const Launch& l, const PackedAttention& p);
+// One token per row of logits [rows, n] under that row's options.
+struct SampleBatch {
+  const __half* logits = nullptr;
+  const float *temperature = nullptr, *top_p = nullptr, *min_p = nullptr, *uniform = nullptr;
+  const uint32_t* top_k = nullptr;
+  uint32_t* tokens = nullptr;
+  uint32_t* fault = nullptr;
+  int rows = 0, n = 0;
+};
+// Largest vocabulary of sample_batch: a block's histogram counts in 16 bits.
+constexpr int kSampleBatchMax = 8 * 65528;
+void sample_batch(const Launch& l, const SampleBatch& p);
+
 // ---- tensor parallelism -----------------------------------------------------------
 // out[i] = half(parts[0][i] + parts[1][i] + ... + parts[tp-1][i]), summed in
 // rank order in FP32 (parts: [tp, n] as gathered from the ranks).

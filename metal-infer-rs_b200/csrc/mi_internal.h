@@ -119,6 +119,9 @@ struct mi_context {
   // Reusable zero-initialised scratch for split reductions (grown on demand).
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
+  // Mapped host word that kernels write when they refuse a device-side
+  // argument (k::Fault), read after a synchronization.
+  uint32_t* fault = nullptr;
 };
 
 struct mi_batch {
@@ -152,6 +155,11 @@ unsigned take_device_wait_status();
 // synchronization): a launch that gave up returns early, so its outputs are
 // not valid and must not be reported as a result.
 void check_device_waits(const char* what);
+
+// Fails with MI_ERR_INVALID_ARGUMENT (MI_ERR_CONFIG for sampling options) when
+// a kernel refused a device-side argument of the context since the last check
+// (after a synchronization).
+void check_device_arguments(mi_context* ctx);
 
 // Per-launch profiling hooks (CUDA events around a launch when enabled).
 struct ProfileScope {

@@ -696,3 +696,322 @@ mi_status mi_fill_tokens_u32(mi_context* ctx, mi_tensor* t, uint64_t seed, uint6
 }
 
 }  // extern "C"
+
+namespace {
+
+// ---- ragged batches ----------------------------------------------------------
+
+// Makes the context's device the calling thread's for one op.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(const mi_context* ctx) {
+    MI_CUDA(cudaGetDevice(&before));
+    if (before == ctx->device) before = -1;
+    else MI_CUDA(cudaSetDevice(ctx->device));
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+// A tensor of the batch's context with this dtype and rank.
+void require_tensor(const mi_context* ctx, const mi_tensor* t, mi_dtype dtype, size_t rank,
+                    const char* what) {
+  require(t, what);
+  MI_REQUIRE(t->buf->ctx == ctx, MI_ERR_INVALID_ARGUMENT, "%s belongs to another context", what);
+  if (t->dtype != dtype)
+    fail(MI_ERR_DTYPE, "unsupported dtype: %s expects %s, got %s", what, dtype_name(dtype),
+         dtype_name(t->dtype));
+  if (t->shape.size() != rank)
+    fail(MI_ERR_SHAPE, "invalid tensor shape: %s must have rank %zu, got %s", what, rank,
+         shape_str(t->shape).c_str());
+}
+
+void require_shape(const mi_tensor* t, const std::vector<size_t>& shape, const char* what) {
+  if (t->shape != shape)
+    fail(MI_ERR_SHAPE, "invalid tensor shape: %s must be %s, got %s", what,
+         shape_str(shape).c_str(), shape_str(t->shape).c_str());
+}
+
+void require_aligned(const mi_tensor* t, size_t bytes, const char* what) {
+  MI_REQUIRE(reinterpret_cast<uintptr_t>(t->base()) % bytes == 0, MI_ERR_INVALID_ARGUMENT,
+             "%s must start on a %zu-byte boundary", what, bytes);
+}
+
+void require_apart(const mi_tensor* out, const mi_tensor* in, const char* what) {
+  const char *a = out->base(), *b = in->base();
+  MI_REQUIRE(a + out->bytes() <= b || b + in->bytes() <= a, MI_ERR_INVALID_ARGUMENT,
+             "the output overlaps %s", what);
+}
+
+// Heads and head_dim of a query / KV pair of shapes.
+void require_heads(size_t qh, size_t qd, size_t kvh, size_t kd) {
+  if (qd != kd)
+    fail(MI_ERR_SHAPE, "invalid tensor shape: query and key head_dim differ: %zu and %zu", qd, kd);
+  if (kd != 64 && kd != 128)
+    fail(MI_ERR_SHAPE, "invalid tensor shape: head_dim must be 64 or 128, got %zu", kd);
+  if (kvh == 0 || qh == 0 || qh % kvh != 0)
+    fail(MI_ERR_SHAPE, "invalid tensor shape: query_heads must be divisible by kv_heads");
+  if (qh > 65535) fail(MI_ERR_SHAPE, "invalid tensor shape: more than 65535 query heads");
+}
+
+struct Pages {
+  size_t pages, page, kvh, hd, sequences, width;
+};
+
+Pages require_pages(const mi_context* ctx, const mi_tensor* key_cache,
+                    const mi_tensor* value_cache, const mi_tensor* lengths,
+                    const mi_tensor* table) {
+  require_tensor(ctx, key_cache, MI_F16, 4, "key cache");
+  require_tensor(ctx, value_cache, MI_F16, 4, "value cache");
+  require_tensor(ctx, lengths, MI_U32, 1, "lengths");
+  require_tensor(ctx, table, MI_U32, 2, "page table");
+  require_same_shape(key_cache, value_cache);
+  require_aligned(key_cache, 16, "key cache");
+  require_aligned(value_cache, 16, "value cache");
+  require_aligned(lengths, 4, "lengths");
+  require_aligned(table, 4, "page table");
+  Pages p{key_cache->shape[0], key_cache->shape[1], key_cache->shape[2], key_cache->shape[3],
+          lengths->shape[0], table->shape[1]};
+  if (table->shape[0] != p.sequences)
+    fail(MI_ERR_SHAPE, "invalid tensor shape: page table has %zu rows for %zu sequences",
+         table->shape[0], p.sequences);
+  if (p.page == 0) fail(MI_ERR_SHAPE, "invalid tensor shape: page size is 0");
+  // positions and cache rows are 31-bit in the kernels
+  if (p.page > 0x7FFFFFFFull || p.pages > 0x7FFFFFFFull / p.page ||
+      p.width > 0x7FFFFFFFull / p.page)
+    fail(MI_ERR_SHAPE, "invalid tensor shape: cache rows or table positions exceed 2^31");
+  if (p.sequences > 0xFFFFFFull)
+    fail(MI_ERR_SHAPE, "invalid tensor shape: more than 2^24 sequences");
+  return p;
+}
+
+void require_starts(const mi_context* ctx, const mi_tensor* starts, const char* what) {
+  require_tensor(ctx, starts, MI_U32, 1, what);
+  require_aligned(starts, 4, what);
+  if (starts->shape[0] == 0)
+    fail(MI_ERR_SHAPE, "invalid tensor shape: %s must hold sequences + 1 values", what);
+}
+
+}  // namespace
+
+extern "C" {
+
+mi_status mi_batch_paged_append(mi_batch* b, const mi_tensor* query, const mi_tensor* key,
+                                const mi_tensor* value, const mi_tensor* query_weight,
+                                const mi_tensor* key_weight, const mi_tensor* starts,
+                                const mi_tensor* lengths, const mi_tensor* table,
+                                mi_tensor* key_cache, mi_tensor* value_cache,
+                                mi_tensor* query_out, mi_paged_rope config) {
+  return guard([&] {
+    mi_context* ctx = ctx_of(b);
+    require_tensor(ctx, key, MI_F16, 3, "key");
+    require_tensor(ctx, value, MI_F16, 3, "value");
+    require_same_shape(key, value);
+    require_starts(ctx, starts, "starts");
+    const Pages pg = require_pages(ctx, key_cache, value_cache, lengths, table);
+    const size_t tokens = key->shape[0], kvh = key->shape[1], hd = key->shape[2];
+    if (kvh != pg.kvh || hd != pg.hd)
+      fail(MI_ERR_SHAPE, "invalid tensor shape: KV source/cache shapes are incompatible");
+    require_shape(starts, {pg.sequences + 1}, "starts");
+    MI_REQUIRE((query != nullptr) == (query_out != nullptr), MI_ERR_INVALID_ARGUMENT,
+               "query and query_out go together");
+    MI_REQUIRE((query_weight != nullptr) == (query != nullptr && key_weight != nullptr),
+               MI_ERR_INVALID_ARGUMENT, "query_weight goes with a query and key_weight");
+    require_heads(query ? query->shape.size() == 3 ? query->shape[1] : 0 : kvh,
+                  query && query->shape.size() == 3 ? query->shape[2] : hd, kvh, hd);
+    if (key_weight) {
+      require_tensor(ctx, key_weight, MI_F16, 1, "key weight");
+      require_shape(key_weight, {hd}, "key weight");
+      require_aligned(key_weight, 16, "key weight");
+      MI_REQUIRE(std::isfinite(config.epsilon), MI_ERR_INVALID_ARGUMENT, "epsilon is not finite");
+    }
+    if (query) {
+      require_tensor(ctx, query, MI_F16, 3, "query");
+      require_tensor(ctx, query_out, MI_F16, 3, "query output");
+      require_same_shape(query, query_out);
+      if (query->shape[0] != tokens)
+        fail(MI_ERR_SHAPE, "invalid tensor shape: %zu query and %zu key tokens",
+             query->shape[0], tokens);
+      require_aligned(query, 16, "query");
+      require_aligned(query_out, 16, "query output");
+      if (query_weight) {
+        require_tensor(ctx, query_weight, MI_F16, 1, "query weight");
+        require_shape(query_weight, {hd}, "query weight");
+        require_aligned(query_weight, 16, "query weight");
+      }
+      if (query_out->base() != query->base()) require_apart(query_out, query, "query");
+      for (const mi_tensor* t : {key, value, (const mi_tensor*)key_cache,
+                                 (const mi_tensor*)value_cache, starts, lengths, table})
+        require_apart(query_out, t, "another tensor of the call");
+    }
+    MI_REQUIRE(std::isfinite(config.theta) && config.theta > 0.f, MI_ERR_INVALID_ARGUMENT,
+               "theta must be positive and finite");
+    require_aligned(key, 16, "key");
+    require_aligned(value, 16, "value");
+    require_apart(key_cache, value_cache, "the value cache");
+    for (mi_tensor* c : {key_cache, value_cache})
+      for (const mi_tensor* t : {query, key, value, query_weight, key_weight, starts, lengths, table})
+        if (t) require_apart(c, t, "an input");
+    if (tokens == 0 || pg.sequences == 0) return;
+    DeviceScope device(ctx);
+    k::PagedAppend p;
+    if (query) {
+      p.q = query->f16();
+      p.q_out = query_out->f16();
+      p.qh = to_int(query->shape[1], "query heads");
+    }
+    p.k = key->f16();
+    p.v = value->f16();
+    p.qw = query_weight ? query_weight->f16() : nullptr;
+    p.kw = key_weight ? key_weight->f16() : nullptr;
+    p.key_cache = key_cache->f16();
+    p.value_cache = value_cache->f16();
+    p.starts = starts->u32();
+    p.lengths = lengths->u32();
+    p.table = table->u32();
+    p.fault = ctx->fault;
+    p.tokens = to_int(tokens, "tokens");
+    p.sequences = (int)pg.sequences;
+    p.kvh = to_int(kvh, "KV heads");
+    p.hd = (int)hd;
+    p.table_width = (int)pg.width;
+    p.page = (int)pg.page;
+    p.pages = (uint32_t)pg.pages;
+    p.theta = config.theta;
+    p.eps = config.epsilon;
+    ProfileScope ps(ctx, "paged_append");
+    k::paged_append(launch_of(ctx), p);
+  });
+}
+
+mi_status mi_batch_paged_attention(mi_batch* b, const mi_tensor* query,
+                                   const mi_tensor* key_cache, const mi_tensor* value_cache,
+                                   const mi_tensor* lengths, const mi_tensor* table,
+                                   mi_tensor* out) {
+  return guard([&] {
+    mi_context* ctx = ctx_of(b);
+    require_tensor(ctx, query, MI_F16, 3, "query");
+    require_tensor(ctx, out, MI_F16, 3, "output");
+    require_same_shape(query, out);
+    const Pages pg = require_pages(ctx, key_cache, value_cache, lengths, table);
+    if (query->shape[0] != pg.sequences)
+      fail(MI_ERR_SHAPE, "invalid tensor shape: %zu queries for %zu sequences", query->shape[0],
+           pg.sequences);
+    require_heads(query->shape[1], query->shape[2], pg.kvh, pg.hd);
+    require_aligned(query, 16, "query");
+    require_aligned(out, 16, "output");
+    for (const mi_tensor* t : {query, key_cache, value_cache, lengths, table})
+      require_apart(out, t, "an input");
+    if (pg.sequences == 0) return;
+    DeviceScope device(ctx);
+    k::PagedAttention p;
+    p.q = query->f16();
+    p.key_cache = key_cache->f16();
+    p.value_cache = value_cache->f16();
+    p.out = out->f16();
+    p.lengths = lengths->u32();
+    p.table = table->u32();
+    p.fault = ctx->fault;
+    p.sequences = (int)pg.sequences;
+    p.qh = to_int(query->shape[1], "query heads");
+    p.kvh = to_int(pg.kvh, "KV heads");
+    p.hd = (int)pg.hd;
+    p.table_width = (int)pg.width;
+    p.page = (int)pg.page;
+    p.pages = (uint32_t)pg.pages;
+    // stream-ordered scratch of this call: a captured call keeps its own, so
+    // two graphs never share it
+    Out ws;
+    ws.t = new_tensor(ctx, {k::paged_attention_workspace(ctx->sm_count, p.hd) / 4}, MI_F32);
+    ProfileScope ps(ctx, "paged_attention");
+    k::paged_attention(launch_of(ctx), p, ws.t->base());
+  });
+}
+
+mi_status mi_batch_packed_attention(mi_batch* b, const mi_tensor* query, const mi_tensor* key,
+                                    const mi_tensor* value, const mi_tensor* query_starts,
+                                    const mi_tensor* key_starts, int causal, mi_tensor* out) {
+  return guard([&] {
+    mi_context* ctx = ctx_of(b);
+    require_tensor(ctx, query, MI_F16, 3, "query");
+    require_tensor(ctx, key, MI_F16, 3, "key");
+    require_tensor(ctx, value, MI_F16, 3, "value");
+    require_tensor(ctx, out, MI_F16, 3, "output");
+    require_same_shape(key, value);
+    require_same_shape(query, out);
+    require_starts(ctx, query_starts, "query starts");
+    require_starts(ctx, key_starts, "key starts");
+    require_shape(key_starts, query_starts->shape, "key starts");
+    require_heads(query->shape[1], query->shape[2], key->shape[1], key->shape[2]);
+    for (const mi_tensor* t : {query, key, value, (const mi_tensor*)out})
+      require_aligned(t, 16, "a tensor of attention");
+    for (const mi_tensor* t : {query, key, value, query_starts, key_starts})
+      require_apart(out, t, "an input");
+    k::PackedAttention p;
+    p.tokens = to_int(query->shape[0], "query tokens");
+    p.keys = to_int(key->shape[0], "key tokens");
+    p.sequences = to_int(query_starts->shape[0] - 1, "sequences");
+    p.qh = to_int(query->shape[1], "query heads");
+    p.kvh = to_int(key->shape[1], "KV heads");
+    p.hd = to_int(query->shape[2], "head dim");
+    if (p.sequences > 0xFFFFFF)
+      fail(MI_ERR_SHAPE, "invalid tensor shape: more than 2^24 sequences");
+    if (p.tokens == 0 || p.sequences == 0) return;
+    DeviceScope device(ctx);
+    p.q = query->f16();
+    p.k = key->f16();
+    p.v = value->f16();
+    p.out = out->f16();
+    p.query_starts = query_starts->u32();
+    p.key_starts = key_starts->u32();
+    p.fault = ctx->fault;
+    p.causal = causal != 0;
+    ProfileScope ps(ctx, "packed_attention");
+    k::packed_attention(launch_of(ctx), p);
+  });
+}
+
+mi_status mi_batch_sample(mi_batch* b, const mi_tensor* logits, const mi_tensor* temperature,
+                          const mi_tensor* top_k, const mi_tensor* top_p, const mi_tensor* min_p,
+                          const mi_tensor* uniform, mi_tensor* tokens) {
+  return guard([&] {
+    mi_context* ctx = ctx_of(b);
+    require_tensor(ctx, logits, MI_F16, 2, "logits");
+    require_tensor(ctx, temperature, MI_F32, 1, "temperature");
+    require_tensor(ctx, top_k, MI_U32, 1, "top_k");
+    require_tensor(ctx, top_p, MI_F32, 1, "top_p");
+    require_tensor(ctx, min_p, MI_F32, 1, "min_p");
+    require_tensor(ctx, uniform, MI_F32, 1, "uniform");
+    require_tensor(ctx, tokens, MI_U32, 1, "tokens");
+    const size_t rows = logits->shape[0], n = logits->shape[1];
+    for (const mi_tensor* t : {temperature, top_k, top_p, min_p, uniform, (const mi_tensor*)tokens}) {
+      require_shape(t, {rows}, "a per-row tensor");
+      require_aligned(t, 4, "a per-row tensor");
+      if (t != tokens) require_apart(tokens, t, "an input");
+    }
+    require_aligned(logits, 2, "logits");
+    require_apart(tokens, logits, "the logits");
+    if (n == 0 || n > (size_t)k::kSampleBatchMax)
+      fail(MI_ERR_SHAPE, "invalid tensor shape: sampling takes 1 to %d logits a row, got %zu",
+           k::kSampleBatchMax, n);
+    if (rows > 0xFFFFFFull) fail(MI_ERR_SHAPE, "invalid tensor shape: more than 2^24 rows");
+    if (rows == 0) return;
+    DeviceScope device(ctx);
+    k::SampleBatch p;
+    p.logits = logits->f16();
+    p.temperature = temperature->f32();
+    p.top_k = top_k->u32();
+    p.top_p = top_p->f32();
+    p.min_p = min_p->f32();
+    p.uniform = uniform->f32();
+    p.tokens = tokens->u32();
+    p.fault = ctx->fault;
+    p.rows = (int)rows;
+    p.n = (int)n;
+    ProfileScope ps(ctx, "sample_batch");
+    k::sample_batch(launch_of(ctx), p);
+  });
+}
+
+}  // extern "C"

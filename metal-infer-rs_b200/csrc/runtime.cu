@@ -63,6 +63,7 @@ void context_release(mi_context* ctx) {
   }
   if (ctx->scratch) cudaFreeAsync(ctx->scratch, ctx->stream);
   cudaStreamSynchronize(ctx->stream);
+  if (ctx->fault) cudaFreeHost(ctx->fault);
   cudaStreamDestroy(ctx->stream);
   delete ctx;
 }
@@ -136,6 +137,28 @@ void check_device_waits(const char* what) {
   if (unsigned code = take_device_wait_status())
     fail(MI_ERR_TIMEOUT, "%s: a bounded device wait expired (code 0x%x); the results are not valid",
          what, code);
+}
+
+void check_device_arguments(mi_context* ctx) {
+  const uint32_t code = *reinterpret_cast<volatile uint32_t*>(ctx->fault);
+  if (!code) return;
+  *reinterpret_cast<volatile uint32_t*>(ctx->fault) = 0;
+  switch (code) {
+    case k::kFaultStarts:
+      fail(MI_ERR_INVALID_ARGUMENT,
+           "starts do not rise or leave their rows; the results are not valid");
+    case k::kFaultLength:
+      fail(MI_ERR_INVALID_ARGUMENT,
+           "a length does not fit its page table or its tokens; the results are not valid");
+    case k::kFaultPage:
+      fail(MI_ERR_INVALID_ARGUMENT,
+           "a page table names a page outside of the cache; the results are not valid");
+    case k::kFaultSampling:
+      fail(MI_ERR_CONFIG,
+           "invalid model configuration: sampling options outside of their ranges");
+    default:
+      fail(MI_ERR_COMMAND, "a kernel refused its arguments (code %u)", code);
+  }
 }
 
 ProfileScope::ProfileScope(mi_context* c, const char* n) : ctx(c), name(n) {
@@ -243,6 +266,14 @@ mi_status mi_context_create(int device, mi_context** out) {
       delete ctx;
       fail(MI_ERR_RESOURCE, "stream creation failed: %s", cudaGetErrorString(err));
     }
+    err = cudaHostAlloc(&ctx->fault, sizeof(uint32_t),
+                        cudaHostAllocMapped | cudaHostAllocPortable);
+    if (err != cudaSuccess) {
+      cudaStreamDestroy(ctx->stream);
+      delete ctx;
+      fail(MI_ERR_RESOURCE, "host allocation failed: %s", cudaGetErrorString(err));
+    }
+    *ctx->fault = 0;
     // Keep freed stream-ordered memory in the pool (no release to the OS
     // between steps).
     cudaMemPool_t pool;
@@ -324,6 +355,7 @@ mi_status mi_context_kernel_status(mi_context* ctx, uint32_t* code) {
     require_ctx(code, "code");
     sync_context(ctx);
     *code = take_device_wait_status();
+    if (*code == 0) check_device_arguments(ctx);
   });
   if (st == MI_OK && *code != 0) {
     set_error("a bounded device wait expired (code %u)", *code);
@@ -631,10 +663,15 @@ mi_status mi_pending_wait(mi_pending* p, mi_dispatch_stats* stats) {
     auto wall = std::chrono::steady_clock::now() - p->wall_start;
     cudaEventDestroy(p->start);
     cudaEventDestroy(p->stop);
-    context_release(p->ctx);
+    // the context stays until the checks below have read it
+    struct Release {
+      mi_context* ctx;
+      ~Release() { context_release(ctx); }
+    } release{p->ctx};
     delete p;
     if (err != cudaSuccess) fail(MI_ERR_COMMAND, "command failed: %s", cudaGetErrorString(err));
     check_device_waits("batch");
+    check_device_arguments(release.ctx);
     if (stats) {
       stats->gpu_time = ms * 1e-3;
       stats->wall_time = std::chrono::duration<double>(wall).count();

@@ -82,6 +82,10 @@ class QkNormRopeCacheConfig(ctypes.Structure):
                 ("epsilon", ctypes.c_float)]
 
 
+class PagedRope(ctypes.Structure):
+    _fields_ = [("theta", ctypes.c_float), ("epsilon", ctypes.c_float)]
+
+
 class DispatchStats(ctypes.Structure):
     _fields_ = [("gpu_time", ctypes.c_double), ("wall_time", ctypes.c_double)]
 
@@ -197,7 +201,8 @@ EXPORTS = [
     "mi_batch_add_rms_norm", "mi_batch_swiglu", "mi_batch_embedding", "mi_batch_argmax",
     "mi_batch_rope", "mi_batch_qk_norm_rope_cache", "mi_batch_attention",
     "mi_batch_attention_flash_decode_with_configuration", "mi_batch_copy_into_cache",
-    "mi_attention_flash_decode_noalloc",
+    "mi_attention_flash_decode_noalloc", "mi_batch_paged_append", "mi_batch_paged_attention",
+    "mi_batch_packed_attention", "mi_batch_sample",
     "mi_qwen3_config_validate", "mi_qwen3_create_random", "mi_qwen3_load", "mi_qwen3_destroy",
     "mi_qwen3_get_config", "mi_qwen3_set_attention_kind", "mi_qwen3_set_fusion_options",
     "mi_qwen3_fusion_options", "mi_qwen3_set_decode_graphs",
@@ -245,6 +250,10 @@ def lib() -> ctypes.CDLL:
                  "mi_pending_is_complete"):
         getattr(L, name).argtypes = [_vp]
     L.mi_tensor_shape.argtypes = [_vp, _szp, _sz]
+    L.mi_batch_paged_append.argtypes = [_vp] * 12 + [PagedRope]
+    L.mi_batch_paged_attention.argtypes = [_vp] * 7
+    L.mi_batch_packed_attention.argtypes = [_vp] * 6 + [ctypes.c_int, _vp]
+    L.mi_batch_sample.argtypes = [_vp] * 8
     L.mi_qwen3_fusion_options.restype = FusionOptions
     L.mi_qwen3_fusion_options.argtypes = [_vp]
     _lib = L
@@ -541,6 +550,10 @@ class PendingBatch:
             pass
 
 
+def _optional(t: Optional[Tensor]):
+    return None if t is None else t.handle
+
+
 class CommandBatch:
     """CommandBatch (context.rs:155-1045) and its ops (ops.rs:221-1285)."""
 
@@ -626,6 +639,39 @@ class CommandBatch:
 
     def copy_into_cache(self, source, cache, offset):
         _check(lib().mi_batch_copy_into_cache(self._h, source.handle, cache.handle, _sz(offset)))
+
+    # ragged batches (include/mi.h): outputs are tensors of the caller
+    def paged_append(self, query: Optional[Tensor], key: Tensor, value: Tensor,
+                     query_weight: Optional[Tensor], key_weight: Optional[Tensor], starts: Tensor,
+                     lengths: Tensor, table: Tensor, key_cache: Tensor, value_cache: Tensor,
+                     query_out: Optional[Tensor], theta: float, epsilon: float = 1e-6) -> None:
+        """Per-head RMSNorm (with weights) and RoPE of a packed batch's queries and
+        keys, and the append of keys and values to their pages."""
+        _check(lib().mi_batch_paged_append(
+            self._h, _optional(query), key.handle, value.handle,
+            _optional(query_weight), _optional(key_weight), starts.handle,
+            lengths.handle, table.handle, key_cache.handle, value_cache.handle,
+            _optional(query_out), PagedRope(theta, epsilon)))
+
+    def paged_attention(self, query: Tensor, key_cache: Tensor, value_cache: Tensor,
+                        lengths: Tensor, table: Tensor, out: Tensor) -> None:
+        """Attention of one new token per sequence over its pages."""
+        _check(lib().mi_batch_paged_attention(self._h, query.handle, key_cache.handle,
+                                              value_cache.handle, lengths.handle, table.handle,
+                                              out.handle))
+
+    def packed_attention(self, query: Tensor, key: Tensor, value: Tensor, query_starts: Tensor,
+                         key_starts: Tensor, causal: bool, out: Tensor) -> None:
+        """Attention over packed prompts of different lengths."""
+        _check(lib().mi_batch_packed_attention(self._h, query.handle, key.handle, value.handle,
+                                               query_starts.handle, key_starts.handle, int(causal),
+                                               out.handle))
+
+    def sample(self, logits: Tensor, temperature: Tensor, top_k: Tensor, top_p: Tensor,
+               min_p: Tensor, uniform: Tensor, tokens: Tensor) -> None:
+        """One token per row of logits under that row's options."""
+        _check(lib().mi_batch_sample(self._h, logits.handle, temperature.handle, top_k.handle,
+                                     top_p.handle, min_p.handle, uniform.handle, tokens.handle))
 
 
 # ---- model ---------------------------------------------------------------------------

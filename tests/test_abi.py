@@ -56,3 +56,12 @@ def test_config_validation_matches_reference_rules():
     assert mi.lib().mi_qwen3_config_validate(ctypes.byref(bad)) == mi.ERR_CONFIG
     bad = mi.Qwen3Config.from_dict(dict(mi.QWEN3_0_6B, num_key_value_heads=3))
     assert mi.lib().mi_qwen3_config_validate(ctypes.byref(bad)) == mi.ERR_CONFIG
+
+
+def test_batched_ops_refuse_null_arguments():
+    lib = mi.lib()
+    assert lib.mi_batch_paged_append(*[None] * 12, mi.PagedRope(1e6, 1e-6)) == mi.ERR_INVALID_ARGUMENT
+    assert b"batch is NULL" in lib.mi_last_error_message()
+    assert lib.mi_batch_paged_attention(*[None] * 7) == mi.ERR_INVALID_ARGUMENT
+    assert lib.mi_batch_packed_attention(*[None] * 6, 1, None) == mi.ERR_INVALID_ARGUMENT
+    assert lib.mi_batch_sample(*[None] * 8) == mi.ERR_INVALID_ARGUMENT
