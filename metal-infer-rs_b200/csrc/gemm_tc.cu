@@ -526,6 +526,25 @@ bool persistent_enabled() {
 
 bool gemm_tc_available() { return enabled() && encoder() != nullptr; }
 
+bool make_f16_map(void* map, const __half* ptr, int rank, const uint64_t* dims,
+                  const uint32_t* box) {
+  EncodeTiled enc = encoder();
+  if (!enc) return false;
+  cuuint64_t d[5], strides[4];
+  cuuint32_t b[5], elem[5] = {1, 1, 1, 1, 1};
+  cuuint64_t bytes = 2;
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    bytes *= dims[i];
+    if (i + 1 < rank) strides[i] = bytes;
+  }
+  return enc(static_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
+             const_cast<__half*>(ptr), d, strides, b, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool make_kv_tile_map(void* map, const __half* cache, int capacity, int kv_heads, int box_rows) {
   EncodeTiled enc = encoder();
   if (!enc) return false;

@@ -131,6 +131,11 @@ bool gemm_tc_available();
 // swizzled (rows past the capacity read as zeros). False when the driver's
 // encoder is unavailable.
 bool make_kv_tile_map(void* map, const __half* cache, int capacity, int kv_heads, int box_rows);
+// A 128-byte-swizzled tensor map over a dense FP16 tensor of `rank` (at most
+// 5) dimensions, innermost first; box[0] is 64. False when it cannot be
+// encoded.
+bool make_f16_map(void* map, const __half* ptr, int rank, const uint64_t* dims,
+                  const uint32_t* box);
 
 // ---- row / elementwise kernels ---------------------------------------------
 void add(const Launch& l, const __half* a, const __half* b, __half* out, size_t n);
@@ -224,7 +229,8 @@ enum Fault : uint32_t {
   kFaultStarts = 1,   // starts that do not rise, or leave the rows
   kFaultLength = 2,   // a length its page table cannot hold, or below the appended tokens
   kFaultPage = 3,     // a page id outside of the cache
-  kFaultSampling = 4  // sampling options outside of their ranges
+  kFaultSampling = 4, // sampling options outside of their ranges
+  kFaultTimeout = 5   // a bounded wait expired (nothing refused: an engine error)
 };
 // Q/K norm (with weights), RoPE and the append to pages of a packed batch:
 // sequence s holds tokens [starts[s], starts[s + 1]), the last of them at

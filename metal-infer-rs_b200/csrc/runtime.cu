@@ -156,6 +156,8 @@ void check_device_arguments(mi_context* ctx) {
     case k::kFaultSampling:
       fail(MI_ERR_CONFIG,
            "invalid model configuration: sampling options outside of their ranges");
+    case k::kFaultTimeout:
+      fail(MI_ERR_TIMEOUT, "a bounded device wait expired; the results are not valid");
     default:
       fail(MI_ERR_COMMAND, "a kernel refused its arguments (code %u)", code);
   }
