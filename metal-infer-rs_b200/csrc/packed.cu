@@ -6,27 +6,31 @@
 //
 // Tensor-bound: 4 d operations per visible (query, key) pair and head on the
 // tcgen05 pipe, with the exponentials (16 per clock and SM) close behind at
-// head_dim 128 and ahead of it at 64.
+// head_dim 128 and ahead of it at 64; half of them run as polynomials on the
+// FMA pipe.
 //
 // A CTA takes two row tiles of one sequence and KV head. The rows of a tile
 // are the query heads of the group for up to 128 / group tokens, so a short
 // prompt still fills a tile and a key tile is read once for the whole group.
-// Roles:
+// Roles (warps 10 and 11 only fill their warpgroup; registers go from the last
+// warpgroup to the softmax):
 //   warps 0-3, 4-7  softmax of row tile 0 / 1, one row to a thread: scores from
 //                   TMEM, the running maximum and sum in registers, FP16
-//                   weights back to TMEM over the scores; in the end the output
-//   warp 8          one thread issues tcgen05.mma: S_t = Q_t K^T from shared
-//                   memory, O_t += P_t V with P from TMEM. The tiles alternate,
-//                   so one tile's products run while the other's softmax does
-//   warp 9          TMA: the query tiles once, then K and V tiles of 128 keys
-//                   through one ring
-// TMEM: S_0, S_1 (128 columns each, P over them), O_0, O_1.
+//                   weights to TMEM; in the end the output
+//   warp 8          tcgen05.mma: S_t = Q_t K^T from shared memory, O_t += P_t V
+//                   with P from TMEM
+//   warp 9          TMA: the query tiles once, then K and V tiles through a ring
+// TMEM holds S, P and O of both tiles with P beside S, so the next key tile's
+// scores are computed while the softmax of this one runs and the products
+// leave its chain: 80 keys to a tile at head_dim 128 (2 (80 + 40 + 128)
+// columns of 512), 128 at 64. With P over S and 128 keys the chain scores ->
+// softmax -> values took 3,460 clocks to a tile (a hand-over between the
+// roles is 150 to 370 of them) where the products take 1,024.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the
 // last time (weights then stay below 2^8, far inside FP16, and the final
-// division by the sum of the same weights takes the factor out); s_full of
-// step i says that the product of step i - 1 is done, as its commit covers all
-// earlier products, so the row's own thread may rescale O in TMEM.
+// division by the sum of the same weights takes the factor out), once the
+// product of the step before is done.
 
 #include <cuda.h>
 
@@ -38,9 +42,10 @@ namespace k {
 
 namespace {
 
-constexpr int kTile = 128;     // rows of a row tile, keys of a key tile
-constexpr int kThreads = 320;
+constexpr int kTile = 128;     // rows of a row tile
+constexpr int kThreads = 384;
 constexpr uint64_t kWaitNs = 200ull * 1000 * 1000;
+constexpr int kPolyOf4 = 2;    // of four pairs of weights, those on the FMA pipe
 constexpr float kGrowth = 8.f; // log2 of the weights' largest value
 
 struct PackedArgs {
@@ -57,10 +62,17 @@ struct PackedArgs {
 };
 
 template <int HD>
-struct PackedSmem {
-  static constexpr int kTileBytes = kTile * HD * 2;
-  static constexpr int kSlots = HD == 128 ? 5 : 10;  // K and V tiles of the ring
-  static constexpr int kBytes = 1024 /*align*/ + (2 + kSlots) * kTileBytes + 512;
+struct Packed {
+  static constexpr int kKeys = HD == 128 ? 80 : 128;  // of a key tile
+  static constexpr uint32_t kQBytes = kTile * HD * 2;
+  static constexpr uint32_t kSlotBytes = kKeys * HD * 2;
+  static constexpr int kSlots = 8;  // K and V tiles of the ring
+  static constexpr int kBytes = 1024 /*align*/ + 2 * kQBytes + kSlots * kSlotBytes + 512;
+  // TMEM columns
+  static constexpr uint32_t kS = HD == 128 ? 128 : 192;  // S_1's distance from S_0, which is at 0
+  static constexpr uint32_t kP = kKeys;                  // P's distance from its S
+  static constexpr uint32_t kO = HD == 128 ? 256 : 384;  // O_0; O_1 is HD further
+  static_assert(kP + kKeys / 2 <= kS && kS + kP + kKeys / 2 <= kO && kO + 2 * HD <= 512, "TMEM");
 };
 
 // One row by one warp, from the formula, over the first `visible` keys and
@@ -124,10 +136,12 @@ __device__ __forceinline__ void fence_before() {
 __device__ __forceinline__ void fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-__device__ __forceinline__ void commit(uint64_t* bar) {
+__device__ __forceinline__ void commit(uint64_t* bar, bool one) {
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-          pipe::smem_u32(bar))
+      "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(
+          pipe::smem_u32(bar)),
+      "r"((uint32_t)one)
       : "memory");
 }
 __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0,
@@ -147,59 +161,78 @@ __device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, uint64
       "r"(c3)
       : "memory");
 }
-// Shared-memory matrix descriptor of a 128-byte-swizzled operand (version 1):
-// K-major (Q, K: rows of 64 values of the product's depth), 8-row groups 1024
-// bytes apart; MN-major (V: rows are keys, the depth; 64 values of N to a row),
-// the next 64 values of N `lead` bytes on, the next 8 keys 1024 bytes on.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lead) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Shared-memory matrix descriptor of a 128-byte-swizzled operand (version 1),
+// low and high word: K-major (Q, K: rows of 64 values of the product's depth),
+// 8-row groups 1024 bytes apart; MN-major (V: rows are keys, the depth; 64
+// values of N to a row), the next 64 values of N `lead` bytes on, the next 8
+// keys 1024 bytes on. A step inside the operand adds its bytes / 16.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lead) {
+  return (addr >> 4) | ((lead >> 4) << 16);
 }
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
 // Instruction descriptor of kind::f16: F16 operands, F32 result, M = 128.
 __host__ __device__ constexpr uint32_t idesc_f16(int n, bool b_mn_major) {
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
+// The products are issued by a warp that runs their loop as a whole, `one` set
+// in one lane: operands of tcgen05.mma live in uniform registers, and a loop
+// that one lane runs alone moves each of them there every time (95 clocks to a
+// product where the tensor cores take 64).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
+                                       bool accumulate, bool one) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .b64 x, y;\n"
+      " setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+      " mov.b64 x, {%1, %6};\n mov.b64 y, {%2, %6};\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"((uint32_t)accumulate), "r"((uint32_t)one),
+      "n"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc,
+                                       bool accumulate, bool one) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p, q;\n .reg .b64 y;\n"
+      " setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+      " mov.b64 y, {%2, %6};\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(idesc), "r"((uint32_t)accumulate), "r"((uint32_t)one), "n"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t (&r)[32], uint32_t addr) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
-      "%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr));
+// 16 or 32 columns of a thread's TMEM lane; r is an array indexed by constants.
+__device__ __forceinline__ void tmem_ld16(uint32_t* r, uint32_t addr) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
-      "%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(
-          addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
-      "r"(r[30]), "r"(r[31])
-      : "memory");
+__device__ __forceinline__ void tmem_ld32(uint32_t* r, uint32_t addr) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// Ties loaded registers to this point, so that no use moves above the wait.
+__device__ __forceinline__ void tie16(uint32_t* r) {
+  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
+__device__ __forceinline__ void tie32(uint32_t* r) {
+  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -208,6 +241,54 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two FP32 lanes in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two values on the FMA pipe, x <= 126: x = n + f with n the nearest
+// integer (the low bits of x + 1.5 2^23), 2^f by a degree-4 polynomial (least
+// largest relative error on [-1/2, 1/2], fitted: 2.6e-6), n added to the
+// exponent. x is held at -126 from below, whose power FP16 rounds to 0.
+__device__ __forceinline__ void exp2_poly2(uint64_t x, float& lo, float& hi) {
+  float a, b;
+  split(x, a, b);
+  x = pair_of(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t magic = pair_of(12582912.f, 12582912.f);
+  const uint64_t t = add2(x, magic);
+  const uint64_t n = add2(t, pair_of(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, pair_of(-1.f, -1.f), x);
+  uint64_t p = pair_of(0.009570101276f, 0.009570101276f);
+  p = fma2(p, f, pair_of(0.05591785908f, 0.05591785908f));
+  p = fma2(p, f, pair_of(0.2402474433f, 0.2402474433f));
+  p = fma2(p, f, pair_of(0.6931217909f, 0.6931217909f));
+  p = fma2(p, f, pair_of(0.9999992847f, 0.9999992847f));
+  float ta, tb;
+  split(p, a, b);
+  split(t, ta, tb);
+  lo = __int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23));
+  hi = __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23));
 }
 
 // What a CTA works on.
@@ -223,20 +304,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     packed_kernel(const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const PackedArgs a) {
-  using S = PackedSmem<HD>;
-  constexpr int kSlots = S::kSlots;
-  constexpr uint32_t kTileBytes = S::kTileBytes;
+  using C = Packed<HD>;
+  constexpr int kSlots = C::kSlots, kKeys = C::kKeys;
   constexpr int kHalves = HD / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint8_t* ring = smem + 2 * kTileBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kSlots * kTileBytes);
-  uint64_t* q_full = bars;            // [1]
-  uint64_t* s_full = bars + 1;        // [2] scores are in TMEM
-  uint64_t* p_full = bars + 3;        // [2] weights are in TMEM
-  uint64_t* o_full = bars + 5;        // [2] the last product is done
-  uint64_t* kv_full = bars + 7;       // [kSlots]
+  uint8_t* ring = smem + 2 * C::kQBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kSlots * C::kSlotBytes);
+  uint64_t* q_full = bars;         // [1]
+  uint64_t* s_full = bars + 1;     // [2] scores are in TMEM
+  uint64_t* s_free = bars + 3;     // [2] and have been read
+  uint64_t* p_full = bars + 5;     // [2] weights are in TMEM
+  uint64_t* o_full = bars + 7;     // [2] their product is done
+  uint64_t* kv_full = bars + 9;    // [kSlots]
   uint64_t* kv_empty = kv_full + kSlots;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kSlots);
   Work* work = reinterpret_cast<Work*>(tmem_slot + 2);
@@ -286,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int last = min(n, w.token + (i + 1) * a.span) - 1;  // last token of the row tile
         if (last < w.token + i * a.span) continue;
         const long long seen = a.causal ? (long long)w.keys - (n - 1 - last) : w.keys;
-        w.blocks[i] = seen > 0 ? (int)((seen + kTile - 1) / kTile) : 0;
+        w.blocks[i] = seen > 0 ? (int)((seen + kKeys - 1) / kKeys) : 0;
       }
     } else {
       w.token = -1;
@@ -295,6 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     pipe::mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
       pipe::mbar_init(s_full + i, 1);
+      pipe::mbar_init(s_free + i, 4);
       pipe::mbar_init(p_full + i, 4);
       pipe::mbar_init(o_full + i, 1);
     }
@@ -319,26 +401,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t tmem_o = tmem + 2 * kTile;
 
-  if (warp == 9) {
+  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp >= 10) {
+    // no role
+  } else if (warp == 9) {
     if (lane == 0 && blocks > 0) {
       // ---- TMA ------------------------------------------------------------------
       pipe::mbar_expect_tx(q_full, 2u * kHalves * a.heads * a.span * 128u);
       for (int t = 0; t < 2; ++t)
         for (int h = 0; h < kHalves; ++h)
-          tma_4d(smem + t * kTileBytes + h * (kTile * 128), &map_q, q_full, h * 64, head0, kv,
+          tma_4d(smem + t * C::kQBytes + h * (kTile * 128), &map_q, q_full, h * 64, head0, kv,
                  w.q0 + w.token + t * a.span);
-      bool ok = true;
+      // in the order of use: K_0, K_1, V_0, K_2, V_1, ..., V_last
       int n = 0;
-      for (; n < 2 * blocks && ok; ++n) {
+      for (; n < 2 * blocks; ++n) {
         const int slot = n % kSlots;
-        ok = wait_for(kv_empty + slot, ((n / kSlots) & 1) ^ 1, a.fault);
-        if (!ok) break;
-        pipe::mbar_expect_tx(kv_full + slot, kTileBytes);
+        if (!wait_for(kv_empty + slot, ((n / kSlots) & 1) ^ 1, a.fault)) break;
+        const bool is_v = n == 2 * blocks - 1 || (n > 0 && n % 2 == 0);
+        const int tile = n == 2 * blocks - 1 ? blocks - 1 : is_v ? n / 2 - 1 : (n + 1) / 2;
+        pipe::mbar_expect_tx(kv_full + slot, C::kSlotBytes);
         for (int h = 0; h < kHalves; ++h)
-          tma_3d(ring + slot * kTileBytes + h * (kTile * 128), n & 1 ? &map_v : &map_k,
-                 kv_full + slot, h * 64, kv, w.k0 + (n >> 1) * kTile);
+          tma_3d(ring + slot * C::kSlotBytes + h * (kKeys * 128), is_v ? &map_v : &map_k,
+                 kv_full + slot, h * 64, kv, w.k0 + tile * kKeys);
       }
       // the copies land before the CTA leaves
       wait_for(q_full, 0, a.fault);
@@ -346,141 +431,185 @@ __global__ void __launch_bounds__(kThreads, 1)
         wait_for(kv_full + i % kSlots, (i / kSlots) & 1, a.fault);
     }
   } else if (warp == 8) {
-    if (lane == 0 && blocks > 0) {
+    if (blocks > 0) {
       // ---- products -----------------------------------------------------------------
-      constexpr uint32_t idesc_s = idesc_f16(kTile, false);
+      constexpr uint32_t idesc_s = idesc_f16(kKeys, false);
       constexpr uint32_t idesc_o = idesc_f16(HD, true);
+      const bool one = elect_one();
+      const uint32_t q_lo = desc_lo(pipe::smem_u32(smem), 16);
+      const uint32_t k_lo = desc_lo(pipe::smem_u32(ring), 16);
+      const uint32_t v_lo = desc_lo(pipe::smem_u32(ring), kKeys * 128);
+      const int blocks0 = __shfl_sync(0xffffffffu, w.blocks[0], 0);
+      const int blocks1 = __shfl_sync(0xffffffffu, w.blocks[1], 0);
       auto scores = [&](int t, int slot) {
-        const uint32_t qa = pipe::smem_u32(smem + t * kTileBytes);
-        const uint32_t ka = pipe::smem_u32(ring + slot * kTileBytes);
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = (kk / 4) * (kTile * 128) + (kk % 4) * 32;
-          mma_ss(tmem + t * kTile, desc_sw128(qa + off, 16), desc_sw128(ka + off, 16), idesc_s,
-                 kk != 0);
-        }
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_ss(tmem + t * C::kS,
+                 q_lo + (t * C::kQBytes + (kk / 4) * (kTile * 128) + (kk % 4) * 32) / 16,
+                 k_lo + (slot * C::kSlotBytes + (kk / 4) * (kKeys * 128) + (kk % 4) * 32) / 16,
+                 idesc_s, kk != 0, one);
+        commit(s_full + t, one);
+      };
+      auto values = [&](int t, int slot, bool more) {
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          mma_ts(tmem + C::kO + t * HD, tmem + t * C::kS + C::kP + kk * 8,
+                 v_lo + (slot * C::kSlotBytes + kk * 2048) / 16, idesc_o, more || kk != 0, one);
+        commit(o_full + t, one);
+      };
+      // the next ring slot and its phase
+      int slot = 0;
+      uint32_t phase = 0;
+      auto next = [&] {
+        if (++slot == kSlots) slot = 0, phase ^= 1;
       };
       bool ok = wait_for(q_full, 0, a.fault) && wait_for(kv_full, 0, a.fault);
       if (ok) {
         fence_after();
-        for (int t = 0; t < 2; ++t)
-          if (w.blocks[t] > 0) {
-            scores(t, 0);
-            commit(s_full + t);
-          }
-        commit(kv_empty);
+        if (blocks0 > 0) scores(0, 0);
+        if (blocks1 > 0) scores(1, 0);
+        commit(kv_empty, one);
       }
+      next();
       for (int i = 0; i < blocks && ok; ++i) {
-        const int nv = 2 * i + 1, nk = 2 * i + 2;
-        const int sv = nv % kSlots, sk = nk % kSlots;
-        ok = wait_for(kv_full + sv, (nv / kSlots) & 1, a.fault);
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (i < w.blocks[t]) {
-            ok = wait_for(p_full + t, i & 1, a.fault);
-            if (!ok) break;
-            fence_after();
-            const uint32_t va = pipe::smem_u32(ring + sv * kTileBytes);
+        const bool more = i + 1 < blocks;
+        int sk = slot;
+        if (more) {
+          ok = wait_for(kv_full + slot, phase, a.fault);
+          next();
+        }
+        const int sv = slot;
+        ok = ok && wait_for(kv_full + slot, phase, a.fault);
+        next();
 #pragma unroll
-            for (int kk = 0; kk < kTile / 16; ++kk)
-              mma_ts(tmem_o + t * HD, tmem + t * kTile + kk * 8,
-                     desc_sw128(va + kk * 2048, kTile * 128), idesc_o, (i | kk) != 0);
-            if (i + 1 == w.blocks[t]) commit(o_full + t);
-          }
-          if (t == 1) commit(kv_empty + sv);
-          if (i + 1 < w.blocks[t]) {
-            ok = wait_for(kv_full + sk, (nk / kSlots) & 1, a.fault);
-            if (!ok) break;
+        for (int t = 0; t < 2; ++t) {
+          const int mine = t ? blocks1 : blocks0;
+          if (i + 1 < mine && ok) {
+            ok = wait_for(s_free + t, i & 1, a.fault);
             fence_after();
-            scores(t, sk);
-            commit(s_full + t);
+            if (ok) scores(t, sk);
+          }
+          if (t == 1 && more) commit(kv_empty + sk, one);
+          if (i < mine && ok) {
+            ok = wait_for(p_full + t, i & 1, a.fault);
+            fence_after();
+            if (ok) values(t, sv, i != 0);
           }
         }
-        if (ok && i + 1 < blocks) commit(kv_empty + sk);
+        commit(kv_empty + sv, one);
       }
     }
   } else {
     // ---- softmax -------------------------------------------------------------------
+    // 8 warps of 208 and 4 of 88 registers: the launch's 12 of 168
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2;                // row tile
     const int row = (warp & 3) * 32 + lane; // of the tile: the TMEM lane
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + t * kTile;
-    const uint32_t to = tmem_o + lanes + t * HD;
+    const uint32_t ts = tmem + lanes + t * C::kS;
+    const uint32_t tp = ts + C::kP;
+    const uint32_t to = tmem + lanes + C::kO + t * HD;
     const int n = w.q1 - w.q0;
     const int token = w.token + t * a.span + row / a.heads;
     const int head = head0 + row % a.heads;
     const bool valid = row < a.heads * a.span && token < n && head < a.group;
-    long long seen = a.causal ? (long long)w.keys - (n - 1 - token) : w.keys;
+    const long long seen = a.causal ? (long long)w.keys - (n - 1 - token) : w.keys;
     const int visible = valid && seen > 0 ? (int)seen : 0;
     // keys that every row of the tile sees
     const long long least =
         a.causal ? (long long)w.keys - (n - 1 - (w.token + t * a.span)) : w.keys;
     const int mine = w.blocks[t];
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY;
+    uint64_t l2 = 0;  // two partial sums
+    const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2);
     bool ok = true;
     for (int i = 0; i < mine; ++i) {
       ok = wait_for(s_full + t, i & 1, a.fault);
       if (!ok) break;
       fence_after();
-      uint32_t s[4][32];
+      uint32_t s[kKeys];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s[c], ts + c * 32);
+      for (int c = 0; c + 32 <= kKeys; c += 32) tmem_ld32(s + c, ts + c);
+      if constexpr (kKeys % 32 != 0) tmem_ld16(s + kKeys - 16, ts + kKeys - 16);
       tmem_wait_ld();
-      const int k0 = i * kTile;
-      if (k0 + kTile > least) {
+#pragma unroll
+      for (int c = 0; c + 32 <= kKeys; c += 32) tie32(s + c);
+      if constexpr (kKeys % 32 != 0) tie16(s + kKeys - 16);
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(s_free + t);
+      const int k0 = i * kKeys;
+      if (k0 + kKeys > least) {
         const int left = visible - k0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (c * 32 + e >= left) s[c][e] = 0xff800000u;  // -inf
+        for (int e = 0; e < kKeys; ++e)
+          if (e >= left) s[e] = 0xff800000u;  // -inf
       }
-      float top = -INFINITY;
+      // a NaN or +inf that the row sees ends in the maximum
+      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(s[c][e]));
-      top *= a.scale_log2;
+      for (int e = 0; e < kKeys; e += 2)
+        tops[(e >> 1) & 3] = max3_nan(tops[(e >> 1) & 3], __uint_as_float(s[e]),
+                                      __uint_as_float(s[e + 1]));
+      float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], -INFINITY) * a.scale_log2;
+      if (!(top < INFINITY)) {  // the row ends as NaN, and is done again below
+        l2 = pair_of(__int_as_float(0x7fc00000), 0.f);
+        top = m;
+      }
       // a maximum that grew past the bound moves the row's base
       const bool grown = top > m + kGrowth || (m == -INFINITY && top > m);
       if (__any_sync(0xffffffffu, grown)) {
-        const float next = grown ? top : m;
-        const float f = m == -INFINITY ? 0.f : exp2_fast(m - next);
-        const float factor = grown ? f : 1.f;
-        m = next;
+        const float base = grown ? top : m;
+        const float factor = !grown ? 1.f : m == -INFINITY ? 0.f : exp2_fast(m - base);
+        m = base;
         if (i > 0) {
-          l *= factor;
+          l2 = fma2(l2, pair_of(factor, factor), 0);
+          ok = wait_for(o_full + t, (i - 1) & 1, a.fault);
+          if (!ok) break;
+          fence_after();
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
             uint32_t o[32];
             tmem_ld32(o, to + c);
             tmem_wait_ld();
+            tie32(o);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
             tmem_st32(to + c, o);
           }
-          tmem_wait_st();
         }
       }
       const float base = m == -INFINITY ? 0.f : -m;
+      const uint64_t base2 = pair_of(base, base);
+      uint32_t p[kKeys / 2];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          // weights rounded to FP16 for the product; the sum takes the rounded
-          // ones, so that it is the sum of what the product weighs
-          const float x0 = __uint_as_float(s[2 * c + (e >> 4)][2 * (e & 15)]);
-          const float x1 = __uint_as_float(s[2 * c + (e >> 4)][2 * (e & 15) + 1]);
-          const __half2 h = __floats2half2_rn(exp2_fast(fmaf(x0, a.scale_log2, base)),
-                                              exp2_fast(fmaf(x1, a.scale_log2, base)));
-          const uint32_t u = *reinterpret_cast<const uint32_t*>(&h);
-          l = fma_f16_f32((unsigned short)(u & 0xffffu), 0x3c00, l);
-          l = fma_f16_f32((unsigned short)(u >> 16), 0x3c00, l);
-          p[e] = u;
+      for (int e = 0; e < kKeys / 2; ++e) {
+        const uint64_t x = fma2(pair_of(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])),
+                                scale2, base2);
+        float w0, w1;
+        if (e % 4 < kPolyOf4) {
+          exp2_poly2(x, w0, w1);
+        } else {
+          split(x, w0, w1);
+          w0 = exp2_fast(w0);
+          w1 = exp2_fast(w1);
         }
-        tmem_st32(ts + c * 32, p);
+        // the sum takes the weights before their rounding to FP16, which is
+        // off by half a step at most and to either side
+        l2 = add2(l2, pair_of(w0, w1));
+        const __half2 h = __floats2half2_rn(w0, w1);
+        p[e] = *reinterpret_cast<const uint32_t*>(&h);
       }
+      // P is free once the product of the step before is done
+      if (i > 0) {
+        ok = wait_for(o_full + t, (i - 1) & 1, a.fault);
+        if (!ok) break;
+        fence_after();
+      }
+#pragma unroll
+      for (int c = 0; c + 32 <= kKeys / 2; c += 32) tmem_st32(tp + c, p + c);
+      if constexpr (kKeys % 64 != 0) tmem_st8(tp + kKeys / 2 - 8, p + kKeys / 2 - 8);
       tmem_wait_st();
       fence_before();
       __syncwarp();
@@ -489,15 +618,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- output ---------------------------------------------------------------------
     const size_t stride = (size_t)a.kvh * HD;
     const size_t at = ((size_t)(w.q0 + token) * a.qh + (size_t)kv * a.group + head) * HD;
-    if (mine > 0 && ok && wait_for(o_full + t, 0, a.fault)) {
+    if (mine > 0 && ok && wait_for(o_full + t, (mine - 1) & 1, a.fault)) {
       fence_after();
-      const float inv = 1.f / l;
+      float la, lb;
+      split(l2, la, lb);
+      const float inv = 1.f / (la + lb);
       bool odd = false;  // something that is not finite
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         uint32_t o[32];
         tmem_ld32(o, to + c);
         tmem_wait_ld();
+        tie32(o);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           uint4 v;
@@ -540,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <int HD>
 void launch_packed(const Launch& l, PackedArgs a) {
-  using S = PackedSmem<HD>;
+  using C = Packed<HD>;
   a.head_tiles = (a.group + kTile - 1) / kTile;
   a.heads = (a.group + a.head_tiles - 1) / a.head_tiles;
   a.span = kTile / a.heads;
@@ -548,18 +680,18 @@ void launch_packed(const Launch& l, PackedArgs a) {
   const uint64_t dq[4] = {(uint64_t)HD, (uint64_t)a.group, (uint64_t)a.kvh, (uint64_t)a.tokens};
   const uint32_t bq[4] = {64, (uint32_t)a.heads, 1, (uint32_t)a.span};
   const uint64_t dk[3] = {(uint64_t)HD, (uint64_t)a.kvh, (uint64_t)std::max(1, a.keys)};
-  const uint32_t bk[3] = {64, 1, (uint32_t)kTile};
+  const uint32_t bk[3] = {64, 1, (uint32_t)C::kKeys};
   if (!make_f16_map(&mq, a.q, 4, dq, bq) || !make_f16_map(&mk, a.k, 3, dk, bk) ||
       !make_f16_map(&mv, a.v, 3, dk, bk))
     fail(MI_ERR_KERNEL, "packed attention: tensor map encoding failed");
   auto kernel = packed_kernel<HD>;
-  allow_dynamic_smem(kernel, S::kBytes);
+  allow_dynamic_smem(kernel, C::kBytes);
   // a place for every pair of row tiles, whatever the lengths are
   const long long places = (long long)a.tokens / (2 * a.span) + a.sequences;
   if (places > 65535)
     fail(MI_ERR_SHAPE, "invalid tensor shape: %d tokens of %d sequences are too many for one call",
          a.tokens, a.sequences);
-  launch_kernel(l, dim3(a.kvh * a.head_tiles, (unsigned)places), dim3(kThreads), S::kBytes, kernel,
+  launch_kernel(l, dim3(a.kvh * a.head_tiles, (unsigned)places), dim3(kThreads), C::kBytes, kernel,
                 mq, mk, mv, a);
 }
 
