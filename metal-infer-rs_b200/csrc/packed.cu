@@ -6,20 +6,23 @@
 //
 // Tensor-bound: 4 d operations per visible (query, key) pair and head on the
 // tcgen05 pipe, with the exponentials (16 per clock and SM) close behind at
-// head_dim 128 and ahead of it at 64; half of them run as polynomials on the
-// FMA pipe.
+// head_dim 128 and ahead of it at 64; a quarter of them run as polynomials on
+// the FMA pipe (none 557 us, half 574, a quarter 532).
 //
 // A CTA takes two row tiles of one sequence and KV head. The rows of a tile
 // are the query heads of the group for up to 128 / group tokens, so a short
 // prompt still fills a tile and a key tile is read once for the whole group.
-// Roles (warps 10 and 11 only fill their warpgroup; registers go from the last
-// warpgroup to the softmax):
+// Roles (warp 11 only fills its warpgroup; registers go from the last warpgroup
+// to the softmax):
 //   warps 0-3, 4-7  softmax of row tile 0 / 1, one row to a thread: scores from
 //                   TMEM, the running maximum and sum in registers, FP16
 //                   weights to TMEM; in the end the output
-//   warp 8          tcgen05.mma: S_t = Q_t K^T from shared memory, O_t += P_t V
-//                   with P from TMEM
-//   warp 9          TMA: the query tiles once, then K and V tiles through a ring
+//   warps 8, 9      tcgen05.mma of row tile 0 / 1: S_t = Q_t K^T from shared
+//                   memory, O_t += P_t V with P from TMEM. A wait costs a warp
+//                   about 170 clocks even when it has nothing to wait for, so
+//                   each tile has an issuer, and K and V come under one barrier
+//   warp 10         TMA: the query tiles once, then a ring of stages, stage n
+//                   holding K tile n and V tile n - 1, which are used together
 // TMEM holds S, P and O of both tiles with P beside S, so the next key tile's
 // scores are computed while the softmax of this one runs and the products
 // leave its chain: 80 keys to a tile at head_dim 128 (2 (80 + 40 + 128)
@@ -45,7 +48,8 @@ namespace {
 constexpr int kTile = 128;     // rows of a row tile
 constexpr int kThreads = 384;
 constexpr uint64_t kWaitNs = 200ull * 1000 * 1000;
-constexpr int kPolyOf4 = 2;    // of four pairs of weights, those on the FMA pipe
+constexpr int kLeadBlocks = 4; // key tiles from which row tile 1 starts after row tile 0
+constexpr int kPolyOf4 = 1;    // of four pairs of weights, those on the FMA pipe
 constexpr float kGrowth = 8.f; // log2 of the weights' largest value
 
 struct PackedArgs {
@@ -65,9 +69,9 @@ template <int HD>
 struct Packed {
   static constexpr int kKeys = HD == 128 ? 80 : 128;  // of a key tile
   static constexpr uint32_t kQBytes = kTile * HD * 2;
-  static constexpr uint32_t kSlotBytes = kKeys * HD * 2;
-  static constexpr int kSlots = 8;  // K and V tiles of the ring
-  static constexpr int kBytes = 1024 /*align*/ + 2 * kQBytes + kSlots * kSlotBytes + 512;
+  static constexpr uint32_t kTileBytes = kKeys * HD * 2;  // a K or V tile
+  static constexpr int kStages = 4;                       // of a K and a V tile
+  static constexpr int kBytes = 1024 /*align*/ + 2 * kQBytes + 2 * kStages * kTileBytes + 512;
   // TMEM columns
   static constexpr uint32_t kS = HD == 128 ? 128 : 192;  // S_1's distance from S_0, which is at 0
   static constexpr uint32_t kP = kKeys;                  // P's distance from its S
@@ -305,21 +309,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const PackedArgs a) {
   using C = Packed<HD>;
-  constexpr int kSlots = C::kSlots, kKeys = C::kKeys;
+  constexpr int kStages = C::kStages, kKeys = C::kKeys;
   constexpr int kHalves = HD / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint8_t* ring = smem + 2 * C::kQBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kSlots * C::kSlotBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + 2 * kStages * C::kTileBytes);
   uint64_t* q_full = bars;         // [1]
   uint64_t* s_full = bars + 1;     // [2] scores are in TMEM
   uint64_t* s_free = bars + 3;     // [2] and have been read
   uint64_t* p_full = bars + 5;     // [2] weights are in TMEM
   uint64_t* o_full = bars + 7;     // [2] their product is done
-  uint64_t* kv_full = bars + 9;    // [kSlots]
-  uint64_t* kv_empty = kv_full + kSlots;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kSlots);
+  uint64_t* lead = bars + 9;       // tile 0 has its first maximum
+  uint64_t* kv_full = bars + 10;   // [kStages]
+  uint64_t* kv_empty = kv_full + kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kStages);
   Work* work = reinterpret_cast<Work*>(tmem_slot + 2);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -374,15 +379,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     *work = w;
     pipe::mbar_init(q_full, 1);
+    pipe::mbar_init(lead, 4);
     for (int i = 0; i < 2; ++i) {
       pipe::mbar_init(s_full + i, 1);
       pipe::mbar_init(s_free + i, 4);
       pipe::mbar_init(p_full + i, 4);
       pipe::mbar_init(o_full + i, 1);
     }
-    for (int i = 0; i < kSlots; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       pipe::mbar_init(kv_full + i, 1);
-      pipe::mbar_init(kv_empty + i, 1);
+      pipe::mbar_init(kv_empty + i, 2);  // both tiles' issuers
     }
     pipe::fence_mbar_init();
   }
@@ -403,9 +409,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  if (warp >= 10) {
+  if (warp == 11) {
     // no role
-  } else if (warp == 9) {
+  } else if (warp == 10) {
     if (lane == 0 && blocks > 0) {
       // ---- TMA ------------------------------------------------------------------
       pipe::mbar_expect_tx(q_full, 2u * kHalves * a.heads * a.span * 128u);
@@ -413,90 +419,75 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int h = 0; h < kHalves; ++h)
           tma_4d(smem + t * C::kQBytes + h * (kTile * 128), &map_q, q_full, h * 64, head0, kv,
                  w.q0 + w.token + t * a.span);
-      // in the order of use: K_0, K_1, V_0, K_2, V_1, ..., V_last
       int n = 0;
-      for (; n < 2 * blocks; ++n) {
-        const int slot = n % kSlots;
-        if (!wait_for(kv_empty + slot, ((n / kSlots) & 1) ^ 1, a.fault)) break;
-        const bool is_v = n == 2 * blocks - 1 || (n > 0 && n % 2 == 0);
-        const int tile = n == 2 * blocks - 1 ? blocks - 1 : is_v ? n / 2 - 1 : (n + 1) / 2;
-        pipe::mbar_expect_tx(kv_full + slot, C::kSlotBytes);
-        for (int h = 0; h < kHalves; ++h)
-          tma_3d(ring + slot * C::kSlotBytes + h * (kKeys * 128), is_v ? &map_v : &map_k,
-                 kv_full + slot, h * 64, kv, w.k0 + tile * kKeys);
+      for (; n <= blocks; ++n) {
+        const int st = n % kStages;
+        if (!wait_for(kv_empty + st, ((n / kStages) & 1) ^ 1, a.fault)) break;
+        uint8_t* at = ring + 2 * st * C::kTileBytes;
+        pipe::mbar_expect_tx(kv_full + st,
+                             ((n < blocks ? 1u : 0u) + (n > 0 ? 1u : 0u)) * C::kTileBytes);
+        for (int h = 0; h < kHalves; ++h) {
+          if (n < blocks)
+            tma_3d(at + h * (kKeys * 128), &map_k, kv_full + st, h * 64, kv, w.k0 + n * kKeys);
+          if (n > 0)
+            tma_3d(at + C::kTileBytes + h * (kKeys * 128), &map_v, kv_full + st, h * 64, kv,
+                   w.k0 + (n - 1) * kKeys);
+        }
       }
       // the copies land before the CTA leaves
       wait_for(q_full, 0, a.fault);
-      for (int i = max(0, n - kSlots); i < n; ++i)
-        wait_for(kv_full + i % kSlots, (i / kSlots) & 1, a.fault);
+      for (int i = max(0, n - kStages); i < n; ++i)
+        wait_for(kv_full + i % kStages, (i / kStages) & 1, a.fault);
     }
-  } else if (warp == 8) {
+  } else if (warp >= 8) {
     if (blocks > 0) {
       // ---- products -----------------------------------------------------------------
       constexpr uint32_t idesc_s = idesc_f16(kKeys, false);
       constexpr uint32_t idesc_o = idesc_f16(HD, true);
       const bool one = elect_one();
-      const uint32_t q_lo = desc_lo(pipe::smem_u32(smem), 16);
+      const int t = __shfl_sync(0xffffffffu, warp - 8, 0);
+      const int mine = __shfl_sync(0xffffffffu, w.blocks[t], 0);
+      const uint32_t q_lo = desc_lo(pipe::smem_u32(smem) + t * C::kQBytes, 16);
       const uint32_t k_lo = desc_lo(pipe::smem_u32(ring), 16);
-      const uint32_t v_lo = desc_lo(pipe::smem_u32(ring), kKeys * 128);
-      const int blocks0 = __shfl_sync(0xffffffffu, w.blocks[0], 0);
-      const int blocks1 = __shfl_sync(0xffffffffu, w.blocks[1], 0);
-      auto scores = [&](int t, int slot) {
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          mma_ss(tmem + t * C::kS,
-                 q_lo + (t * C::kQBytes + (kk / 4) * (kTile * 128) + (kk % 4) * 32) / 16,
-                 k_lo + (slot * C::kSlotBytes + (kk / 4) * (kKeys * 128) + (kk % 4) * 32) / 16,
-                 idesc_s, kk != 0, one);
-        commit(s_full + t, one);
-      };
-      auto values = [&](int t, int slot, bool more) {
-#pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
-          mma_ts(tmem + C::kO + t * HD, tmem + t * C::kS + C::kP + kk * 8,
-                 v_lo + (slot * C::kSlotBytes + kk * 2048) / 16, idesc_o, more || kk != 0, one);
-        commit(o_full + t, one);
-      };
-      // the next ring slot and its phase
-      int slot = 0;
+      const uint32_t v_lo = desc_lo(pipe::smem_u32(ring) + C::kTileBytes, kKeys * 128);
+      const uint32_t d_s = tmem + t * C::kS, d_p = d_s + C::kP, d_o = tmem + C::kO + t * HD;
+      bool ok = wait_for(q_full, 0, a.fault);
+      // The tiles' softmaxes share the exponential unit; begun together they
+      // would stay in step, both at their exponentials and then neither. Tile
+      // 1 begins when tile 0 has its first maximum (8192 tokens: 567 us in step,
+      // 532 so).
+      if (t == 1 && min(w.blocks[0], w.blocks[1]) >= kLeadBlocks)
+        ok = ok && wait_for(lead, 0, a.fault);
+      // stage n: the scores of key tile n, then the values of n - 1
+      int st = 0;
       uint32_t phase = 0;
-      auto next = [&] {
-        if (++slot == kSlots) slot = 0, phase ^= 1;
-      };
-      bool ok = wait_for(q_full, 0, a.fault) && wait_for(kv_full, 0, a.fault);
-      if (ok) {
-        fence_after();
-        if (blocks0 > 0) scores(0, 0);
-        if (blocks1 > 0) scores(1, 0);
-        commit(kv_empty, one);
-      }
-      next();
-      for (int i = 0; i < blocks && ok; ++i) {
-        const bool more = i + 1 < blocks;
-        int sk = slot;
-        if (more) {
-          ok = wait_for(kv_full + slot, phase, a.fault);
-          next();
-        }
-        const int sv = slot;
-        ok = ok && wait_for(kv_full + slot, phase, a.fault);
-        next();
+      for (int n = 0; n <= blocks && ok; ++n) {
+        ok = wait_for(kv_full + st, phase, a.fault);
+        if (n < mine) {
+          if (n > 0) ok = ok && wait_for(s_free + t, (n - 1) & 1, a.fault);
+          fence_after();
+          if (ok) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int mine = t ? blocks1 : blocks0;
-          if (i + 1 < mine && ok) {
-            ok = wait_for(s_free + t, i & 1, a.fault);
-            fence_after();
-            if (ok) scores(t, sk);
-          }
-          if (t == 1 && more) commit(kv_empty + sk, one);
-          if (i < mine && ok) {
-            ok = wait_for(p_full + t, i & 1, a.fault);
-            fence_after();
-            if (ok) values(t, sv, i != 0);
+            for (int kk = 0; kk < HD / 16; ++kk)
+              mma_ss(d_s, q_lo + ((kk / 4) * (kTile * 128) + (kk % 4) * 32) / 16,
+                     k_lo + (2 * st * C::kTileBytes + (kk / 4) * (kKeys * 128) + (kk % 4) * 32) / 16,
+                     idesc_s, kk != 0, one);
+            commit(s_full + t, one);
           }
         }
-        commit(kv_empty + sv, one);
+        if (n > 0 && n <= mine) {
+          ok = ok && wait_for(p_full + t, (n - 1) & 1, a.fault);
+          fence_after();
+          if (ok) {
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+              mma_ts(d_o, d_p + kk * 8, v_lo + (2 * st * C::kTileBytes + kk * 2048) / 16, idesc_o,
+                     n > 1 || kk != 0, one);
+            commit(o_full + t, one);
+          }
+        }
+        commit(kv_empty + st, one);
+        if (++st == kStages) st = 0, phase ^= 1;
       }
     }
   } else {
@@ -580,6 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      if (i == 0 && t == 0 && lane == 0) arrive(lead);
       const float base = m == -INFINITY ? 0.f : -m;
       const uint64_t base2 = pair_of(base, base);
       uint32_t p[kKeys / 2];
