@@ -190,11 +190,16 @@ void launch_append(const Launch& l, const AppendArgs& a) {
 // ---- attention of one token -----------------------------------------------------
 // o = sum_j softmax_j(q . k_j / sqrt(d)) v_j over the positions of each
 // sequence. HBM-bound: every key and value is read once for all query heads
-// of its group, which are the rows of an m16n8k16 product (a group of more
-// than 16 takes several row tiles).
+// of its group.
+//
+// The products are m16n8k16 with keys (then dims) as rows and the group's
+// heads as the 8 or 16 columns: S^T = K Q^T, O^T += V^T P^T. Heads as the 16
+// rows would leave half or more of every product and twice the registers to
+// padding at the usual 1 to 8 heads a group; P^T's operand layout is S^T's
+// result layout transposed (movmatrix).
 //
 // The work is cut evenly whatever the lengths are: all (sequence, KV head,
-// row tile) units are laid end to end in tiles of 64 keys, and CTA c of C
+// head tile) units are laid end to end in tiles of 64 keys, and CTA c of C
 // takes tiles [c N / C, (c + 1) N / C). A unit that lies inside a CTA is
 // finished there; one that crosses CTAs leaves unnormalised pieces that a
 // second kernel joins in order of position, so results do not depend on
@@ -204,11 +209,13 @@ void launch_append(const Launch& l, const AppendArgs& a) {
 // Each of a CTA's four warps owns 16 keys of a tile, with its own ring of
 // cp.async stages (rows past the length are filled with zeros, so stale
 // values never enter a product) and its own running maximum and sum; the
-// warps meet only at a unit's end.
+// warps meet only at a unit's end, where each leaves its state in the ring
+// stage that it has just used up. Two CTAs to an SM keep about 130 KB of
+// loads in flight.
 constexpr int kTileKeys = 64;
 constexpr int kWarps = 4;
-constexpr int kStages = 3;
-constexpr int kRowsMax = 16;
+constexpr int kThreads = kWarps * 32;
+constexpr int kHeadsMax = 16;
 
 struct PagedArgs {
   const __half *q, *kc, *vc;
@@ -218,17 +225,20 @@ struct PagedArgs {
   uint4* meta;      // [C]: of the unit that slot 1 begins: sequence, unit, last CTA, flag
   uint32_t* fault;
   int sequences, qh, kvh, table_width, page;
+  int group;        // query heads per KV head
+  int head_tiles;   // head tiles of a group
+  int heads;        // heads of a tile (the last may have fewer)
   uint32_t pages;
   float scale_log2; // log2(e) / sqrt(HD)
 };
 
 template <int HD>
 struct PagedSmem {
+  static constexpr int kStages = HD == 128 ? 3 : 6;
   static constexpr int kStageBytes = 2 * 16 * HD * 2;  // a warp's keys and values
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kMerge = 2 * kRowsMax * HD * 4;
-  static constexpr int kBytes = kRing + kMerge + kWarps * kRowsMax * 8 + 64;
+  static constexpr int kBytes = kWarps * kStages * kStageBytes;
 };
+constexpr size_t piece_floats(int hd) { return kHeadsMax * hd + 2 * kHeadsMax; }
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
@@ -241,12 +251,19 @@ __device__ __forceinline__ void cp_async_wait() {
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+               : "r"(addr)
+               : "memory");
 }
 __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
@@ -260,6 +277,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Weight of a state with maximum m under the common maximum `top`.
+__device__ __forceinline__ float state_weight(float m, float top) {
+  return m == -INFINITY ? 0.f : exp2_fast(m - top);
 }
 
 // Length of a sequence as the kernels use it: 0 where the table cannot hold it.
@@ -275,28 +296,31 @@ struct Cursor {
   uint32_t len;
 };
 
-template <int HD>
-__global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const PagedArgs a) {
+// NT: 8-head column tiles. kRuns: the page size is a multiple of 16, so a
+// warp's 16 keys lie in one page (one table entry and one address to a stage).
+template <int HD, int NT, bool kRuns>
+__global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const PagedArgs a) {
   using S = PagedSmem<HD>;
-  constexpr int kK = HD / 16;      // k16 steps of a score
-  constexpr int kN = HD / 8;       // n8 tiles of an output row
+  constexpr int kStages = S::kStages;
+  constexpr int kK = HD / 16;      // k16 steps of a score, m16 tiles of an output column
   constexpr int kChunks = HD / 8;  // 16-byte chunks of a row
+  // row of a state in the ring: padded against bank conflicts where it fits
+  constexpr int kRow = NT == 1 ? HD + 4 : HD;
+  static_assert(8 * NT * kRow * 4 <= S::kStageBytes, "a state fits a stage");
   extern __shared__ __align__(128) uint8_t smem[];
-  float* merge = reinterpret_cast<float*>(smem + S::kRing);
-  float* stats = reinterpret_cast<float*>(smem + S::kRing + S::kMerge);  // [warp][16][2]
+  __shared__ float stats[kWarps][kHeadsMax][2];
+  __shared__ float* states[kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int group = a.qh / a.kvh;
-  const int row_tiles = (group + kRowsMax - 1) / kRowsMax;
-  const int units = a.kvh * row_tiles;
+  const int units = a.kvh * a.head_tiles;
 
   pdl_trigger();
   pdl_wait();
 
   // Where this CTA's tiles begin: tiles per sequence, summed by the block
   // (each thread a run of consecutive sequences).
-  __shared__ unsigned long long scan[kWarps * 32 + 1];
+  __shared__ unsigned long long scan[kWarps];
   __shared__ Cursor first;
-  const int run = (a.sequences + kWarps * 32 - 1) / (kWarps * 32);
+  const int run = (a.sequences + kThreads - 1) / kThreads;
   unsigned long long mine = 0;
   for (int i = 0; i < run; ++i) {
     const int s = tid * run + i;
@@ -307,6 +331,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const P
         report_fault(a.fault, kFaultLength);
     }
   }
+  unsigned long long all = 0;
   {
     unsigned long long v = mine;
 #pragma unroll
@@ -316,20 +341,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const P
     }
     if (lane == 31) scan[warp] = v;
     __syncthreads();
-    unsigned long long base = 0, all = 0;
+    unsigned long long base = 0;
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) base += scan[w];
       all += scan[w];
     }
-    __syncthreads();
     mine = base + v - mine;  // tiles before this thread's sequences
-    if (tid == 0) {
-      scan[0] = all;
-      first.s = a.sequences;
-    }
   }
-  __syncthreads();
-  const unsigned long long total = scan[0] * units;
+  const unsigned long long total = all * units;
   // no more CTAs than tiles, so that every one between a unit's first and last
   // holds a piece of it
   const unsigned long long ctas = total < gridDim.x ? total : gridDim.x;
@@ -354,7 +373,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const P
   // Rows of sequences without keys are zero.
   for (int s = blockIdx.x; s < a.sequences; s += gridDim.x)
     if (paged_length(a, s) == 0)
-      for (int i = tid; i < a.qh * HD / 8; i += kWarps * 32)
+      for (int i = tid; i < a.qh * HD / 8; i += kThreads)
         reinterpret_cast<uint4*>(a.out + (size_t)s * a.qh * HD)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   uint4 note = make_uint4(0, 0, 0, 0);
@@ -373,10 +392,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const P
   };
 
   const uint32_t ring = pipe::smem_u32(smem) + warp * kStages * S::kStageBytes;
-  const size_t row_stride = (size_t)a.kvh * HD;
-  // Issues one stage: lane l looks up row l % 16, then copies 16-byte chunks.
+  const uint32_t row_stride = a.kvh * HD;
+  // Cache row of this warp's key lane % 16 of a tile (its first one, kRuns);
+  // all ones where there is none.
   auto row_of = [&](const Cursor& c) -> uint32_t {
-    const uint32_t p = (uint32_t)c.tile * kTileKeys + warp * 16 + (lane & 15);
+    const uint32_t p = (uint32_t)c.tile * kTileKeys + warp * 16 + (kRuns ? 0 : lane & 15);
     if (p >= c.len) return 0xFFFFFFFFu;
     const uint32_t pi = p / (uint32_t)a.page;
     const uint32_t pg = a.table[(size_t)c.s * a.table_width + pi];
@@ -386,271 +406,246 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const P
     }
     return pg * a.page + (p - pi * a.page);
   };
+  constexpr int kRowsPerPass = 32 / kChunks;
+  const int chunk = lane % kChunks, row0 = lane / kChunks;
   auto issue = [&](const Cursor& c, uint32_t rows, int stage) {
-    const uint32_t dst = ring + stage * S::kStageBytes;
-    const int kv = c.unit / row_tiles;
-    constexpr int kRowsPerPass = 32 / kChunks;
-    const int chunk = lane % kChunks;
+    const uint32_t dst = ring + stage * S::kStageBytes + row0 * (HD * 2);
+    const int kv = c.unit / a.head_tiles;
+    const size_t head = (size_t)kv * HD + chunk * 8;
+    if constexpr (kRuns) {
+      // rows past the length are not read
+      const int left = rows == 0xFFFFFFFFu ? 0
+                                           : (int)c.len - c.tile * kTileKeys - warp * 16 - row0;
+      const size_t off = rows == 0xFFFFFFFFu ? head : (size_t)(rows + row0) * row_stride + head;
 #pragma unroll
-    for (int i = 0; i < 16 / kRowsPerPass; ++i) {
-      const int r = i * kRowsPerPass + lane / kChunks;
-      const uint32_t row = __shfl_sync(0xffffffffu, rows, r);
-      const bool ok = row != 0xFFFFFFFFu;
-      const size_t off = (size_t)(ok ? row : 0) * row_stride + kv * HD + chunk * 8;
-      const uint32_t d = dst + r * (HD * 2) + ((chunk ^ (r & 7)) << 4);
-      cp_async16_zfill(d, a.kc + off, ok ? 16 : 0);
-      cp_async16_zfill(d + 16 * HD * 2, a.vc + off, ok ? 16 : 0);
+      for (int i = 0; i < 16 / kRowsPerPass; ++i) {
+        const int r = i * kRowsPerPass;
+        const uint32_t bytes = r < left ? 16 : 0;
+        const size_t at = r < left ? off + (size_t)r * row_stride : head;
+        const uint32_t d = dst + r * (HD * 2) + ((chunk ^ ((r + row0) & 7)) << 4);
+        cp_async16_zfill(d, a.kc + at, bytes);
+        cp_async16_zfill(d + 16 * HD * 2, a.vc + at, bytes);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16 / kRowsPerPass; ++i) {
+        const int r = i * kRowsPerPass;
+        const uint32_t row = __shfl_sync(0xffffffffu, rows, r + row0);
+        const uint32_t bytes = row != 0xFFFFFFFFu ? 16 : 0;
+        const size_t at = row != 0xFFFFFFFFu ? (size_t)row * row_stride + head : head;
+        const uint32_t d = dst + r * (HD * 2) + ((chunk ^ ((r + row0) & 7)) << 4);
+        cp_async16_zfill(d, a.kc + at, bytes);
+        cp_async16_zfill(d + 16 * HD * 2, a.vc + at, bytes);
+      }
+    }
+  };
+  // Q^T fragments of a unit: head lane / 4 of each column tile, two values a word.
+  auto load_q = [&](const Cursor& c, uint32_t (&q)[NT][kK][2]) {
+    const int kv = c.unit / a.head_tiles, ht = c.unit % a.head_tiles;
+    const int here = min(a.heads, a.group - ht * a.heads);
+    const __half* base = a.q + ((size_t)c.s * a.qh + kv * a.group + ht * a.heads) * HD;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int h = n * 8 + (lane >> 2);
+#pragma unroll
+      for (int kk = 0; kk < kK; ++kk)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          q[n][kk][e] = h < here ? *reinterpret_cast<const uint32_t*>(
+                                       base + (size_t)h * HD + kk * 16 + e * 8 + (lane & 3) * 2)
+                                 : 0u;
     }
   };
 
   if (count > 0) {
     Cursor load = first, comp = first;
-    long long loaded = 0;
+    long long issued = 0;
     uint32_t rows = row_of(load);
-    for (int i = 0; i < kStages - 1; ++i) {
-      if (loaded < count) {
-        const Cursor now = load;
-        const uint32_t r = rows;
-        if (++loaded < count) {
-          advance(load);
-          rows = row_of(load);
-        }
-        issue(now, r, i);
+    auto issue_next = [&](int stage) {
+      const Cursor now = load;
+      const uint32_t r = rows;
+      if (++issued < count) {
+        advance(load);
+        rows = row_of(load);
       }
+      issue(now, r, stage);
+    };
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (issued < count) issue_next(i);
       pipe::cp_async_commit();
     }
-    uint32_t qf[kK][4];
-    float o[kN][4];
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    bool fresh = true;
-    bool begins = false;  // this segment holds its unit's first tile
+    uint32_t qf[NT][kK][2];
+    load_q(comp, qf);
+    float o[kK][NT][4] = {};
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+    }
+    bool begins = comp.tile == 0;  // this segment holds its unit's first tile
     int stage = 0;
-    long long issued = loaded < count ? loaded : count;
+    const int key_k = lane & 15, chunk_k = lane >> 4;                       // K as rows of keys
+    const int key_v = (lane & 7) + 8 * (lane >> 4), chunk_v = (lane >> 3) & 1;  // V^T as rows of dims
     for (long long it = 0; it < count; ++it) {
-      const int unit = comp.unit;
-      const int kv = unit / row_tiles, rt = unit % row_tiles;
-      const int rows_here = min(kRowsMax, group - rt * kRowsMax);
-      if (fresh) {
-        fresh = false;
-        begins = comp.tile == 0;
-        const __half* q = a.q + ((size_t)comp.s * a.qh + kv * group + rt * kRowsMax) * HD;
-        const int r0 = lane >> 2, c0 = (lane & 3) * 2;
-#pragma unroll
-        for (int kk = 0; kk < kK; ++kk) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = r0 + (e & 1) * 8, c = kk * 16 + c0 + (e >> 1) * 8;
-            qf[kk][e] = r < rows_here ? *reinterpret_cast<const uint32_t*>(q + (size_t)r * HD + c)
-                                      : 0u;
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < kN; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-        m0 = m1 = -INFINITY;
-        l0 = l1 = 0.f;
-      }
       // refill the stage that the previous step read
-      if (issued < count) {
-        const Cursor now = load;
-        const uint32_t r = rows;
-        if (++issued < count) {
-          advance(load);
-          rows = row_of(load);
-        }
-        int st = stage + kStages - 1;
-        if (st >= kStages) st -= kStages;
-        issue(now, r, st);
-      }
+      int st = stage + kStages - 1;
+      if (st >= kStages) st -= kStages;
+      if (issued < count) issue_next(st);
       pipe::cp_async_commit();
       cp_async_wait<kStages - 1>();
       __syncwarp();
       const uint32_t kbase = ring + stage * S::kStageBytes;
       const uint32_t vbase = kbase + 16 * HD * 2;
-      if (++stage == kStages) stage = 0;
 
-      // scores of 16 rows x 16 keys
-      float sc[2][4] = {};
-      const int key = lane & 15;
+      // scores of 16 keys x 8 NT heads
+      float sc[NT][4] = {};
 #pragma unroll
       for (int kk = 0; kk < kK; ++kk) {
-        uint32_t b[4];
-        const int chunk = 2 * kk + (lane >> 4);
-        ldsm4(b, kbase + key * (HD * 2) + ((chunk ^ (key & 7)) << 4));
-        mma16816(sc[0], qf[kk], b[0], b[2]);
-        mma16816(sc[1], qf[kk], b[1], b[3]);
+        uint32_t k4[4];
+        ldsm4(k4, kbase + key_k * (HD * 2) + (((2 * kk + chunk_k) ^ (key_k & 7)) << 4));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816(sc[n], k4, qf[n][kk][0], qf[n][kk][1]);
       }
-      const int p0 = comp.tile * kTileKeys + warp * 16 + (lane & 3) * 2;
+      const uint32_t p0 = (uint32_t)comp.tile * kTileKeys + warp * 16 + (lane >> 2);
+      const bool seen0 = p0 < comp.len, seen1 = p0 + 8 < comp.len;
+      uint32_t pf[NT][2];
+      bool moved = false;
+      float f[NT][2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool seen = (uint32_t)(p0 + n * 8 + (e & 1)) < comp.len;
-          sc[n][e] = seen ? sc[n][e] * a.scale_log2 : -INFINITY;
+        for (int e = 0; e < 2; ++e) {
+          sc[n][e] = seen0 ? sc[n][e] * a.scale_log2 : -INFINITY;
+          sc[n][e + 2] = seen1 ? sc[n][e + 2] * a.scale_log2 : -INFINITY;
+          float x = fmaxf(sc[n][e], sc[n][e + 2]);
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, sh));
+          const float top = fmaxf(m[n][e], x);
+          f[n][e] = state_weight(m[n][e], top);
+          moved |= top > m[n][e];
+          m[n][e] = top;
+          const float z = top == -INFINITY ? 0.f : top;
+          sc[n][e] = exp2_fast(sc[n][e] - z);
+          sc[n][e + 2] = exp2_fast(sc[n][e + 2] - z);
         }
-      float x0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
-      float x1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
-#pragma unroll
-      for (int sh = 1; sh < 4; sh <<= 1) {
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, sh));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, sh));
-      }
-      const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-      if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-        const float f0 = m0 == -INFINITY ? 0.f : exp2_fast(m0 - n0);
-        const float f1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - n1);
-        l0 *= f0;
-        l1 *= f1;
-#pragma unroll
-        for (int n = 0; n < kN; ++n) {
-          o[n][0] *= f0;
-          o[n][1] *= f0;
-          o[n][2] *= f1;
-          o[n][3] *= f1;
-        }
-        m0 = n0;
-        m1 = n1;
-      }
-      const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
-      uint32_t pf[4];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
         // weights rounded to FP16 for the product; the sum takes the rounded
         // ones, so a row of equal values keeps its value
-        const __half2 h0 = __floats2half2_rn(exp2_fast(sc[n][0] - z0), exp2_fast(sc[n][1] - z0));
-        const __half2 h1 = __floats2half2_rn(exp2_fast(sc[n][2] - z1), exp2_fast(sc[n][3] - z1));
+        const __half2 h0 = __floats2half2_rn(sc[n][0], sc[n][1]);
+        const __half2 h1 = __floats2half2_rn(sc[n][2], sc[n][3]);
         const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
-        l0 += g0.x + g0.y;
-        l1 += g1.x + g1.y;
-        pf[2 * n] = *reinterpret_cast<const uint32_t*>(&h0);
-        pf[2 * n + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+        l[n][0] = l[n][0] * f[n][0] + (g0.x + g1.x);
+        l[n][1] = l[n][1] * f[n][1] + (g0.y + g1.y);
+        pf[n][0] = transpose8(*reinterpret_cast<const uint32_t*>(&h0));
+        pf[n][1] = transpose8(*reinterpret_cast<const uint32_t*>(&h1));
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int kk = 0; kk < kK; ++kk)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            o[kk][n][0] *= f[n][0];
+            o[kk][n][1] *= f[n][1];
+            o[kk][n][2] *= f[n][0];
+            o[kk][n][3] *= f[n][1];
+          }
       }
 #pragma unroll
-      for (int nn = 0; nn < kN / 2; ++nn) {
-        uint32_t b[4];
-        const int chunk = 2 * nn + (lane >> 4);
-        ldsm4_trans(b, vbase + key * (HD * 2) + ((chunk ^ (key & 7)) << 4));
-        mma16816(o[2 * nn], pf, b[0], b[1]);
-        mma16816(o[2 * nn + 1], pf, b[2], b[3]);
+      for (int kk = 0; kk < kK; ++kk) {
+        uint32_t v4[4];
+        ldsm4_trans(v4, vbase + key_v * (HD * 2) + (((2 * kk + chunk_v) ^ (key_v & 7)) << 4));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816(o[kk][n], v4, pf[n][0], pf[n][1]);
       }
       __syncwarp();
 
       const bool unit_done = comp.tile + 1 == comp.tiles;
       if (!unit_done && it + 1 < count) {
-        advance(comp);
+        ++comp.tile;
+        if (++stage == kStages) stage = 0;
         continue;
       }
       // ---- a segment ends: the four warps' states become one -----------------
-      fresh = true;
-#pragma unroll
-      for (int sh = 1; sh < 4; sh <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, sh);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, sh);
+      const Cursor done = comp;
+      if (it + 1 < count) {
+        advance(comp);
+        load_q(comp, qf);  // in flight during the join
       }
-      const int r0 = lane >> 2, c0 = (lane & 3) * 2;
-      if ((lane & 3) == 0) {
-        stats[(warp * 16 + r0) * 2] = m0;
-        stats[(warp * 16 + r0) * 2 + 1] = l0;
-        stats[(warp * 16 + r0 + 8) * 2] = m1;
-        stats[(warp * 16 + r0 + 8) * 2 + 1] = l1;
-      }
-      __syncthreads();
-      float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
+      float* state = reinterpret_cast<float*>(smem + (warp * kStages + stage) * S::kStageBytes);
+      if (lane == 0) states[warp] = state;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        M0 = fmaxf(M0, stats[(w * 16 + r0) * 2]);
-        M1 = fmaxf(M1, stats[(w * 16 + r0 + 8) * 2]);
-      }
-      auto weight = [](float m, float top) {
-        return m == -INFINITY ? 0.f : exp2_fast(m - top);
-      };
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        L0 += stats[(w * 16 + r0) * 2 + 1] * weight(stats[(w * 16 + r0) * 2], M0);
-        L1 += stats[(w * 16 + r0 + 8) * 2 + 1] * weight(stats[(w * 16 + r0 + 8) * 2], M1);
-      }
-      const float f0 = weight(m0, M0), f1 = weight(m1, M1);
+        for (int e = 0; e < 2; ++e) {
+          const int h = n * 8 + (lane & 3) * 2 + e;
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        o[n][0] *= f0;
-        o[n][1] *= f0;
-        o[n][2] *= f1;
-        o[n][3] *= f1;
-      }
-      auto put = [&](float* dst) {
-#pragma unroll
-        for (int n = 0; n < kN; ++n) {
-          if (r0 < rows_here)
-            *reinterpret_cast<float2*>(dst + r0 * HD + n * 8 + c0) = make_float2(o[n][0], o[n][1]);
-          if (r0 + 8 < rows_here)
-            *reinterpret_cast<float2*>(dst + (r0 + 8) * HD + n * 8 + c0) =
-                make_float2(o[n][2], o[n][3]);
-        }
-      };
-      auto take = [&](const float* src) {
-#pragma unroll
-        for (int n = 0; n < kN; ++n) {
-          if (r0 < rows_here) {
-            const float2 f = *reinterpret_cast<const float2*>(src + r0 * HD + n * 8 + c0);
-            o[n][0] += f.x;
-            o[n][1] += f.y;
+          for (int sh = 4; sh < 32; sh <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], sh);
+          if (lane < 4) {
+            stats[warp][h][0] = m[n][e];
+            stats[warp][h][1] = l[n][e];
           }
-          if (r0 + 8 < rows_here) {
-            const float2 f = *reinterpret_cast<const float2*>(src + (r0 + 8) * HD + n * 8 + c0);
-            o[n][2] += f.x;
-            o[n][3] += f.y;
+#pragma unroll
+          for (int kk = 0; kk < kK; ++kk) {
+            state[h * kRow + kk * 16 + (lane >> 2)] = o[kk][n][e];
+            state[h * kRow + kk * 16 + (lane >> 2) + 8] = o[kk][n][e + 2];
           }
         }
-      };
-      if (warp >= 2) put(merge + (warp - 2) * kRowsMax * HD);
       __syncthreads();
-      if (warp < 2) take(merge + warp * kRowsMax * HD);
-      __syncthreads();
-      if (warp == 1) put(merge);
-      __syncthreads();
-      if (warp == 0) {
-        take(merge);
-        if (begins && unit_done) {
-          const float i0 = 1.f / L0, i1 = 1.f / L1;
-          __half* dst = a.out + ((size_t)comp.s * a.qh + kv * group + rt * kRowsMax) * HD;
+      const int kv = done.unit / a.head_tiles, ht = done.unit % a.head_tiles;
+      const int here = min(a.heads, a.group - ht * a.heads);
+      const bool whole = begins && unit_done;
+      float* piece = a.pieces + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * piece_floats(HD);
+      __half* dst = a.out + ((size_t)done.s * a.qh + kv * a.group + ht * a.heads) * HD;
+      // two dims to a thread
+      for (int i = tid; i < here * (HD / 2); i += kThreads) {
+        const int h = i / (HD / 2), d = i % (HD / 2) * 2;
+        float top = -INFINITY, sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-          for (int n = 0; n < kN; ++n) {
-            if (r0 < rows_here)
-              *reinterpret_cast<__half2*>(dst + (size_t)r0 * HD + n * 8 + c0) =
-                  __floats2half2_rn(o[n][0] * i0, o[n][1] * i0);
-            if (r0 + 8 < rows_here)
-              *reinterpret_cast<__half2*>(dst + (size_t)(r0 + 8) * HD + n * 8 + c0) =
-                  __floats2half2_rn(o[n][2] * i1, o[n][3] * i1);
-          }
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stats[w][h][0]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float g = state_weight(stats[w][h][0], top);
+          const float2 v = *reinterpret_cast<const float2*>(states[w] + h * kRow + d);
+          sum += g * stats[w][h][1];
+          x += g * v.x;
+          y += g * v.y;
+        }
+        if (whole) {
+          const float inv = 1.f / sum;
+          *reinterpret_cast<__half2*>(dst + h * HD + d) = __floats2half2_rn(x * inv, y * inv);
         } else {
-          float* piece = a.pieces + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) *
-                                        (kRowsMax * HD + 2 * kRowsMax);
-          put(piece);
-          if ((lane & 3) == 0) {
-            float* st = piece + kRowsMax * HD;
-            st[r0 * 2] = M0;
-            st[r0 * 2 + 1] = L0;
-            st[(r0 + 8) * 2] = M1;
-            st[(r0 + 8) * 2 + 1] = L1;
-          }
-          if (begins) {
-            // the CTA that holds the unit's last tile
-            const unsigned long long last = begin + it + (comp.tiles - 1 - comp.tile);
-            const uint32_t c1 = (uint32_t)(((last + 1) * ctas - 1) / total);
-            note = make_uint4((uint32_t)comp.s, (uint32_t)unit, c1, 1);
+          *reinterpret_cast<float2*>(piece + h * HD + d) = make_float2(x, y);
+          if (d == 0) {
+            piece[kHeadsMax * HD + 2 * h] = top;
+            piece[kHeadsMax * HD + 2 * h + 1] = sum;
           }
         }
       }
+      if (begins && !unit_done && tid == 0) {
+        // the CTA that holds the unit's last tile
+        const unsigned long long last = begin + it + (done.tiles - 1 - done.tile);
+        note = make_uint4((uint32_t)done.s, (uint32_t)done.unit,
+                          (uint32_t)(((last + 1) * ctas - 1) / total), 1);
+      }
       __syncthreads();
-      if (it + 1 < count) advance(comp);
+      begins = true;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < kK; ++kk) o[kk][n][0] = o[kk][n][1] = o[kk][n][2] = o[kk][n][3] = 0.f;
+      }
+      if (++stage == kStages) stage = 0;
     }
     cp_async_wait<0>();
   }
   if (tid == 0) a.meta[blockIdx.x] = note;
 }
 
-// Joins the pieces of the unit that CTA blockIdx.x began, one row to a block:
-// the pieces' maxima and sums first, then their rows weighted by them. Four
-// warps take the pieces in turn.
+// Joins the pieces of the unit that CTA blockIdx.x began, one head to a block:
+// the pieces' maxima first, then their rows weighted by them. Four warps take
+// the pieces in turn.
 template <int HD>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a) {
   constexpr int kV = HD / 32;
@@ -660,29 +655,25 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a) {
   pdl_wait();
   const uint4 note = a.meta[blockIdx.x];
   if (!note.w) return;
-  const int group = a.qh / a.kvh;
-  const int row_tiles = (group + kRowsMax - 1) / kRowsMax;
-  const int kv = note.y / row_tiles, rt = note.y % row_tiles;
-  const int row = blockIdx.y;
-  if (rt * kRowsMax + row >= group) return;
+  const int kv = note.y / a.head_tiles, ht = note.y % a.head_tiles;
+  const int h = blockIdx.y;
+  if (ht * a.heads + h >= a.group) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c0 = blockIdx.x, n = (int)note.z - c0 + 1;
-  constexpr size_t kPiece = kRowsMax * HD + 2 * kRowsMax;
   auto piece = [&](int i) {
-    return a.pieces + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPiece;
+    return a.pieces + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * piece_floats(HD);
   };
   float top = -INFINITY;
-  for (int i = lane; i < n; i += 32) top = fmaxf(top, piece(i)[kRowsMax * HD + 2 * row]);
+  for (int i = lane; i < n; i += 32) top = fmaxf(top, piece(i)[kHeadsMax * HD + 2 * h]);
   top = warp_max(top);
   float acc[kV] = {}, total = 0.f;
 #pragma unroll 4
   for (int i = warp; i < n; i += 4) {
     const float* p = piece(i);
-    const float m = p[kRowsMax * HD + 2 * row];
-    const float w = m == -INFINITY ? 0.f : exp2_fast(m - top);
-    total += w * p[kRowsMax * HD + 2 * row + 1];
+    const float w = state_weight(p[kHeadsMax * HD + 2 * h], top);
+    total += w * p[kHeadsMax * HD + 2 * h + 1];
 #pragma unroll
-    for (int e = 0; e < kV; ++e) acc[e] += w * p[row * HD + lane * kV + e];
+    for (int e = 0; e < kV; ++e) acc[e] += w * p[h * HD + lane * kV + e];
   }
 #pragma unroll
   for (int e = 0; e < kV; ++e) part[warp][lane * kV + e] = acc[e];
@@ -691,21 +682,32 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a) {
   for (int d = threadIdx.x; d < HD; d += 128) {
     const float l = sums[0] + sums[1] + sums[2] + sums[3];
     const float v = part[0][d] + part[1][d] + part[2][d] + part[3][d];
-    a.out[((size_t)note.x * a.qh + kv * group + rt * kRowsMax + row) * HD + d] =
+    a.out[((size_t)note.x * a.qh + kv * a.group + ht * a.heads + h) * HD + d] =
         __float2half_rn(v / l);
   }
 }
 
 int paged_grid(int sm_count) { return 2 * sm_count; }
 
-template <int HD>
+template <int HD, int NT, bool kRuns>
 void launch_paged(const Launch& l, const PagedArgs& a) {
-  auto kernel = paged_attention_kernel<HD>;
+  auto kernel = paged_attention_kernel<HD, NT, kRuns>;
   allow_dynamic_smem(kernel, PagedSmem<HD>::kBytes);
   const int grid = paged_grid(l.sm_count);
-  launch_kernel(l, dim3(grid), dim3(kWarps * 32), PagedSmem<HD>::kBytes, kernel, a);
-  launch_kernel(l, dim3(grid, std::min(a.qh / a.kvh, kRowsMax)), dim3(128), 0,
-                paged_join_kernel<HD>, a);
+  launch_kernel(l, dim3(grid), dim3(kThreads), PagedSmem<HD>::kBytes, kernel, a);
+  launch_kernel(l, dim3(grid, a.heads), dim3(128), 0, paged_join_kernel<HD>, a);
+}
+
+template <int HD>
+void launch_paged(const Launch& l, PagedArgs& a) {
+  const bool runs = a.page % 16 == 0;
+  const int most = a.group <= 8 ? 8 : kHeadsMax;
+  a.head_tiles = (a.group + most - 1) / most;
+  a.heads = (a.group + a.head_tiles - 1) / a.head_tiles;
+  if (a.heads <= 8)
+    runs ? launch_paged<HD, 1, true>(l, a) : launch_paged<HD, 1, false>(l, a);
+  else
+    runs ? launch_paged<HD, 2, true>(l, a) : launch_paged<HD, 2, false>(l, a);
 }
 
 }  // namespace
@@ -723,7 +725,7 @@ void paged_append(const Launch& l, const PagedAppend& p) {
 
 size_t paged_attention_workspace(int sm_count, int hd) {
   const size_t c = paged_grid(sm_count);
-  return c * 2 * (kRowsMax * hd + 2 * kRowsMax) * 4 + c * sizeof(uint4);
+  return c * 2 * piece_floats(hd) * sizeof(float) + c * sizeof(uint4);
 }
 
 void paged_attention(const Launch& l, const PagedAttention& p, void* workspace) {
@@ -744,6 +746,7 @@ void paged_attention(const Launch& l, const PagedAttention& p, void* workspace) 
   a.kvh = p.kvh;
   a.table_width = p.table_width;
   a.page = p.page;
+  a.group = p.qh / p.kvh;
   a.pages = p.pages;
   a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)p.hd));
   if (p.hd == 128)
