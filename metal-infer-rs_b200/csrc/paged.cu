@@ -199,8 +199,11 @@ void launch_append(const Launch& l, const AppendArgs& a) {
 // result layout transposed (movmatrix).
 //
 // The work is cut evenly whatever the lengths are: all (sequence, KV head,
-// head tile) units are laid end to end in tiles of 64 keys, and CTA c of C
-// takes tiles [c N / C, (c + 1) N / C). A unit that lies inside a CTA is
+// head tile) units are laid end to end, each its tiles of 64 keys and kUnitCost
+// empty places for what its end costs, and CTA c of C takes the places
+// [c N / C, (c + 1) N / C). (Without them the CTAs that met the many units of
+// short sequences set the time: 64 sequences of 1 to 8192 took 78 us, 57 with
+// them.) A unit that lies inside a CTA is
 // finished there; one that crosses CTAs leaves unnormalised pieces that a
 // second kernel joins in order of position, so results do not depend on
 // timing. A CTA has at most two pieces: one that continues a unit from the
@@ -213,6 +216,7 @@ void launch_append(const Launch& l, const AppendArgs& a) {
 // stage that it has just used up. Two CTAs to an SM keep about 130 KB of
 // loads in flight.
 constexpr int kTileKeys = 64;
+constexpr int kUnitCost = 2;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kHeadsMax = 16;
@@ -232,9 +236,13 @@ struct PagedArgs {
   float scale_log2; // log2(e) / sqrt(HD)
 };
 
-template <int HD>
-struct PagedSmem {
-  static constexpr int kStages = HD == 128 ? 3 : 6;
+template <int HD, int NT>
+struct PagedShape {
+  // CTAs to an SM, what their registers allow; head_dim 64 has half the bytes
+  // to a step of the same length, so more warps keep the loads coming (4
+  // against 2: 256 sequences of 100 to 1500 take 62 us against 63)
+  static constexpr int kCtas = HD == 128 ? 2 : NT == 1 ? 4 : 3;
+  static constexpr int kStages = 3;
   static constexpr int kStageBytes = 2 * 16 * HD * 2;  // a warp's keys and values
   static constexpr int kBytes = kWarps * kStages * kStageBytes;
 };
@@ -291,16 +299,22 @@ __device__ __forceinline__ uint32_t paged_length(const PagedArgs& a, int s) {
 
 // Walks a CTA's tiles in order.
 struct Cursor {
-  int s, unit, tile;  // sequence, unit of the sequence, tile of the unit
-  int tiles;          // tiles of a unit of this sequence
+  unsigned long long place;  // of the tile
+  int s, unit, tile;         // sequence, unit of the sequence, tile of the unit
+  int tiles;                 // tiles of a unit of this sequence
   uint32_t len;
 };
+// Places of a unit of n keys.
+__device__ __forceinline__ uint32_t unit_places(uint32_t n) {
+  return n ? (n + kTileKeys - 1) / kTileKeys + kUnitCost : 0;
+}
 
 // NT: 8-head column tiles. kRuns: the page size is a multiple of 16, so a
 // warp's 16 keys lie in one page (one table entry and one address to a stage).
 template <int HD, int NT, bool kRuns>
-__global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const PagedArgs a) {
-  using S = PagedSmem<HD>;
+__global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
+    paged_attention_kernel(const PagedArgs a) {
+  using S = PagedShape<HD, NT>;
   constexpr int kStages = S::kStages;
   constexpr int kK = HD / 16;      // k16 steps of a score, m16 tiles of an output column
   constexpr int kChunks = HD / 8;  // 16-byte chunks of a row
@@ -313,10 +327,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int units = a.kvh * a.head_tiles;
 
-  pdl_trigger();
   pdl_wait();
 
-  // Where this CTA's tiles begin: tiles per sequence, summed by the block
+  // Where this CTA's places begin: places per sequence, summed by the block
   // (each thread a run of consecutive sequences).
   __shared__ unsigned long long scan[kWarps];
   __shared__ Cursor first;
@@ -326,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
     const int s = tid * run + i;
     if (s < a.sequences) {
       const uint32_t n = paged_length(a, s);
-      mine += (n + kTileKeys - 1) / kTileKeys;
+      mine += unit_places(n);
       if (n == 0 && s % gridDim.x == blockIdx.x && a.lengths[s] != 0)
         report_fault(a.fault, kFaultLength);
     }
@@ -346,10 +359,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
       if (w < warp) base += scan[w];
       all += scan[w];
     }
-    mine = base + v - mine;  // tiles before this thread's sequences
+    mine = base + v - mine;  // places before this thread's sequences
   }
   const unsigned long long total = all * units;
-  // no more CTAs than tiles, so that every one between a unit's first and last
+  // no more CTAs than places, so that every one between a unit's first and last
   // holds a piece of it
   const unsigned long long ctas = total < gridDim.x ? total : gridDim.x;
   const bool works = blockIdx.x < ctas;
@@ -361,11 +374,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
       const int s = tid * run + i;
       if (s >= a.sequences) break;
       const uint32_t n = paged_length(a, s);
-      const int tiles = (n + kTileKeys - 1) / kTileKeys;
-      const unsigned long long next = at + (unsigned long long)tiles * units;
+      const uint32_t places = unit_places(n);
+      const unsigned long long next = at + (unsigned long long)places * units;
       if (at <= begin && begin < next) {
         const unsigned long long w = begin - at;
-        first = Cursor{s, (int)(w / tiles), (int)(w % tiles), tiles, n};
+        first = Cursor{begin, s, (int)(w / places), (int)(w % places), (int)places - kUnitCost, n};
       }
       at = next;
     }
@@ -377,15 +390,19 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
         reinterpret_cast<uint4*>(a.out + (size_t)s * a.qh * HD)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   uint4 note = make_uint4(0, 0, 0, 0);
-  const long long count = (long long)(end - begin);
 
   auto advance = [&](Cursor& c) {
+    ++c.place;
     if (++c.tile < c.tiles) return;
+    c.place += c.tiles + kUnitCost - c.tile;  // the rest of the unit's places
     c.tile = 0;
     if (++c.unit < units) return;
     c.unit = 0;
     do {
-      if (++c.s >= a.sequences) return;
+      if (++c.s >= a.sequences) {
+        c.place = end;
+        return;
+      }
       c.len = paged_length(a, c.s);
       c.tiles = (c.len + kTileKeys - 1) / kTileKeys;
     } while (c.tiles == 0);
@@ -457,21 +474,22 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
     }
   };
 
-  if (count > 0) {
-    Cursor load = first, comp = first;
-    long long issued = 0;
+  Cursor comp = first;
+  if (begin < end && comp.tile >= comp.tiles) {  // a unit's empty places come first
+    advance(comp);
+  }
+  if (begin < end && comp.place < end) {
+    Cursor load = comp;
     uint32_t rows = row_of(load);
     auto issue_next = [&](int stage) {
       const Cursor now = load;
       const uint32_t r = rows;
-      if (++issued < count) {
-        advance(load);
-        rows = row_of(load);
-      }
+      advance(load);
+      if (load.place < end) rows = row_of(load);
       issue(now, r, stage);
     };
     for (int i = 0; i < kStages - 1; ++i) {
-      if (issued < count) issue_next(i);
+      if (load.place < end) issue_next(i);
       pipe::cp_async_commit();
     }
     uint32_t qf[NT][kK][2];
@@ -487,11 +505,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
     int stage = 0;
     const int key_k = lane & 15, chunk_k = lane >> 4;                       // K as rows of keys
     const int key_v = (lane & 7) + 8 * (lane >> 4), chunk_v = (lane >> 3) & 1;  // V^T as rows of dims
-    for (long long it = 0; it < count; ++it) {
+    while (true) {
       // refill the stage that the previous step read
       int st = stage + kStages - 1;
       if (st >= kStages) st -= kStages;
-      if (issued < count) issue_next(st);
+      if (load.place < end) issue_next(st);
       pipe::cp_async_commit();
       cp_async_wait<kStages - 1>();
       __syncwarp();
@@ -560,17 +578,17 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
       __syncwarp();
 
       const bool unit_done = comp.tile + 1 == comp.tiles;
-      if (!unit_done && it + 1 < count) {
+      if (!unit_done && comp.place + 1 < end) {
         ++comp.tile;
+        ++comp.place;
         if (++stage == kStages) stage = 0;
         continue;
       }
       // ---- a segment ends: the four warps' states become one -----------------
       const Cursor done = comp;
-      if (it + 1 < count) {
-        advance(comp);
-        load_q(comp, qf);  // in flight during the join
-      }
+      advance(comp);
+      const bool more = comp.place < end;
+      if (more) load_q(comp, qf);  // in flight during the join
       float* state = reinterpret_cast<float*>(smem + (warp * kStages + stage) * S::kStageBytes);
       if (lane == 0) states[warp] = state;
 #pragma unroll
@@ -623,10 +641,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
       }
       if (begins && !unit_done && tid == 0) {
         // the CTA that holds the unit's last tile
-        const unsigned long long last = begin + it + (done.tiles - 1 - done.tile);
+        const unsigned long long last = done.place + (done.tiles - 1 - done.tile);
         note = make_uint4((uint32_t)done.s, (uint32_t)done.unit,
                           (uint32_t)(((last + 1) * ctas - 1) / total), 1);
       }
+      if (!more) break;
       __syncthreads();
       begins = true;
 #pragma unroll
@@ -641,6 +660,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
     cp_async_wait<0>();
   }
   if (tid == 0) a.meta[blockIdx.x] = note;
+  pdl_trigger();
 }
 
 // Joins the pieces of the unit that CTA blockIdx.x began, one head to a block:
@@ -651,8 +671,10 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a) {
   constexpr int kV = HD / 32;
   __shared__ float part[4][HD];
   __shared__ float sums[4];
-  pdl_trigger();
+  // The next op's grid starts only when this one's wait is over: launched
+  // earlier, its waiting CTAs take the places of the ones that still work.
   pdl_wait();
+  pdl_trigger();
   const uint4 note = a.meta[blockIdx.x];
   if (!note.w) return;
   const int kv = note.y / a.head_tiles, ht = note.y % a.head_tiles;
@@ -687,14 +709,16 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a) {
   }
 }
 
-int paged_grid(int sm_count) { return 2 * sm_count; }
+constexpr int kCtasMax = 4;
 
 template <int HD, int NT, bool kRuns>
 void launch_paged(const Launch& l, const PagedArgs& a) {
   auto kernel = paged_attention_kernel<HD, NT, kRuns>;
-  allow_dynamic_smem(kernel, PagedSmem<HD>::kBytes);
-  const int grid = paged_grid(l.sm_count);
-  launch_kernel(l, dim3(grid), dim3(kThreads), PagedSmem<HD>::kBytes, kernel, a);
+  using S = PagedShape<HD, NT>;
+  static_assert(S::kCtas <= kCtasMax, "workspace");
+  allow_dynamic_smem(kernel, S::kBytes);
+  const int grid = S::kCtas * l.sm_count;
+  launch_kernel(l, dim3(grid), dim3(kThreads), S::kBytes, kernel, a);
   launch_kernel(l, dim3(grid, a.heads), dim3(128), 0, paged_join_kernel<HD>, a);
 }
 
@@ -724,13 +748,13 @@ void paged_append(const Launch& l, const PagedAppend& p) {
 }
 
 size_t paged_attention_workspace(int sm_count, int hd) {
-  const size_t c = paged_grid(sm_count);
+  const size_t c = kCtasMax * sm_count;
   return c * 2 * piece_floats(hd) * sizeof(float) + c * sizeof(uint4);
 }
 
 void paged_attention(const Launch& l, const PagedAttention& p, void* workspace) {
   if (p.sequences == 0) return;
-  const size_t c = paged_grid(l.sm_count);
+  const size_t c = kCtasMax * l.sm_count;
   PagedArgs a{};
   a.q = p.q;
   a.kc = p.key_cache;
