@@ -13,10 +13,12 @@
 // finite values: the row is counted into a histogram of order keys, an exact
 // and order-free sum, and each distinct value's weight is computed once.
 //
-// A cluster of 8 CTAs takes a row: each counts an eighth of the row's indexes
-// into a histogram of 16-bit counts in its shared memory, then sums a
-// contiguous range of 8,192 keys over the cluster's histograms and scans it.
-// Ranges descend with the CTA's rank, so running sums go from rank 0 up.
+// A cluster of 8 CTAs takes a row, of 4 where the rows fill the GPU: each
+// counts its share of the row's indexes into a histogram of 16-bit counts in
+// its shared memory, then sums its keys over the cluster's histograms and
+// scans them. The keys go to the CTAs in blocks of 1,024 by turns, since a
+// row's values share a few exponents; the scan is by descending key: threads,
+// blocks of a CTA, then the 64 blocks' sums of all CTAs.
 
 #include <cooperative_groups.h>
 
@@ -29,24 +31,25 @@ namespace k {
 
 namespace {
 
-constexpr int kCtas = 8;
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
-constexpr int kKeys = 65536 / kCtas;      // keys a CTA scans
-constexpr int kPer = kKeys / kThreads;    // keys a thread scans
-static_assert(kPer == 8, "a thread reads its keys as one 16-byte word");
+constexpr int kBlockKeys = 1024;
+constexpr int kBlocks = 65536 / kBlockKeys;
+static_assert(kBlocks == 64, "a warp sums the blocks two to a lane");
 
 struct Shared {
   uint32_t hist[65536 / 2];  // two 16-bit counts to a word
   double warp_mass[kWarps];
   uint32_t warp_count[kWarps];
+  uint32_t equals[kWarps];
   // read by the cluster's other CTAs
-  uint32_t top;              // largest key + 1
-  uint32_t count;            // candidates of this CTA's range
-  double mass;               // their weight (after top_k)
-  double kept;               // running sum at this range's last kept candidate, or -1
-  uint32_t key, place;       // the token's key + 1 and place (0: not here)
-  uint32_t before[kWarps];
+  uint32_t top;                // largest key + 1
+  uint32_t count[kBlocks / 4]; // candidates of this CTA's blocks
+  double mass[kBlocks / 4];    // their weight (after top_k)
+  uint32_t last;               // order + 1 of this CTA's last kept group
+  double kept;                 // running sum at its end
+  uint32_t first;              // ~order of this CTA's first group that crosses the target
+  uint32_t key, place;         // its key + 1, the place among the equals
 };
 
 __device__ __forceinline__ float key_value(uint32_t key) {
@@ -54,9 +57,12 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __half2float(__ushort_as_half(bits));
 }
 
-// Sum over the threads before this one, and over the block.
-template <class T>
-__device__ __forceinline__ T block_exclusive(T v, T* warps, T& total) {
+// Sum over everything before this thread in descending key order, and over
+// the row. `sums` (this CTA's blocks) is read by the cluster.
+template <int kCtas, class T>
+__device__ __forceinline__ T row_exclusive(cg::cluster_group& cluster, T v, T* warps, T* sums,
+                                           T& total) {
+  constexpr int kBlockWarps = kThreads / (kBlocks / kCtas) / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   T x = v;
 #pragma unroll
@@ -64,46 +70,43 @@ __device__ __forceinline__ T block_exclusive(T v, T* warps, T& total) {
     const T y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
-  __syncthreads();
   if (lane == 31) warps[warp] = x;
+  T before = __shfl_up_sync(0xffffffffu, x, 1);
+  if (lane == 0) before = T(0);
   __syncthreads();
-  T w = warps[lane];
+  const int block = warp / kBlockWarps;
+  T all = T(0), base = T(0);
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += y;
+  for (int w = 0; w < kBlockWarps; ++w) {
+    const T y = warps[block * kBlockWarps + w];
+    if (w < warp % kBlockWarps) base += y;
+    all += y;
   }
-  total = __shfl_sync(0xffffffffu, w, 31);
-  const T base = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-  T up = __shfl_up_sync(0xffffffffu, x, 1);
-  if (lane == 0) up = T(0);
-  return (warp ? base : T(0)) + up;
+  if (lane == 0 && warp % kBlockWarps == 0) sums[block] = all;
+  cluster.sync();
+  // block b of the row is block b / kCtas of CTA b % kCtas
+  const int mine = block * kCtas + (int)cluster.block_rank();
+  T earlier = T(0), every = T(0);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int b = lane + 32 * i;
+    const T y = cluster.map_shared_rank(sums, b % kCtas)[b / kCtas];
+    every += y;
+    if (b < mine) earlier += y;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    every += __shfl_xor_sync(0xffffffffu, every, o);
+    earlier += __shfl_xor_sync(0xffffffffu, earlier, o);
+  }
+  total = every;
+  return earlier + (base + before);
 }
 
-// The first / last thread for which `yes` holds, or -1.
-__device__ __forceinline__ int block_first(bool yes, uint32_t* warps) {
-  const unsigned has = __ballot_sync(0xffffffffu, yes);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = has;
-  __syncthreads();
-  const unsigned any = __ballot_sync(0xffffffffu, warps[threadIdx.x & 31] != 0);
-  if (!any) return -1;
-  const int w = __ffs(any) - 1;
-  return 32 * w + __ffs(warps[w]) - 1;
-}
-__device__ __forceinline__ int block_last(bool yes, uint32_t* warps) {
-  const unsigned has = __ballot_sync(0xffffffffu, yes);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = has;
-  __syncthreads();
-  const unsigned any = __ballot_sync(0xffffffffu, warps[threadIdx.x & 31] != 0);
-  if (!any) return -1;
-  const int w = 31 - __clz(any);
-  return 32 * w + 31 - __clz(warps[w]);
-}
-
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1)
-    sample_batch_kernel(const SampleBatch p) {
+template <int kCtas>
+__global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleBatch p) {
+  constexpr int kPer = 65536 / kCtas / kThreads;  // keys of a thread
+  constexpr int kBlockThreads = kBlockKeys / kPer;
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
   cg::cluster_group cluster = cg::this_cluster();
@@ -115,6 +118,8 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1)
     reinterpret_cast<uint4*>(sh.hist)[i] = make_uint4(0, 0, 0, 0);
   if (tid == 0) {
     sh.top = 0;
+    sh.last = 0;
+    sh.first = 0;
     sh.key = 0;
   }
   pdl_trigger();
@@ -149,10 +154,12 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1)
   };
   {
     // 16-byte words of the range, and what lies before and behind them
-    const int head = min(last - first, (int)((16 - (reinterpret_cast<uintptr_t>(x + first) & 15)) & 15) / 2);
+    const int head =
+        min(last - first, (int)((16 - (reinterpret_cast<uintptr_t>(x + first) & 15)) & 15) / 2);
     const int words = (last - first - head) / 8;
     if (tid < head) count(x[first + tid]);
     const uint4* w = reinterpret_cast<const uint4*>(x + first + head);
+#pragma unroll 2
     for (int i = tid; i < words; i += kThreads) {
       const uint4 v = w[i];
       const uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -169,38 +176,43 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1)
   if (lane == 0 && top) atomicMax(&sh.top, top);
   cluster.sync();
   top = 0;
+#pragma unroll
   for (int c = 0; c < kCtas; ++c) top = max(top, *cluster.map_shared_rank(&sh.top, c));
 
-  // ---- this thread's keys, descending from `high` ----------------------------------
-  const int high = 65536 - rank * kKeys - tid * kPer;  // keys high - 1 ... high - kPer
+  // ---- this thread's keys, descending: high - 1 ... high - kPer ----------------------
+  const int block = tid / kBlockThreads * kCtas + rank;
+  const int high = 65536 - block * kBlockKeys - tid % kBlockThreads * kPer;
+  const uint32_t order = block * kBlockThreads + tid % kBlockThreads;
   uint32_t c[kPer] = {};
-  for (int r = 0; r < kCtas; ++r) {
-    const uint4 v =
-        *reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.hist, r) + (high - kPer) / 2);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      c[kPer - 1 - 2 * e] += u[e] & 0xffffu;
-      c[kPer - 2 - 2 * e] += u[e] >> 16;
+  for (int r = 0; r < kCtas; ++r) {
+    const uint4* h =
+        reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.hist, r) + (high - kPer) / 2);
+#pragma unroll
+    for (int i = 0; i < kPer / 8; ++i) {
+      const uint4 v = h[i];
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c[kPer - 1 - 8 * i - 2 * e] += u[e] & 0xffffu;
+        c[kPer - 2 - 8 * i - 2 * e] += u[e] >> 16;
+      }
     }
   }
-  uint32_t place = 0, key = 0;  // the token, where it is in this thread's keys
-  bool chosen = false;
   if (top == 0) {
     // no finite logit
   } else if (temperature == 0.f) {
-    key = top - 1;
-    chosen = rank == 0 && tid == 0;
+    if (rank == 0 && tid == 0) {
+      sh.first = ~0u;
+      sh.key = top;
+      sh.place = 0;
+    }
   } else {
-    const double most = (double)key_value(top - 1);
     if (top_k) {  // the first top_k candidates stay
       uint32_t own = 0, all;
 #pragma unroll
       for (int e = 0; e < kPer; ++e) own += c[e];
-      uint32_t at = block_exclusive(own, sh.warp_count, all);
-      if (tid == 0) sh.count = all;
-      cluster.sync();
-      for (int r = 0; r < rank; ++r) at += *cluster.map_shared_rank(&sh.count, r);
+      uint32_t at = row_exclusive<kCtas>(cluster, own, sh.warp_count, sh.count, all);
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
         const uint32_t n = c[e];
@@ -208,36 +220,30 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1)
         at += n;
       }
     }
-    double w[kPer], own = 0.0, all;
+    const double most = (double)key_value(top - 1), inverse = 1.0 / (double)temperature;
+    double w[kPer], own = 0.0, total;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      w[e] = c[e] ? exp(((double)key_value(high - 1 - e) - most) / (double)temperature) : 0.0;
+      w[e] = c[e] ? exp(((double)key_value(high - 1 - e) - most) * inverse) : 0.0;
       own += c[e] * w[e];
     }
-    double at = block_exclusive(own, sh.warp_mass, all);
-    if (tid == 0) sh.mass = all;
-    cluster.sync();
-    double before = 0.0, total = 0.0;
-    for (int r = 0; r < kCtas; ++r) {
-      const double m = *cluster.map_shared_rank(&sh.mass, r);
-      if (r < rank) before += m;
-      total += m;
-    }
-    at += before;
+    const double at = row_exclusive<kCtas>(cluster, own, sh.warp_mass, sh.mass, total);
     // What top_p and min_p keep is a prefix again: the kept sum is the sum at
     // the end of the last kept group.
     const double limit = top_p >= 1.f ? INFINITY : (double)top_p * total;
     double kept = -1.0, sum = at;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      uint32_t n = c[e];
-      if (!(w[e] >= (double)min_p)) n = 0;
-      if (n && limit != INFINITY) {
+      uint32_t n = w[e] >= (double)min_p ? c[e] : 0u;
+      if (n && !(sum + (n - 1) * w[e] < limit)) {
         // places j with sum + j w < limit
-        const double j = ceil((limit - sum) / w[e]);
-        uint32_t m = j <= 0.0 ? 0u : j >= (double)n ? n : (uint32_t)j;
-        if (m && !(sum + (m - 1) * w[e] < limit)) --m;
-        else if (m < n && sum + m * w[e] < limit) ++m;
+        uint32_t m = 0;
+        if (sum < limit) {
+          const double j = ceil((limit - sum) / w[e]);
+          m = j >= (double)n ? n : (uint32_t)j;
+          if (m && !(sum + (m - 1) * w[e] < limit)) --m;
+          else if (m < n && sum + m * w[e] < limit) ++m;
+        }
         n = m;
       }
       if (c[e] && n == 0 && (uint32_t)(high - e) == top) n = 1;  // the first always stays
@@ -245,14 +251,21 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1)
       sum += c[e] * w[e];
       c[e] = n;
     }
-    const int last_thread = block_last(kept >= 0.0, sh.before);
-    if (tid == last_thread) sh.kept = kept;
-    if (tid == 0 && last_thread < 0) sh.kept = -1.0;
+    const uint32_t mine = kept >= 0.0 ? order + 1 : 0u;
+    const uint32_t warp_last = __reduce_max_sync(0xffffffffu, mine);
+    if (lane == 0 && warp_last) atomicMax(&sh.last, warp_last);
+    __syncthreads();
+    if (mine && sh.last == mine) sh.kept = kept;
     cluster.sync();
+    uint32_t final = 0;
     double sum_kept = 0.0;
+#pragma unroll
     for (int r = 0; r < kCtas; ++r) {
-      const double s = *cluster.map_shared_rank(&sh.kept, r);
-      if (s >= 0.0) sum_kept = s;
+      const uint32_t q = *cluster.map_shared_rank(&sh.last, r);
+      if (q > final) {
+        final = q;
+        sum_kept = *cluster.map_shared_rank(&sh.kept, r);
+      }
     }
     // The first group whose sum exceeds the target: there is one, as the
     // last kept group's sum is the kept sum itself. Threads' sums meet within
@@ -262,31 +275,40 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1)
     sum = at;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      if (c[e] && !crosses && sum + c[e] * w[e] > target) {
-        const double j = floor((target - sum) / w[e]);
-        uint32_t m = j <= 0.0 ? 0u : j >= (double)c[e] ? c[e] - 1 : (uint32_t)j;
-        if (sum + (m + 1) * w[e] <= target && m + 1 < c[e]) ++m;
-        else if (m && sum + m * w[e] > target) --m;
-        crosses = true;
-        key = high - 1 - e;
-        place = m;
-      }
+      if (c[e] && sum + c[e] * w[e] > target) crosses = true;
       sum += c[e] * w[e];
     }
-    chosen = tid == block_first(crosses, sh.before);
-  }
-  if (chosen) {
-    sh.key = key + 1;
-    sh.place = place;
+    const uint32_t hit = crosses ? ~order : 0u;
+    const uint32_t warp_first = __reduce_max_sync(0xffffffffu, hit);
+    if (lane == 0 && warp_first) atomicMax(&sh.first, warp_first);
+    __syncthreads();
+    if (hit && sh.first == hit) {
+      sum = at;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        if (crosses && c[e] && sum + c[e] * w[e] > target) {
+          const double j = floor((target - sum) / w[e]);
+          uint32_t m = j <= 0.0 ? 0u : j >= (double)c[e] ? c[e] - 1 : (uint32_t)j;
+          if (sum + (m + 1) * w[e] <= target && m + 1 < c[e]) ++m;
+          else if (m && sum + m * w[e] > target) --m;
+          sh.key = high - e;
+          sh.place = m;
+          crosses = false;
+        }
+        sum += c[e] * w[e];
+      }
+    }
   }
   cluster.sync();
 
   // ---- key and place to an index -----------------------------------------------------
-  key = 0;
-  for (int r = kCtas - 1; r >= 0; --r) {
-    const uint32_t q = *cluster.map_shared_rank(&sh.key, r);
-    if (q) {
-      key = q;
+  uint32_t key = 0, place = 0, best = 0;
+#pragma unroll
+  for (int r = 0; r < kCtas; ++r) {
+    const uint32_t q = *cluster.map_shared_rank(&sh.first, r);
+    if (q > best) {
+      best = q;
+      key = *cluster.map_shared_rank(&sh.key, r);
       place = *cluster.map_shared_rank(&sh.place, r);
     }
   }
@@ -303,21 +325,19 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1)
       // that holds the place walks its run
       const int run = (last - first + kWarps * 32 - 1) / (kWarps * 32) * 32;
       const int a = min(last, first + warp * run), b = min(last, a + run);
+      // the FP16 bits of the key
+      const uint16_t bits = (uint16_t)((key & 0x8000u) ? (key ^ 0x8000u) : (~key & 0xffffu));
       int equals = 0;
-      for (int i = a; i < b; i += 32) {
-        const bool eq = i + lane < b && (x[i + lane] & 0x7c00u) != 0x7c00u &&
-                        sample_key16(x[i + lane]) == key;
-        equals += __popc(__ballot_sync(0xffffffffu, eq));
-      }
-      __syncthreads();
-      if (lane == 0) sh.before[warp] = equals;
+#pragma unroll 4
+      for (int i = a; i < b; i += 32)
+        equals += __popc(__ballot_sync(0xffffffffu, i + lane < b && x[i + lane] == bits));
+      if (lane == 0) sh.equals[warp] = equals;
       __syncthreads();
       int rest = at;
-      for (int q = 0; q < warp; ++q) rest -= (int)sh.before[q];
+      for (int q = 0; q < warp; ++q) rest -= (int)sh.equals[q];
       if (rest >= 0 && rest < equals) {
         for (int i = a; i < b; i += 32) {
-          const bool eq = i + lane < b && (x[i + lane] & 0x7c00u) != 0x7c00u &&
-                          sample_key16(x[i + lane]) == key;
+          const bool eq = i + lane < b && x[i + lane] == bits;
           const unsigned hits = __ballot_sync(0xffffffffu, eq);
           const int n = __popc(hits);
           if (rest < n) {
@@ -332,12 +352,40 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1)
   cluster.sync();  // no CTA leaves while another reads its shared memory
 }
 
+template <int kCtas>
+void launch_sample(const Launch& l, const SampleBatch& p) {
+  auto kernel = sample_batch_kernel<kCtas>;
+  allow_dynamic_smem(kernel, sizeof(Shared));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.rows * kCtas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.stream = l.stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = l.pdl ? 2 : 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (err != cudaSuccess)
+    fail(MI_ERR_COMMAND, "kernel launch failed: %s", cudaGetErrorString(err));
+}
+
 }  // namespace
 
 void sample_batch(const Launch& l, const SampleBatch& p) {
   if (p.rows == 0) return;
-  allow_dynamic_smem(sample_batch_kernel, sizeof(Shared));
-  launch_kernel(l, dim3(p.rows * kCtas), dim3(kThreads), sizeof(Shared), sample_batch_kernel, p);
+  // Four CTAs to a row leave fewer fixed costs, eight are quicker with a row:
+  // eight while the rows fit the GPU at once, or where a CTA's share of the
+  // row would outgrow its 16-bit counts.
+  if (p.rows * 8 <= l.sm_count || p.n > 4 * 65528)
+    launch_sample<8>(l, p);
+  else
+    launch_sample<4>(l, p);
 }
 
 }  // namespace k
