@@ -336,7 +336,7 @@ mi_status mi_batch_paged_attention(mi_batch* b, const mi_tensor* query,
 mi_status mi_batch_packed_attention(mi_batch* b, const mi_tensor* query, const mi_tensor* key,
                                     const mi_tensor* value, const mi_tensor* query_starts,
                                     const mi_tensor* key_starts, int causal, mi_tensor* out);
-/* One token per row of logits [rows, vocab] (vocab up to 524224): temperature,
+/* One token per row of logits [rows, vocab] (vocab up to 2^22): temperature,
  * top_p, min_p and uniform F32 [rows], top_k U32 [rows] (0: all). Candidates
  * are the finite logits, ordered as in mi_sample_logits. top_k keeps the
  * first; over their exp((v - max) / temperature), in FP64, top_p keeps the

@@ -281,8 +281,8 @@ struct SampleBatch {
   uint32_t* fault = nullptr;
   int rows = 0, n = 0;
 };
-// Largest vocabulary of sample_batch: a block's histogram counts in 16 bits.
-constexpr int kSampleBatchMax = 8 * 65528;
+// Largest vocabulary of sample_batch.
+constexpr int kSampleBatchMax = 1 << 22;
 void sample_batch(const Launch& l, const SampleBatch& p);
 
 // ---- tensor parallelism -----------------------------------------------------------

@@ -985,6 +985,9 @@ mi_status mi_batch_sample(mi_batch* b, const mi_tensor* logits, const mi_tensor*
     require_tensor(ctx, uniform, MI_F32, 1, "uniform");
     require_tensor(ctx, tokens, MI_U32, 1, "tokens");
     const size_t rows = logits->shape[0], n = logits->shape[1];
+    if (n == 0 || n > (size_t)k::kSampleBatchMax)
+      fail(MI_ERR_SHAPE, "invalid tensor shape: sampling takes 1 to %d logits a row, got %zu",
+           k::kSampleBatchMax, n);
     for (const mi_tensor* t : {temperature, top_k, top_p, min_p, uniform, (const mi_tensor*)tokens}) {
       require_shape(t, {rows}, "a per-row tensor");
       require_aligned(t, 4, "a per-row tensor");
@@ -992,9 +995,6 @@ mi_status mi_batch_sample(mi_batch* b, const mi_tensor* logits, const mi_tensor*
     }
     require_aligned(logits, 2, "logits");
     require_apart(tokens, logits, "the logits");
-    if (n == 0 || n > (size_t)k::kSampleBatchMax)
-      fail(MI_ERR_SHAPE, "invalid tensor shape: sampling takes 1 to %d logits a row, got %zu",
-           k::kSampleBatchMax, n);
     if (rows > 0xFFFFFFull) fail(MI_ERR_SHAPE, "invalid tensor shape: more than 2^24 rows");
     if (rows == 0) return;
     DeviceScope device(ctx);

@@ -11,14 +11,18 @@
 // Weights and sums are FP64, so a token depends on the order of additions only
 // where the uniform number lies within about 1e-15 of a border. FP16 has 63,488
 // finite values: the row is counted into a histogram of order keys, an exact
-// and order-free sum, and each distinct value's weight is computed once.
+// and order-free sum, and weights belong to values, not to candidates. Eight
+// neighbouring keys share an exponent, so their weights are one exponential
+// and powers of another.
 //
-// A cluster of 8 CTAs takes a row, of 4 where the rows fill the GPU: each
-// counts its share of the row's indexes into a histogram of 16-bit counts in
-// its shared memory, then sums its keys over the cluster's histograms and
-// scans them. The keys go to the CTAs in blocks of 1,024 by turns, since a
-// row's values share a few exponents; the scan is by descending key: threads,
-// blocks of a CTA, then the 64 blocks' sums of all CTAs.
+// A CTA counts 16 bits to a key (128 KB of shared memory). The shared-memory
+// additions set the pace, so a row that shares the GPU with many others has
+// one CTA and nothing to add up between CTAs; where rows are few, a cluster of
+// 8 CTAs takes a row: each counts an eighth of it, then adds up the keys of
+// its own over the cluster's histograms (blocks of 64 keys by turns, as a
+// row's values share a few exponents). Measured, 96 rows of 151,936: 115 us
+// with 4 CTAs to a row, 120 with every CTA reading the whole row for its own
+// keys, XXX so; one row XXX with 8 CTAs, XXX with one.
 
 #include <cooperative_groups.h>
 
@@ -33,94 +37,156 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBlockKeys = 1024;
+constexpr int kBlockKeys = 64;
 constexpr int kBlocks = 65536 / kBlockKeys;
-static_assert(kBlocks == 64, "a warp sums the blocks two to a lane");
+static_assert(kBlocks == kThreads, "a thread takes a block's sum");
+// Finite keys, descending: 65535 - the order key, so that the largest value
+// comes first; infinities and NaN lie outside of [kFirst, kEnd).
+constexpr uint32_t kFirst = 0x400, kEnd = 0xFC00;
+// A count may grow by a segment's elements before it is looked at again;
+// those above kLarge then move to a list of their own.
+constexpr int kSegment = 49152;
+constexpr uint32_t kLarge = 65535 - kSegment;
+constexpr int kLargeMax = kSampleBatchMax / (int)kLarge + 1;
 
 struct Shared {
   uint32_t hist[65536 / 2];  // two 16-bit counts to a word
+  double before[kBlocks];    // sum before each block of the row
   double warp_mass[kWarps];
+  double step[64];           // weight of one step of an exponent's values (sign in front)
   uint32_t warp_count[kWarps];
   uint32_t equals[kWarps];
+  uint32_t least;            // smallest key of this CTA's part - kFirst
+  uint32_t last, first;      // order + 1 of the last kept thread, ~order of the first that crosses
   // read by the cluster's other CTAs
-  uint32_t top;                // largest key + 1
-  uint32_t count[kBlocks / 4]; // candidates of this CTA's blocks
-  double mass[kBlocks / 4];    // their weight (after top_k)
-  uint32_t last;               // order + 1 of this CTA's last kept group
-  double kept;                 // running sum at its end
-  uint32_t first;              // ~order of this CTA's first group that crosses the target
-  uint32_t key, place;         // its key + 1, the place among the equals
+  uint32_t large;            // counts moved out of the histogram
+  uint32_t large_key[kLargeMax], large_count[kLargeMax];
+  double mass[kBlocks];      // sums of this CTA's blocks
+  uint32_t count[kBlocks];
+  double kept;               // running sum where this CTA's kept candidates end
+  uint32_t kept_order;       // order + 1 of the thread that has it, 0: none
+  // written by them
+  uint32_t crossing[8][3];   // ~order, key, place of a CTA's first crossing
+  uint32_t matches[8];       // the token's equals in a CTA's part of the row
 };
 
-__device__ __forceinline__ float key_value(uint32_t key) {
-  const uint16_t bits = (uint16_t)((key & 0x8000u) ? (key ^ 0x8000u) : (~key & 0xffffu));
-  return __half2float(__ushort_as_half(bits));
+__device__ __forceinline__ uint16_t key_bits(uint32_t key) {
+  return (uint16_t)(key < 0x8000u ? key ^ 0x7fffu : key);
+}
+__device__ __forceinline__ double key_value(uint32_t key) {
+  return (double)__half2float(__ushort_as_half(key_bits(key)));
+}
+// Descending keys of the two halves of a word: 0x7fff - bits for a positive
+// value, bits for a negative one.
+__device__ __forceinline__ uint32_t keys_of(uint32_t w) {
+  uint32_t negative;  // each half's sign, spread over it
+  asm("prmt.b32 %0, %1, 0, 0xBB99;" : "=r"(negative) : "r"(w));
+  return w ^ (~negative & 0x7fff7fffu);
 }
 
-// Sum over everything before this thread in descending key order, and over
-// the row. `sums` (this CTA's blocks) is read by the cluster.
+// A row as 16-byte words; places outside of it read as +inf, no candidate.
+struct Row {
+  const uint16_t* base;  // aligned down to 16 bytes
+  int from, to;          // the row's places from `base`
+  __device__ Row(const uint16_t* x, int n) {
+    from = (int)((reinterpret_cast<uintptr_t>(x) & 15) / 2);
+    base = x - from;
+    to = from + n;
+  }
+  __device__ int words() const { return (to + 7) / 8; }
+  __device__ uint4 word(int i) const {
+    if (8 * i >= from && 8 * i + 8 <= to) return reinterpret_cast<const uint4*>(base)[i];
+    uint32_t u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int a = 8 * i + 2 * e, b = a + 1;
+      const uint32_t lo = a >= from && a < to ? base[a] : 0x7c00u;
+      const uint32_t hi = b >= from && b < to ? base[b] : 0x7c00u;
+      u[e] = lo | hi << 16;
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+
+template <int kCtas>
+__device__ __forceinline__ void row_sync() {
+  if constexpr (kCtas == 1)
+    __syncthreads();
+  else
+    cg::this_cluster().sync();
+}
 template <int kCtas, class T>
-__device__ __forceinline__ T row_exclusive(cg::cluster_group& cluster, T v, T* warps, T* sums,
-                                           T& total) {
-  constexpr int kBlockWarps = kThreads / (kBlocks / kCtas) / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  T x = v;
+__device__ __forceinline__ T* of_rank(T* p, int rank) {
+  if constexpr (kCtas == 1)
+    return p;
+  else
+    return cg::this_cluster().map_shared_rank(p, rank);
+}
+
+// Sum over the row before this thread's keys, and over the row: v is the
+// thread's share of its block, which kGroup threads have; `own` takes this
+// CTA's blocks' sums for the cluster to read.
+template <int kCtas, int kGroup, class T>
+__device__ __forceinline__ T row_exclusive(int rank, T v, T* own, T* before, T* warps, T& total) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  T x = v;  // inclusive over the block's threads
+#pragma unroll
+  for (int o = 1; o < kGroup; o <<= 1) {
+    const T y = __shfl_up_sync(0xffffffffu, x, o, kGroup);
+    if (tid % kGroup >= o) x += y;
+  }
+  T up = __shfl_up_sync(0xffffffffu, x, 1, kGroup);
+  if (tid % kGroup == 0) up = T(0);
+  T z = x;
+  if constexpr (kCtas > 1) {
+    if (tid % kGroup == kGroup - 1) own[tid / kGroup] = x;
+    row_sync<kCtas>();
+    // block b of the row is block b / kCtas of CTA b % kCtas
+    z = of_rank<kCtas>(own, tid % kCtas)[tid / kCtas];
+  }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+    const T y = __shfl_up_sync(0xffffffffu, z, o);
+    if (lane >= o) z += y;
   }
-  if (lane == 31) warps[warp] = x;
-  T before = __shfl_up_sync(0xffffffffu, x, 1);
-  if (lane == 0) before = T(0);
+  if (lane == 31) warps[warp] = z;
   __syncthreads();
-  const int block = warp / kBlockWarps;
-  T all = T(0), base = T(0);
+  T w = warps[lane];
 #pragma unroll
-  for (int w = 0; w < kBlockWarps; ++w) {
-    const T y = warps[block * kBlockWarps + w];
-    if (w < warp % kBlockWarps) base += y;
-    all += y;
+  for (int o = 1; o < 32; o <<= 1) {
+    const T y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
   }
-  if (lane == 0 && warp % kBlockWarps == 0) sums[block] = all;
-  cluster.sync();
-  // block b of the row is block b / kCtas of CTA b % kCtas
-  const int mine = block * kCtas + (int)cluster.block_rank();
-  T earlier = T(0), every = T(0);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int b = lane + 32 * i;
-    const T y = cluster.map_shared_rank(sums, b % kCtas)[b / kCtas];
-    every += y;
-    if (b < mine) earlier += y;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    every += __shfl_xor_sync(0xffffffffu, every, o);
-    earlier += __shfl_xor_sync(0xffffffffu, earlier, o);
-  }
-  total = every;
-  return earlier + (base + before);
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const T base = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  T earlier = __shfl_up_sync(0xffffffffu, z, 1);
+  if (lane == 0) earlier = T(0);
+  if (warp) earlier += base;
+  if constexpr (kCtas == 1) return earlier;
+  before[tid] = earlier;
+  __syncthreads();
+  return before[tid / kGroup * kCtas + rank] + up;
 }
 
 template <int kCtas>
 __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleBatch p) {
   constexpr int kPer = 65536 / kCtas / kThreads;  // keys of a thread
-  constexpr int kBlockThreads = kBlockKeys / kPer;
+  constexpr int kGroup = kBlockKeys / kPer;       // threads of a block
+  static_assert(kPer % 8 == 0 && kGroup >= 1, "shape");
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank();
+  const int rank = kCtas == 1 ? 0 : (int)(blockIdx.x % kCtas);
   const int row = blockIdx.x / kCtas;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   for (int i = tid; i < 65536 / 8; i += kThreads)
     reinterpret_cast<uint4*>(sh.hist)[i] = make_uint4(0, 0, 0, 0);
   if (tid == 0) {
-    sh.top = 0;
+    sh.least = 0xFFFFu;
     sh.last = 0;
     sh.first = 0;
-    sh.key = 0;
+    sh.large = 0;
+    sh.kept_order = 0;
   }
   pdl_trigger();
   pdl_wait();
@@ -131,225 +197,333 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
   const bool fine = temperature >= 0.f && temperature <= 3.4028234664e38f && top_p >= 0.f &&
                     top_p <= 1.f && min_p >= 0.f && min_p <= 1.f && uniform >= 0.f &&
                     uniform < 1.f;
-  if (!fine) {  // the same in every CTA of the cluster
+  if (!fine) {  // the same in every CTA of the row
     if (rank == 0 && tid == 0) {
       p.tokens[row] = 0xFFFFFFFEu;
       report_fault(p.fault, kFaultSampling);
     }
     return;
   }
+  const double inverse = 1.0 / (double)temperature;
+  if (tid < 64) {
+    // values of exponent e are 2^(max(e, 1) - 25) apart
+    sh.step[tid] = exp(-ldexp(1.0, max(tid & 31, 1) - 25) * inverse);
+  }
   __syncthreads();
 
   // ---- count ---------------------------------------------------------------------
-  const uint16_t* x = reinterpret_cast<const uint16_t*>(p.logits) + (size_t)row * p.n;
-  const int chunk = ((p.n + kCtas - 1) / kCtas + 7) / 8 * 8;
-  const int first = min(p.n, rank * chunk), last = min(p.n, first + chunk);
-  uint32_t top = 0;
-  auto count = [&](uint32_t bits) {
-    if ((bits & 0x7c00u) != 0x7c00u) {
-      const uint32_t key = sample_key16((uint16_t)bits);
-      top = max(top, key + 1);
-      atomicAdd(&sh.hist[key >> 1], 1u << (16 * (key & 1)));
-    }
-  };
+  const Row x(reinterpret_cast<const uint16_t*>(p.logits) + (size_t)row * p.n, p.n);
+  // this CTA's words
+  const int share = (x.words() + kCtas - 1) / kCtas;
+  const int w0 = min(x.words(), rank * share), w1 = min(x.words(), w0 + share);
   {
-    // 16-byte words of the range, and what lies before and behind them
-    const int head =
-        min(last - first, (int)((16 - (reinterpret_cast<uintptr_t>(x + first) & 15)) & 15) / 2);
-    const int words = (last - first - head) / 8;
-    if (tid < head) count(x[first + tid]);
-    const uint4* w = reinterpret_cast<const uint4*>(x + first + head);
+    uint32_t least = 0xFFFFFFFFu;  // two smallest key - kFirst, wrapped below it
+    auto add = [&](uint32_t d, uint32_t n) {
+      if (d - kFirst < kEnd - kFirst) atomicAdd(&sh.hist[d >> 1], n << (16 * (d & 1)));
+    };
+    for (int a = w0; a < w1; a += kSegment / 8) {
+      const int b = min(w1, a + kSegment / 8);
 #pragma unroll 2
-    for (int i = tid; i < words; i += kThreads) {
-      const uint4 v = w[i];
-      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+      for (int i = a + tid; i - lane < b; i += kThreads) {
+        const uint4 v = i < b ? x.word(i) : make_uint4(0x7c007c00u, 0x7c007c00u, 0x7c007c00u, 0x7c007c00u);
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        // a stretch of one value (a mask) is one addition
+        const uint32_t one = __shfl_sync(0xffffffffu, v.x, 0);
+        const bool same = v.x == one && v.y == one && v.z == one && v.w == one;
+        if (__all_sync(0xffffffffu, same) && (one & 0xffffu) == one >> 16) {
+          const uint32_t d = keys_of(one);
+          least = __viaddmin_u16x2(d, 0xFC00FC00u, least);
+          if (lane == 0) add(d & 0xffffu, 256);
+          continue;
+        }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        count(u[e] & 0xffffu);
-        count(u[e] >> 16);
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t d = keys_of(u[e]);
+          least = __viaddmin_u16x2(d, 0xFC00FC00u, least);
+          add(d & 0xffffu, 1);
+          add(d >> 16, 1);
+        }
+      }
+      if (b < w1) {  // more to come: room in every count
+        __syncthreads();
+        for (int i = tid; i < 65536 / 2; i += kThreads) {
+          const uint32_t c = sh.hist[i];
+          if ((c & 0xffffu) > kLarge || c >> 16 > kLarge) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t n = (c >> (16 * h)) & 0xffffu;
+              if (n > kLarge) {
+                const uint32_t at = atomicAdd(&sh.large, 1u);
+                sh.large_key[at] = 2 * i + h;
+                sh.large_count[at] = n;
+                reinterpret_cast<uint16_t*>(sh.hist)[2 * i + h] = 0;
+              }
+            }
+          }
+        }
+        __syncthreads();
       }
     }
-    const int tail = first + head + words * 8 + tid;
-    if (tail < last) count(x[tail]);
+    least = __reduce_min_sync(0xffffffffu, min(least & 0xffffu, least >> 16));
+    if (lane == 0) atomicMin(&sh.least, least);
   }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0 && top) atomicMax(&sh.top, top);
-  cluster.sync();
-  top = 0;
-#pragma unroll
-  for (int c = 0; c < kCtas; ++c) top = max(top, *cluster.map_shared_rank(&sh.top, c));
-
-  // ---- this thread's keys, descending: high - 1 ... high - kPer ----------------------
-  const int block = tid / kBlockThreads * kCtas + rank;
-  const int high = 65536 - block * kBlockKeys - tid % kBlockThreads * kPer;
-  const uint32_t order = block * kBlockThreads + tid % kBlockThreads;
-  uint32_t c[kPer] = {};
+  row_sync<kCtas>();
+  uint32_t top = 0xFFFFu, large = 0;  // the row's largest value, as a descending key
 #pragma unroll
   for (int r = 0; r < kCtas; ++r) {
-    const uint4* h =
-        reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.hist, r) + (high - kPer) / 2);
-#pragma unroll
-    for (int i = 0; i < kPer / 8; ++i) {
-      const uint4 v = h[i];
-      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        c[kPer - 1 - 8 * i - 2 * e] += u[e] & 0xffffu;
-        c[kPer - 2 - 8 * i - 2 * e] += u[e] >> 16;
-      }
-    }
+    top = min(top, *of_rank<kCtas>(&sh.least, r));
+    large |= *of_rank<kCtas>(&sh.large, r);
   }
-  if (top == 0) {
-    // no finite logit
-  } else if (temperature == 0.f) {
-    if (rank == 0 && tid == 0) {
-      sh.first = ~0u;
-      sh.key = top;
-      sh.place = 0;
-    }
-  } else {
-    if (top_k) {  // the first top_k candidates stay
-      uint32_t own = 0, all;
+  top += kFirst;
+
+  uint32_t key = top, place = 0;
+  if (top < kEnd && temperature != 0.f) {
+    // ---- this thread's keys: low ... low + kPer - 1 ---------------------------------
+    const uint32_t block = tid / kGroup * kCtas + rank;
+    const uint32_t low = block * kBlockKeys + tid % kGroup * kPer;
+    const uint32_t order = low / kPer;
+    const double most = key_value(top);
+    // Counts of eight keys, over the cluster.
+    auto counts = [&](int g, uint32_t (&c)[8]) {
+      const uint32_t k0 = low + 8 * g;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) own += c[e];
-      uint32_t at = row_exclusive<kCtas>(cluster, own, sh.warp_count, sh.count, all);
+      for (int e = 0; e < 8; ++e) c[e] = 0;
+      if (k0 < top / 8 * 8 || k0 >= kEnd) return;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const uint32_t n = c[e];
-        c[e] = at >= top_k ? 0u : min(n, top_k - at);
-        at += n;
-      }
-    }
-    const double most = (double)key_value(top - 1), inverse = 1.0 / (double)temperature;
-    double w[kPer], own = 0.0, total;
+      for (int r = 0; r < kCtas; ++r) {
+        const uint4 v = *reinterpret_cast<const uint4*>(of_rank<kCtas>(sh.hist, r) + k0 / 2);
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      w[e] = c[e] ? exp(((double)key_value(high - 1 - e) - most) * inverse) : 0.0;
-      own += c[e] * w[e];
-    }
-    const double at = row_exclusive<kCtas>(cluster, own, sh.warp_mass, sh.mass, total);
-    // What top_p and min_p keep is a prefix again: the kept sum is the sum at
-    // the end of the last kept group.
-    const double limit = top_p >= 1.f ? INFINITY : (double)top_p * total;
-    double kept = -1.0, sum = at;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      uint32_t n = w[e] >= (double)min_p ? c[e] : 0u;
-      if (n && !(sum + (n - 1) * w[e] < limit)) {
-        // places j with sum + j w < limit
-        uint32_t m = 0;
-        if (sum < limit) {
-          const double j = ceil((limit - sum) / w[e]);
-          m = j >= (double)n ? n : (uint32_t)j;
-          if (m && !(sum + (m - 1) * w[e] < limit)) --m;
-          else if (m < n && sum + m * w[e] < limit) ++m;
+        for (int e = 0; e < 4; ++e) {
+          c[2 * e] += u[e] & 0xffffu;
+          c[2 * e + 1] += u[e] >> 16;
         }
-        n = m;
       }
-      if (c[e] && n == 0 && (uint32_t)(high - e) == top) n = 1;  // the first always stays
-      if (n) kept = sum + n * w[e];
-      sum += c[e] * w[e];
-      c[e] = n;
-    }
-    const uint32_t mine = kept >= 0.0 ? order + 1 : 0u;
-    const uint32_t warp_last = __reduce_max_sync(0xffffffffu, mine);
-    if (lane == 0 && warp_last) atomicMax(&sh.last, warp_last);
-    __syncthreads();
-    if (mine && sh.last == mine) sh.kept = kept;
-    cluster.sync();
-    uint32_t final = 0;
-    double sum_kept = 0.0;
+      if (large)
+        for (int r = 0; r < kCtas; ++r) {
+          const uint32_t n = *of_rank<kCtas>(&sh.large, r);
+          for (uint32_t i = 0; i < n; ++i) {
+            const uint32_t k = of_rank<kCtas>(sh.large_key, r)[i] - k0;
 #pragma unroll
-    for (int r = 0; r < kCtas; ++r) {
-      const uint32_t q = *cluster.map_shared_rank(&sh.last, r);
-      if (q > final) {
-        final = q;
-        sum_kept = *cluster.map_shared_rank(&sh.kept, r);
+            for (int e = 0; e < 8; ++e)
+              if (k == e) c[e] += of_rank<kCtas>(sh.large_count, r)[i];
+          }
+        }
+    };
+    // Runs f(key, count, weight) over this thread's candidates in order; `at`
+    // is the count of candidates before them, of which top_k stay.
+    auto walk = [&](uint32_t at, auto f) {
+#pragma unroll 1
+      for (int g = 0; g < kPer / 8; ++g) {
+        uint32_t c[8], any = 0;
+        counts(g, c);
+        if (top_k) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t n = c[e];
+            c[e] = at >= top_k ? 0u : min(n, top_k - at);
+            at += n;
+          }
+        }
+#pragma unroll
+        for (int e = 7; e >= 0; --e)
+          if (c[e]) any = e + 1;
+        if (!any) continue;
+        const uint32_t k0 = low + 8 * g, k1 = k0 + any - 1;  // the first that has a count
+        double w = exp((key_value(k1) - most) * inverse);
+        const double step = sh.step[key_bits(k0) >> 10];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (c[e]) f(k0 + e, c[e], w);
+          if (k0 + e >= k1) w *= step;
+        }
+      }
+    };
+    uint32_t at_count = 0;
+    if (top_k) {
+      uint32_t own = 0, all;
+#pragma unroll 1
+      for (int g = 0; g < kPer / 8; ++g) {
+        uint32_t c[8];
+        counts(g, c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) own += c[e];
+      }
+      at_count = row_exclusive<kCtas, kGroup>(rank, own, sh.count, (uint32_t*)sh.before,
+                                              sh.warp_count, all);
+      __syncthreads();  // `before` is used again
+    }
+    double own = 0.0, lightest = INFINITY, total;
+    walk(at_count, [&](uint32_t, uint32_t n, double w) {
+      own += n * w;
+      lightest = w;
+    });
+    const double at =
+        row_exclusive<kCtas, kGroup>(rank, own, sh.mass, sh.before, sh.warp_mass, total);
+    // What top_p and min_p keep is a prefix again: the kept sum is the sum at
+    // the end of the last kept candidate. Only the threads around a border
+    // look at their candidates one by one.
+    const bool cut = top_p < 1.f || min_p > 0.f;
+    const double limit = top_p >= 1.f ? INFINITY : (double)top_p * total;
+    const bool mine_top = top - low < (uint32_t)kPer;
+    // f(key, kept count, weight, sum before it)
+    auto walk_kept = [&](auto f) {
+      double sum = at;
+      walk(at_count, [&](uint32_t k, uint32_t c, double w) {
+        uint32_t n = w >= (double)min_p ? c : 0u;
+        if (n && !(sum + (n - 1) * w < limit)) {
+          // places j with sum + j w < limit
+          uint32_t m = 0;
+          if (sum < limit) {
+            const double j = ceil((limit - sum) / w);
+            m = j >= (double)n ? n : (uint32_t)j;
+            if (m && !(sum + (m - 1) * w < limit)) --m;
+            else if (m < n && sum + m * w < limit) ++m;
+          }
+          n = m;
+        }
+        if (k == top && n == 0) n = 1;  // the first always stays
+        if (n) f(k, n, w, sum);
+        sum += c * w;
+      });
+    };
+    double end = at + own;  // where this thread's kept candidates end
+    bool has = own > 0.0;
+    if (cut && has && !(end < limit && lightest >= (double)min_p)) {
+      has = false;
+      if (at < limit || mine_top)
+        walk_kept([&](uint32_t, uint32_t n, double w, double sum) {
+          has = true;
+          end = sum + n * w;
+        });
+    }
+    double sum_kept = total;
+    if (cut) {
+      const uint32_t mine = has ? order + 1 : 0u;
+      const uint32_t warp_last = __reduce_max_sync(0xffffffffu, mine);
+      if (lane == 0 && warp_last) atomicMax(&sh.last, warp_last);
+      __syncthreads();
+      if (mine && sh.last == mine) {
+        sh.kept = end;
+        sh.kept_order = mine;
+      }
+      row_sync<kCtas>();
+      uint32_t final = 0;
+#pragma unroll
+      for (int r = 0; r < kCtas; ++r) {
+        const uint32_t q = *of_rank<kCtas>(&sh.kept_order, r);
+        const double e = *of_rank<kCtas>(&sh.kept, r);
+        if (q > final) {
+          final = q;
+          sum_kept = e;
+        }
       }
     }
-    // The first group whose sum exceeds the target: there is one, as the
-    // last kept group's sum is the kept sum itself. Threads' sums meet within
-    // rounding only, so the first of all is taken, not the one around it.
+    // The first thread whose sum exceeds the target: there is one, as uniform
+    // is at most 1 - 2^-24 and sums agree to about 1e-15. Threads' sums meet
+    // within rounding only, so the first of all is taken, not the one around it.
     const double target = (double)uniform * sum_kept;
-    bool crosses = false;
-    sum = at;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      if (c[e] && sum + c[e] * w[e] > target) crosses = true;
-      sum += c[e] * w[e];
-    }
-    const uint32_t hit = crosses ? ~order : 0u;
+    const uint32_t hit = has && end > target ? ~order : 0u;
     const uint32_t warp_first = __reduce_max_sync(0xffffffffu, hit);
     if (lane == 0 && warp_first) atomicMax(&sh.first, warp_first);
     __syncthreads();
-    if (hit && sh.first == hit) {
-      sum = at;
+    const uint32_t found = sh.first;
+    if (hit ? found == hit : found == 0 && tid == 0) {
+      uint32_t token = 0, where = 0;
+      if (hit) {
+        bool crossed = false;
+        walk_kept([&](uint32_t k, uint32_t n, double w, double sum) {
+          if (crossed) return;
+          // its first place whose sum exceeds the target; the last candidate
+          // of the thread where rounding leaves none
+          const double j = floor((target - sum) / w);
+          uint32_t m = j <= 0.0 ? 0u : j >= (double)n ? n - 1 : (uint32_t)j;
+          if (sum + (m + 1) * w <= target && m + 1 < n) ++m;
+          else if (m && sum + m * w > target) --m;
+          crossed = sum + (m + 1) * w > target;
+          token = k;
+          where = m;
+        });
+      }
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        if (crosses && c[e] && sum + c[e] * w[e] > target) {
-          const double j = floor((target - sum) / w[e]);
-          uint32_t m = j <= 0.0 ? 0u : j >= (double)c[e] ? c[e] - 1 : (uint32_t)j;
-          if (sum + (m + 1) * w[e] <= target && m + 1 < c[e]) ++m;
-          else if (m && sum + m * w[e] > target) --m;
-          sh.key = high - e;
-          sh.place = m;
-          crosses = false;
-        }
-        sum += c[e] * w[e];
+      for (int r = 0; r < kCtas; ++r) {
+        uint32_t* out = of_rank<kCtas>(&sh.crossing[rank][0], r);
+        out[0] = hit;
+        out[1] = token;
+        out[2] = where;
       }
     }
+    row_sync<kCtas>();
+    uint32_t best = 0;
+#pragma unroll
+    for (int r = 0; r < kCtas; ++r)
+      if (sh.crossing[r][0] > best) {
+        best = sh.crossing[r][0];
+        key = sh.crossing[r][1];
+        place = sh.crossing[r][2];
+      }
   }
-  cluster.sync();
 
   // ---- key and place to an index -----------------------------------------------------
-  uint32_t key = 0, place = 0, best = 0;
-#pragma unroll
-  for (int r = 0; r < kCtas; ++r) {
-    const uint32_t q = *cluster.map_shared_rank(&sh.first, r);
-    if (q > best) {
-      best = q;
-      key = *cluster.map_shared_rank(&sh.key, r);
-      place = *cluster.map_shared_rank(&sh.place, r);
-    }
-  }
-  if (key == 0) {
+  // Each warp takes a run of its CTA's words: equals per warp, then the warp
+  // that holds the place looks for it.
+  if (top >= kEnd) {
     if (rank == 0 && tid == 0) p.tokens[row] = 0xFFFFFFFFu;
   } else {
-    --key;
-    int at = (int)place;  // place among this CTA's and later ones' equals
-    for (int r = 0; r < rank; ++r)
-      at -= (cluster.map_shared_rank(sh.hist, r)[key >> 1] >> (16 * (key & 1))) & 0xffffu;
-    const int here = (sh.hist[key >> 1] >> (16 * (key & 1))) & 0xffffu;
-    if (at >= 0 && at < here) {
-      // each warp takes a run of the range: equals per warp, then the warp
-      // that holds the place walks its run
-      const int run = (last - first + kWarps * 32 - 1) / (kWarps * 32) * 32;
-      const int a = min(last, first + warp * run), b = min(last, a + run);
-      // the FP16 bits of the key
-      const uint16_t bits = (uint16_t)((key & 0x8000u) ? (key ^ 0x8000u) : (~key & 0xffffu));
-      int equals = 0;
+    const uint32_t bits = key_bits(key) * 0x10001u;
+    const int run = (w1 - w0 + kWarps - 1) / kWarps;
+    const int a = min(w1, w0 + warp * run), b = min(w1, a + run);
+    auto equal = [&](int i) {  // a bit for each of the word's equals
+      if (i >= b) return 0u;
+      const uint4 v = x.word(i);
+      const uint32_t u[4] = {v.x ^ bits, v.y ^ bits, v.z ^ bits, v.w ^ bits};
+      uint32_t mask = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        mask |= ((u[e] & 0xffffu) == 0 ? 1u << (2 * e) : 0u) |
+                (u[e] >> 16 == 0 ? 2u << (2 * e) : 0u);
+      return mask;
+    };
+    uint32_t equals = 0;
 #pragma unroll 4
-      for (int i = a; i < b; i += 32)
-        equals += __popc(__ballot_sync(0xffffffffu, i + lane < b && x[i + lane] == bits));
-      if (lane == 0) sh.equals[warp] = equals;
-      __syncthreads();
-      int rest = at;
-      for (int q = 0; q < warp; ++q) rest -= (int)sh.equals[q];
-      if (rest >= 0 && rest < equals) {
-        for (int i = a; i < b; i += 32) {
-          const bool eq = i + lane < b && x[i + lane] == bits;
-          const unsigned hits = __ballot_sync(0xffffffffu, eq);
-          const int n = __popc(hits);
-          if (rest < n) {
-            if (eq && __popc(hits & ((1u << lane) - 1)) == rest) p.tokens[row] = i + lane;
-            break;
-          }
-          rest -= n;
+    for (int i = a + lane; i < b; i += 32) equals += __popc(equal(i));
+    equals = __reduce_add_sync(0xffffffffu, equals);
+    if (lane == 0) sh.equals[warp] = equals;
+    __syncthreads();
+    int rest = (int)place;
+    if constexpr (kCtas > 1) {
+      if (warp == 0) {
+        const uint32_t all = __reduce_add_sync(0xffffffffu, sh.equals[lane]);
+        if (lane < kCtas) *of_rank<kCtas>(&sh.matches[rank], lane) = all;
+      }
+      row_sync<kCtas>();
+      for (int r = 0; r < rank; ++r) rest -= (int)sh.matches[r];
+    }
+    for (int q = 0; q < warp; ++q) rest -= (int)sh.equals[q];
+    if (rest >= 0 && rest < (int)equals) {
+      for (int i = a; i < b; i += 32) {
+        uint32_t mask = equal(i + lane);
+        int n = __popc(mask), upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += y;
         }
+        const int all = __shfl_sync(0xffffffffu, upto, 31);
+        if (rest < all) {
+          int j = rest - (upto - n);  // of this lane's equals
+          if (j >= 0 && j < n) {
+            for (; j > 0; --j) mask &= mask - 1;
+            p.tokens[row] = 8 * (i + lane) + __ffs(mask) - 1 - x.from;
+          }
+          break;
+        }
+        rest -= all;
       }
     }
   }
-  cluster.sync();  // no CTA leaves while another reads its shared memory
+  // no CTA leaves while another reads its shared memory
+  if constexpr (kCtas > 1) row_sync<kCtas>();
 }
 
 template <int kCtas>
@@ -379,13 +553,12 @@ void launch_sample(const Launch& l, const SampleBatch& p) {
 
 void sample_batch(const Launch& l, const SampleBatch& p) {
   if (p.rows == 0) return;
-  // Four CTAs to a row leave fewer fixed costs, eight are quicker with a row:
-  // eight while the rows fit the GPU at once, or where a CTA's share of the
-  // row would outgrow its 16-bit counts.
-  if (p.rows * 8 <= l.sm_count || p.n > 4 * 65528)
+  // Clusters of 8 while the rows fit the GPU at once so, one CTA to a row
+  // otherwise.
+  if (p.rows * 8 <= l.sm_count)
     launch_sample<8>(l, p);
   else
-    launch_sample<4>(l, p);
+    launch_sample<1>(l, p);
 }
 
 }  // namespace k

@@ -808,5 +808,7 @@ def test_refusals(ctx):
     refused(mi.ERR_SHAPE, "per-row", sample_with(p=f(3)))
     refused(mi.ERR_DTYPE, "top_k", sample_with(k=f(2)))
     refused(mi.ERR_SHAPE, "logits a row", sample_with(x=e(2, 0)))
-    refused(mi.ERR_SHAPE, "logits a row", sample_with(x=e(2, 524225)))
+    few = e(64)  # shapes are refused before anything is read
+    huge = ctx.tensor_from_device(few.data_ptr(), [2, 2 ** 22 + 1], F16)
+    refused(mi.ERR_SHAPE, "logits a row", sample_with(x=huge, o=u(2)))
     refused(mi.ERR_INVALID_ARGUMENT, "NULL", lambda b: mi._check(mi.lib().mi_batch_sample(b._h, *[None] * 7)))
