@@ -37,8 +37,8 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBlockKeys = 64;
-constexpr int kBlocks = 65536 / kBlockKeys;
+constexpr int kGroups = 65536 / 8;  // of eight keys
+constexpr int kBlocks = kGroups / 8; // a cluster's CTAs take blocks of 64 keys by turns
 static_assert(kBlocks == kThreads, "a thread takes a block's sum");
 // Finite keys, descending: 65535 - the order key, so that the largest value
 // comes first; infinities and NaN lie outside of [kFirst, kEnd).
@@ -49,23 +49,31 @@ constexpr int kSegment = 49152;
 constexpr uint32_t kLarge = 65535 - kSegment;
 constexpr int kLargeMax = kSampleBatchMax / (int)kLarge + 1;
 
+// A thread has groups of eight keys: one where a cluster shares the row, and
+// 8 of a CTA's own, 1,024 groups apart, so that the few exponents that hold
+// most of a row keep all warps busy.
+template <int kCtas>
+constexpr int kRounds = kGroups / kThreads / kCtas;
+
+template <int kCtas>
 struct Shared {
   uint32_t hist[65536 / 2];  // two 16-bit counts to a word
-  double before[kBlocks];    // sum before each block of the row
-  double warp_mass[kWarps];
+  double mass[kRounds<kCtas>][kThreads];  // sum of a thread's candidates, per round
+  double warp_sums[kRounds<kCtas> * kWarps];
+  double total;
+  double blocks_before[kCtas == 1 ? 1 : kBlocks];
   double step[64];           // weight of one step of an exponent's values (sign in front)
-  uint32_t warp_count[kWarps];
   uint32_t equals[kWarps];
-  uint32_t least;            // smallest key of this CTA's part - kFirst
-  uint32_t last, first;      // order + 1 of the last kept thread, ~order of the first that crosses
+  uint32_t last, first;      // order + 1 of the last kept group, ~order of the first that crosses
   // read by the cluster's other CTAs
+  uint32_t least;            // smallest key of this CTA's part - kFirst
   uint32_t large;            // counts moved out of the histogram
   uint32_t large_key[kLargeMax], large_count[kLargeMax];
-  double mass[kBlocks];      // sums of this CTA's blocks
-  uint32_t count[kBlocks];
+  double block_sums[kCtas == 1 ? 1 : kBlocks / kCtas];
   double kept;               // running sum where this CTA's kept candidates end
-  uint32_t kept_order;       // order + 1 of the thread that has it, 0: none
+  uint32_t kept_order;       // order + 1 of the group that has it, 0: none
   // written by them
+  uint32_t cutoff[8][3];     // ~order, key, count of it that top_k leaves (a CTA's first)
   uint32_t crossing[8][3];   // ~order, key, place of a CTA's first crossing
   uint32_t matches[8];       // the token's equals in a CTA's part of the row
 };
@@ -88,14 +96,17 @@ __device__ __forceinline__ uint32_t keys_of(uint32_t w) {
 struct Row {
   const uint16_t* base;  // aligned down to 16 bytes
   int from, to;          // the row's places from `base`
+  int whole0, whole1;    // words that lie inside
   __device__ Row(const uint16_t* x, int n) {
     from = (int)((reinterpret_cast<uintptr_t>(x) & 15) / 2);
     base = x - from;
     to = from + n;
+    whole0 = from ? 1 : 0;
+    whole1 = to / 8;
   }
   __device__ int words() const { return (to + 7) / 8; }
   __device__ uint4 word(int i) const {
-    if (8 * i >= from && 8 * i + 8 <= to) return reinterpret_cast<const uint4*>(base)[i];
+    if (i >= whole0 && i < whole1) return reinterpret_cast<const uint4*>(base)[i];
     uint32_t u[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -105,6 +116,20 @@ struct Row {
       u[e] = lo | hi << 16;
     }
     return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  // Words i, i + stride, ..., kMany of them (nothing from `end` on): the loads
+  // of words inside the row are in flight together.
+  template <int kMany>
+  __device__ void load(uint4 (&v)[kMany], int i, int stride, int end) const {
+    if (i >= whole0 && i + (kMany - 1) * stride < min(whole1, end)) {
+#pragma unroll
+      for (int k = 0; k < kMany; ++k) v[k] = reinterpret_cast<const uint4*>(base)[i + k * stride];
+    } else {
+#pragma unroll
+      for (int k = 0; k < kMany; ++k)
+        v[k] = i + k * stride < end ? word(i + k * stride)
+                                    : make_uint4(0x7c007c00u, 0x7c007c00u, 0x7c007c00u, 0x7c007c00u);
+    }
   }
 };
 
@@ -123,58 +148,136 @@ __device__ __forceinline__ T* of_rank(T* p, int rank) {
     return cg::this_cluster().map_shared_rank(p, rank);
 }
 
-// Sum over the row before this thread's keys, and over the row: v is the
-// thread's share of its block, which kGroup threads have; `own` takes this
-// CTA's blocks' sums for the cluster to read.
-template <int kCtas, int kGroup, class T>
-__device__ __forceinline__ T row_exclusive(int rank, T v, T* own, T* before, T* warps, T& total) {
+// Sums over the row before each of a thread's groups, and over the row: a
+// count or a sum of weights, v[r] the thread's of round r.
+template <int kCtas, class T>
+__device__ __forceinline__ T row_exclusive(Shared<kCtas>& sh, int rank,
+                                           const T (&v)[kRounds<kCtas>],
+                                           T (&before)[kRounds<kCtas>]) {
+  constexpr int kR = kRounds<kCtas>;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  T x = v;  // inclusive over the block's threads
+  T* sums = reinterpret_cast<T*>(sh.warp_sums);
+  __syncthreads();
+  if constexpr (kCtas == 1) {
 #pragma unroll
-  for (int o = 1; o < kGroup; o <<= 1) {
-    const T y = __shfl_up_sync(0xffffffffu, x, o, kGroup);
-    if (tid % kGroup >= o) x += y;
-  }
-  T up = __shfl_up_sync(0xffffffffu, x, 1, kGroup);
-  if (tid % kGroup == 0) up = T(0);
-  T z = x;
-  if constexpr (kCtas > 1) {
-    if (tid % kGroup == kGroup - 1) own[tid / kGroup] = x;
+    for (int r = 0; r < kR; ++r) {
+      T x = v[r];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const T y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31) sums[r * kWarps + warp] = x;
+      before[r] = __shfl_up_sync(0xffffffffu, x, 1);
+      if (lane == 0) before[r] = T(0);
+    }
+    __syncthreads();
+    if (warp == 0) {  // eight warp sums to a lane
+      T z = T(0);
+#pragma unroll
+      for (int i = 0; i < kR; ++i) z += sums[lane * kR + i];
+      T x = z;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const T y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      T at = __shfl_up_sync(0xffffffffu, x, 1);
+      if (lane == 0) at = T(0);
+#pragma unroll
+      for (int i = 0; i < kR; ++i) {
+        const T y = sums[lane * kR + i];
+        sums[lane * kR + i] = at;
+        at += y;
+      }
+      if (lane == 31) *reinterpret_cast<T*>(&sh.total) = at;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kR; ++r) before[r] += sums[r * kWarps + warp];
+    return *reinterpret_cast<T*>(&sh.total);
+  } else {
+    // eight threads to a block; block b of the row is block b / kCtas of CTA
+    // b % kCtas. Each CTA adds up all blocks.
+    T x = v[0];
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      const T y = __shfl_up_sync(0xffffffffu, x, o, 8);
+      if (tid % 8 >= o) x += y;
+    }
+    T up = __shfl_up_sync(0xffffffffu, x, 1, 8);
+    if (tid % 8 == 0) up = T(0);
+    T* own = reinterpret_cast<T*>(sh.block_sums);
+    T* all = reinterpret_cast<T*>(sh.blocks_before);
+    if (tid % 8 == 7) own[tid / 8] = x;
     row_sync<kCtas>();
-    // block b of the row is block b / kCtas of CTA b % kCtas
-    z = of_rank<kCtas>(own, tid % kCtas)[tid / kCtas];
-  }
+    T z = of_rank<kCtas>(own, tid % kCtas)[tid / kCtas];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(0xffffffffu, z, o);
-    if (lane >= o) z += y;
-  }
-  if (lane == 31) warps[warp] = z;
-  __syncthreads();
-  T w = warps[lane];
+    for (int o = 1; o < 32; o <<= 1) {
+      const T y = __shfl_up_sync(0xffffffffu, z, o);
+      if (lane >= o) z += y;
+    }
+    if (lane == 31) sums[warp] = z;
+    __syncthreads();
+    T w = sums[lane];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += y;
+    for (int o = 1; o < 32; o <<= 1) {
+      const T y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    const T total = __shfl_sync(0xffffffffu, w, 31);
+    const T base = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+    T earlier = __shfl_up_sync(0xffffffffu, z, 1);
+    if (lane == 0) earlier = T(0);
+    if (warp) earlier += base;
+    all[tid] = earlier;
+    __syncthreads();
+    before[0] = all[tid / 8 * kCtas + rank] + up;
+    return total;
   }
-  total = __shfl_sync(0xffffffffu, w, 31);
-  const T base = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-  T earlier = __shfl_up_sync(0xffffffffu, z, 1);
-  if (lane == 0) earlier = T(0);
-  if (warp) earlier += base;
-  if constexpr (kCtas == 1) return earlier;
-  before[tid] = earlier;
+}
+
+// Which of the row's threads comes first: `order` of this one where it has
+// `hit`. The CTA's first runs f(out) and leaves out[0..1] beside ~order in
+// `to` of every CTA; returns the row's first of them (0: none has hit).
+template <int kCtas, class F>
+__device__ __forceinline__ bool row_first(Shared<kCtas>& sh, int rank, bool has, uint32_t order,
+                                          uint32_t (*to)[3], F f, uint32_t& a, uint32_t& b) {
+  const uint32_t hit = has ? ~order : 0u;
+  const uint32_t warp_first = __reduce_max_sync(0xffffffffu, hit);
+  if ((threadIdx.x & 31) == 0 && warp_first) atomicMax(&sh.first, warp_first);
   __syncthreads();
-  return before[tid / kGroup * kCtas + rank] + up;
+  const uint32_t found = sh.first;
+  if (hit ? found == hit : found == 0 && threadIdx.x == 0) {
+    uint32_t out[2] = {0, 0};
+    if (hit) f(out);
+#pragma unroll
+    for (int r = 0; r < kCtas; ++r) {
+      uint32_t* q = of_rank<kCtas>(&to[rank][0], r);
+      q[0] = hit;
+      q[1] = out[0];
+      q[2] = out[1];
+    }
+  }
+  row_sync<kCtas>();
+  if (threadIdx.x == 0) sh.first = 0;
+  uint32_t best = 0;
+#pragma unroll
+  for (int r = 0; r < kCtas; ++r)
+    if (to[r][0] > best) {
+      best = to[r][0];
+      a = to[r][1];
+      b = to[r][2];
+    }
+  return best != 0;
 }
 
 template <int kCtas>
 __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleBatch p) {
-  constexpr int kPer = 65536 / kCtas / kThreads;  // keys of a thread
-  constexpr int kGroup = kBlockKeys / kPer;       // threads of a block
-  static_assert(kPer % 8 == 0 && kGroup >= 1, "shape");
+  constexpr int kR = kRounds<kCtas>;
+  static_assert(kCtas == 1 || kR == 1, "a thread of a cluster has one group");
   extern __shared__ __align__(16) uint8_t smem[];
-  Shared& sh = *reinterpret_cast<Shared*>(smem);
+  Shared<kCtas>& sh = *reinterpret_cast<Shared<kCtas>*>(smem);
   const int rank = kCtas == 1 ? 0 : (int)(blockIdx.x % kCtas);
   const int row = blockIdx.x / kCtas;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -221,27 +324,32 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
     auto add = [&](uint32_t d, uint32_t n) {
       if (d - kFirst < kEnd - kFirst) atomicAdd(&sh.hist[d >> 1], n << (16 * (d & 1)));
     };
+    constexpr int kMany = 3;
+    static_assert(kSegment % (8 * kMany * kThreads) == 0, "whole steps to a segment");
     for (int a = w0; a < w1; a += kSegment / 8) {
       const int b = min(w1, a + kSegment / 8);
-#pragma unroll 2
-      for (int i = a + tid; i - lane < b; i += kThreads) {
-        const uint4 v = i < b ? x.word(i) : make_uint4(0x7c007c00u, 0x7c007c00u, 0x7c007c00u, 0x7c007c00u);
-        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-        // a stretch of one value (a mask) is one addition
-        const uint32_t one = __shfl_sync(0xffffffffu, v.x, 0);
-        const bool same = v.x == one && v.y == one && v.z == one && v.w == one;
-        if (__all_sync(0xffffffffu, same) && (one & 0xffffu) == one >> 16) {
-          const uint32_t d = keys_of(one);
-          least = __viaddmin_u16x2(d, 0xFC00FC00u, least);
-          if (lane == 0) add(d & 0xffffu, 256);
-          continue;
-        }
+      for (int i = a + tid; i - lane < b; i += kMany * kThreads) {
+        uint4 v[kMany];
+        x.load(v, i, kThreads, b);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t d = keys_of(u[e]);
-          least = __viaddmin_u16x2(d, 0xFC00FC00u, least);
-          add(d & 0xffffu, 1);
-          add(d >> 16, 1);
+        for (int k = 0; k < kMany; ++k) {
+          const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          // a stretch of one value (a mask) is one addition
+          const uint32_t one = __shfl_sync(0xffffffffu, u[0], 0);
+          const bool same = u[0] == one && u[1] == one && u[2] == one && u[3] == one;
+          if (__all_sync(0xffffffffu, same) && (one & 0xffffu) == one >> 16) {
+            const uint32_t d = keys_of(one);
+            least = __viaddmin_u16x2(d, 0xFC00FC00u, least);
+            if (lane == 0) add(d & 0xffffu, 256);
+            continue;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t d = keys_of(u[e]);
+            least = __viaddmin_u16x2(d, 0xFC00FC00u, least);
+            add(d & 0xffffu, 1);
+            add(d >> 16, 1);
+          }
         }
       }
       if (b < w1) {  // more to come: room in every count
@@ -278,14 +386,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
 
   uint32_t key = top, place = 0;
   if (top < kEnd && temperature != 0.f) {
-    // ---- this thread's keys: low ... low + kPer - 1 ---------------------------------
-    const uint32_t block = tid / kGroup * kCtas + rank;
-    const uint32_t low = block * kBlockKeys + tid % kGroup * kPer;
-    const uint32_t order = low / kPer;
     const double most = key_value(top);
-    // Counts of eight keys, over the cluster.
-    auto counts = [&](int g, uint32_t (&c)[8]) {
-      const uint32_t k0 = low + 8 * g;
+    // this thread's group of a round, in descending order of keys
+    auto group_of = [&](int r) -> uint32_t {
+      return kCtas == 1 ? r * kThreads + tid : (tid / 8 * kCtas + rank) * 8 + tid % 8;
+    };
+    // Counts of a group's keys, over the cluster.
+    auto counts = [&](uint32_t k0, uint32_t (&c)[8]) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) c[e] = 0;
       if (k0 < top / 8 * 8 || k0 >= kEnd) return;
@@ -310,66 +417,88 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
           }
         }
     };
-    // Runs f(key, count, weight) over this thread's candidates in order; `at`
-    // is the count of candidates before them, of which top_k stay.
-    auto walk = [&](uint32_t at, auto f) {
-#pragma unroll 1
-      for (int g = 0; g < kPer / 8; ++g) {
-        uint32_t c[8], any = 0;
-        counts(g, c);
-        if (top_k) {
+    // top_k: of key `cutoff` the first `leaves` candidates stay, of later ones none.
+    uint32_t cutoff = 0xFFFFFFFFu, leaves = 0;
+    if (top_k) {
+      uint32_t own[kR], before[kR];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t n = c[e];
-            c[e] = at >= top_k ? 0u : min(n, top_k - at);
-            at += n;
-          }
+      for (int r = 0; r < kR; ++r) {
+        uint32_t c[8];
+        counts(group_of(r) * 8, c);
+        own[r] = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) own[r] += c[e];
+      }
+      row_exclusive<kCtas, uint32_t>(sh, rank, own, before);
+      int round = -1;
+      uint32_t at = 0;
+#pragma unroll
+      for (int r = kR - 1; r >= 0; --r)
+        if (own[r] && before[r] + own[r] >= top_k) {
+          round = r;
+          at = before[r];
         }
+      uint32_t k = 0, n = 0;
+      if (row_first<kCtas>(sh, rank, round >= 0, round >= 0 ? group_of(round) : 0, sh.cutoff,
+                           [&](uint32_t (&out)[2]) {
+                             uint32_t c[8];
+                             counts(group_of(round) * 8, c);
+                             bool done = false;
 #pragma unroll
-        for (int e = 7; e >= 0; --e)
-          if (c[e]) any = e + 1;
-        if (!any) continue;
-        const uint32_t k0 = low + 8 * g, k1 = k0 + any - 1;  // the first that has a count
-        double w = exp((key_value(k1) - most) * inverse);
-        const double step = sh.step[key_bits(k0) >> 10];
+                             for (int e = 0; e < 8; ++e) {
+                               if (!done && at + c[e] >= top_k) {
+                                 out[0] = group_of(round) * 8 + e;
+                                 out[1] = top_k - at;
+                                 done = true;
+                               }
+                               at += c[e];
+                             }
+                           },
+                           k, n)) {
+        cutoff = k;
+        leaves = n;
+      }
+    }
+    // Runs f(key, count, weight) over the candidates of a round's group.
+    auto walk = [&](int r, auto f) {
+      const uint32_t k0 = group_of(r) * 8;
+      uint32_t c[8], any = 0;
+      counts(k0, c);
+      if (k0 + 7 >= cutoff) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (c[e]) f(k0 + e, c[e], w);
-          if (k0 + e >= k1) w *= step;
-        }
+        for (int e = 0; e < 8; ++e)
+          c[e] = k0 + e < cutoff ? c[e] : k0 + e == cutoff ? leaves : 0u;
+      }
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if (c[e]) any = e + 1;
+      if (!any) return;
+      const uint32_t k1 = k0 + any - 1;  // the first that has a count
+      double w = exp((key_value(k1) - most) * inverse);
+      const double step = sh.step[key_bits(k0) >> 10];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (c[e]) f(k0 + e, c[e], w);
+        if (k0 + e >= k1) w *= step;
       }
     };
-    uint32_t at_count = 0;
-    if (top_k) {
-      uint32_t own = 0, all;
 #pragma unroll 1
-      for (int g = 0; g < kPer / 8; ++g) {
-        uint32_t c[8];
-        counts(g, c);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) own += c[e];
-      }
-      at_count = row_exclusive<kCtas, kGroup>(rank, own, sh.count, (uint32_t*)sh.before,
-                                              sh.warp_count, all);
-      __syncthreads();  // `before` is used again
+    for (int r = 0; r < kR; ++r) {
+      double own = 0.0;
+      walk(r, [&](uint32_t, uint32_t n, double w) { own += n * w; });
+      sh.mass[r][tid] = own;
     }
-    double own = 0.0, lightest = INFINITY, total;
-    walk(at_count, [&](uint32_t, uint32_t n, double w) {
-      own += n * w;
-      lightest = w;
-    });
-    const double at =
-        row_exclusive<kCtas, kGroup>(rank, own, sh.mass, sh.before, sh.warp_mass, total);
+    double own[kR], before[kR];
+#pragma unroll
+    for (int r = 0; r < kR; ++r) own[r] = sh.mass[r][tid];
+    const double total = row_exclusive<kCtas, double>(sh, rank, own, before);
     // What top_p and min_p keep is a prefix again: the kept sum is the sum at
-    // the end of the last kept candidate. Only the threads around a border
-    // look at their candidates one by one.
-    const bool cut = top_p < 1.f || min_p > 0.f;
+    // the end of the last kept candidate. Only the groups around a border
+    // are looked at one candidate at a time.
     const double limit = top_p >= 1.f ? INFINITY : (double)top_p * total;
-    const bool mine_top = top - low < (uint32_t)kPer;
     // f(key, kept count, weight, sum before it)
-    auto walk_kept = [&](auto f) {
-      double sum = at;
-      walk(at_count, [&](uint32_t k, uint32_t c, double w) {
+    auto walk_kept = [&](int r, double sum, auto f) {
+      walk(r, [&](uint32_t k, uint32_t c, double w) {
         uint32_t n = w >= (double)min_p ? c : 0u;
         if (n && !(sum + (n - 1) * w < limit)) {
           // places j with sum + j w < limit
@@ -387,28 +516,49 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
         sum += c * w;
       });
     };
-    double end = at + own;  // where this thread's kept candidates end
-    bool has = own > 0.0;
-    if (cut && has && !(end < limit && lightest >= (double)min_p)) {
-      has = false;
-      if (at < limit || mine_top)
-        walk_kept([&](uint32_t, uint32_t n, double w, double sum) {
-          has = true;
-          end = sum + n * w;
-        });
-    }
+    uint32_t final = 0xFFFFFFFFu;  // order + 1 of the last kept group
     double sum_kept = total;
-    if (cut) {
-      const uint32_t mine = has ? order + 1 : 0u;
+    if (top_p < 1.f || min_p > 0.f) {
+      // weights of a group are at least min_p where its exponents are above
+      // log(min_p), none is where they are below; the margin is far above the
+      // errors of both and leaves the groups between to be looked at
+      const double least_x = log((double)min_p), margin = 1e-6;
+      uint32_t mine = 0, border = 0;
+      double mine_end = 0.0;
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        const uint32_t k0 = group_of(r) * 8;
+        if (!(own[r] > 0.0)) continue;
+        const double end = before[r] + own[r];
+        const double high_x = (key_value(k0) - most) * inverse;
+        const double low_x = (key_value(k0 + 7) - most) * inverse;
+        if (end < limit && low_x > least_x + margin) {
+          mine = group_of(r) + 1;
+          mine_end = end;
+        } else if (top / 8 == k0 / 8 || (before[r] < limit && high_x > least_x - margin)) {
+          border |= 1u << r;
+        }
+      }
+      for (; border; border &= border - 1) {
+        const int r = __ffs(border) - 1;
+        double at = 0.0, end = -1.0;
+#pragma unroll
+        for (int q = 0; q < kR; ++q) at = q == r ? before[q] : at;
+        walk_kept(r, at, [&](uint32_t, uint32_t n, double w, double sum) { end = sum + n * w; });
+        if (end >= 0.0 && group_of(r) + 1 > mine) {
+          mine = group_of(r) + 1;
+          mine_end = end;
+        }
+      }
       const uint32_t warp_last = __reduce_max_sync(0xffffffffu, mine);
       if (lane == 0 && warp_last) atomicMax(&sh.last, warp_last);
       __syncthreads();
       if (mine && sh.last == mine) {
-        sh.kept = end;
+        sh.kept = mine_end;
         sh.kept_order = mine;
       }
       row_sync<kCtas>();
-      uint32_t final = 0;
+      final = 0;
 #pragma unroll
       for (int r = 0; r < kCtas; ++r) {
         const uint32_t q = *of_rank<kCtas>(&sh.kept_order, r);
@@ -419,49 +569,38 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
         }
       }
     }
-    // The first thread whose sum exceeds the target: there is one, as uniform
-    // is at most 1 - 2^-24 and sums agree to about 1e-15. Threads' sums meet
-    // within rounding only, so the first of all is taken, not the one around it.
+    // The first group whose kept sum exceeds the target: there is one, as
+    // uniform is at most 1 - 2^-24 and sums agree to about 1e-15. Groups' sums
+    // meet within rounding only, so the first of all is taken, not the one
+    // around it.
     const double target = (double)uniform * sum_kept;
-    const uint32_t hit = has && end > target ? ~order : 0u;
-    const uint32_t warp_first = __reduce_max_sync(0xffffffffu, hit);
-    if (lane == 0 && warp_first) atomicMax(&sh.first, warp_first);
-    __syncthreads();
-    const uint32_t found = sh.first;
-    if (hit ? found == hit : found == 0 && tid == 0) {
-      uint32_t token = 0, where = 0;
-      if (hit) {
-        bool crossed = false;
-        walk_kept([&](uint32_t k, uint32_t n, double w, double sum) {
-          if (crossed) return;
-          // its first place whose sum exceeds the target; the last candidate
-          // of the thread where rounding leaves none
-          const double j = floor((target - sum) / w);
-          uint32_t m = j <= 0.0 ? 0u : j >= (double)n ? n - 1 : (uint32_t)j;
-          if (sum + (m + 1) * w <= target && m + 1 < n) ++m;
-          else if (m && sum + m * w > target) --m;
-          crossed = sum + (m + 1) * w > target;
-          token = k;
-          where = m;
-        });
-      }
+    int round = -1;
+    double at = 0.0;
 #pragma unroll
-      for (int r = 0; r < kCtas; ++r) {
-        uint32_t* out = of_rank<kCtas>(&sh.crossing[rank][0], r);
-        out[0] = hit;
-        out[1] = token;
-        out[2] = where;
+    for (int r = kR - 1; r >= 0; --r) {
+      const uint32_t o = group_of(r) + 1;
+      if (own[r] > 0.0 && o <= final && (o == final ? sum_kept : before[r] + own[r]) > target) {
+        round = r;
+        at = before[r];
       }
     }
-    row_sync<kCtas>();
-    uint32_t best = 0;
-#pragma unroll
-    for (int r = 0; r < kCtas; ++r)
-      if (sh.crossing[r][0] > best) {
-        best = sh.crossing[r][0];
-        key = sh.crossing[r][1];
-        place = sh.crossing[r][2];
-      }
+    row_first<kCtas>(sh, rank, round >= 0, round >= 0 ? group_of(round) : 0, sh.crossing,
+                     [&](uint32_t (&out)[2]) {
+                       bool crossed = false;
+                       walk_kept(round, at, [&](uint32_t k, uint32_t n, double w, double sum) {
+                         if (crossed) return;
+                         // its first place whose sum exceeds the target; the last
+                         // candidate of the group where rounding leaves none
+                         const double j = floor((target - sum) / w);
+                         uint32_t m = j <= 0.0 ? 0u : j >= (double)n ? n - 1 : (uint32_t)j;
+                         if (sum + (m + 1) * w <= target && m + 1 < n) ++m;
+                         else if (m && sum + m * w > target) --m;
+                         crossed = sum + (m + 1) * w > target;
+                         out[0] = k;
+                         out[1] = m;
+                       });
+                     },
+                     key, place);
   }
 
   // ---- key and place to an index -----------------------------------------------------
@@ -473,9 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
     const uint32_t bits = key_bits(key) * 0x10001u;
     const int run = (w1 - w0 + kWarps - 1) / kWarps;
     const int a = min(w1, w0 + warp * run), b = min(w1, a + run);
-    auto equal = [&](int i) {  // a bit for each of the word's equals
-      if (i >= b) return 0u;
-      const uint4 v = x.word(i);
+    auto equal = [&](const uint4& v) {  // a bit for each of the word's equals
       const uint32_t u[4] = {v.x ^ bits, v.y ^ bits, v.z ^ bits, v.w ^ bits};
       uint32_t mask = 0;
 #pragma unroll
@@ -485,8 +622,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
       return mask;
     };
     uint32_t equals = 0;
-#pragma unroll 4
-    for (int i = a + lane; i < b; i += 32) equals += __popc(equal(i));
+    for (int i = a + lane; i < b; i += 4 * 32) {
+      uint4 v[4];
+      x.load(v, i, 32, b);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) equals += __popc(equal(v[k]));
+    }
     equals = __reduce_add_sync(0xffffffffu, equals);
     if (lane == 0) sh.equals[warp] = equals;
     __syncthreads();
@@ -502,7 +643,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
     for (int q = 0; q < warp; ++q) rest -= (int)sh.equals[q];
     if (rest >= 0 && rest < (int)equals) {
       for (int i = a; i < b; i += 32) {
-        uint32_t mask = equal(i + lane);
+        uint4 v[1];
+        x.load(v, i + lane, 32, b);
+        uint32_t mask = equal(v[0]);
         int n = __popc(mask), upto = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -529,11 +672,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
 template <int kCtas>
 void launch_sample(const Launch& l, const SampleBatch& p) {
   auto kernel = sample_batch_kernel<kCtas>;
-  allow_dynamic_smem(kernel, sizeof(Shared));
+  allow_dynamic_smem(kernel, sizeof(Shared<kCtas>));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.rows * kCtas);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.dynamicSmemBytes = sizeof(Shared<kCtas>);
   cfg.stream = l.stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
