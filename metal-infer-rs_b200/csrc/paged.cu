@@ -19,14 +19,17 @@ namespace {
 // ---- append -------------------------------------------------------------------
 // y = half(rot(x * rsqrt(mean(x^2) + eps) * w)) for Q and K heads (the norm is
 // left out without weights), V as it is; each head row is read and written
-// once by HD / 8 lanes (16 bytes a lane). The arithmetic is that of
-// qk_norm_rope_cache and rope (numerics.cuh), so a paged cache holds the same
-// bits as a contiguous one.
+// once. The arithmetic is that of qk_norm_rope_cache and rope (numerics.cuh),
+// so a paged cache holds the same bits as a contiguous one.
 //
-// A block takes kTok tokens at a time and first fills a table of their
-// cosines and sines: the angles need double precision (numerics.cuh), which a
-// thread per (token, pair) pays once for all heads, and the frequency's pow
-// once for all of a block's tokens.
+// HBM-bound for prompts. A row has HD / 16 lanes, each with a chunk of eight
+// values and the chunk that it rotates with: the first step of the canonical
+// sum of squares and the whole rotation stay inside a lane (with a chunk to a
+// lane and the partner fetched by shuffles, 5.7 K tokens of 32/8 heads took 55
+// us, XXX so). A block takes kTok tokens at a time and first fills a table of
+// their cosines and sines: the angles need double precision (numerics.cuh),
+// which a thread per (token, pair) pays once for all heads, and the
+// frequency's pow once for all of a block's tokens.
 constexpr int kAppendThreads = 256;
 
 struct AppendArgs {
@@ -37,11 +40,29 @@ struct AppendArgs {
   int tokens, sequences, qh, kvh, table_width, page;
   uint32_t pages;
   float theta, eps;
+  float inverse_heads;  // 1 / (qh + 2 kvh), rows to a token
 };
+
+__device__ __forceinline__ void widen8(const uint4& raw, float (&x)[8]) {
+  const __half2* h = reinterpret_cast<const __half2*>(&raw);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = __half22float2(h[e]);
+    x[2 * e] = f.x;
+    x[2 * e + 1] = f.y;
+  }
+}
+__device__ __forceinline__ uint4 narrow8(const float (&x)[8]) {
+  uint4 packed;
+  __half2* h = reinterpret_cast<__half2*>(&packed);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+  return packed;
+}
 
 template <int HD, int kTok>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendArgs a) {
-  constexpr int kLanes = HD / 8;           // lanes of a head row
+  constexpr int kLanes = HD / 16;          // lanes of a head row
   constexpr int kRows = kAppendThreads / kLanes;
   constexpr int kPairs = HD / 2;
   __shared__ float2 cs[kTok][kPairs];
@@ -104,8 +125,43 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
       slot[tid] = row;
     }
     __syncthreads();
-    for (int i = tid; i < kTok * kPairs; i += kAppendThreads) {
-      const int t = i / kPairs;
+    const int heads = a.qh + 2 * a.kvh;
+    const int rows = min(kTok, a.tokens - t0) * heads;
+    // the chunks of row r of the block's tokens, and where they go
+    auto source = [&](int r, const __half*& src, __half*& dst, int& i, int& h) {
+      i = kTok == 1 ? 0 : (int)(((float)r + 0.5f) * a.inverse_heads);
+      h = r - i * heads;
+      const size_t t = t0 + i;
+      const uint32_t row = slot[i];
+      src = nullptr;
+      dst = nullptr;
+      if (row == 0xFFFFFFFFu) return;
+      if (h < a.qh) {
+        src = a.q + (t * a.qh + h) * HD;
+        dst = a.q_out + (t * a.qh + h) * HD;
+      } else {
+        const bool is_v = h >= a.qh + a.kvh;
+        const int kv = h - a.qh - (is_v ? a.kvh : 0);
+        src = (is_v ? a.v : a.k) + (t * a.kvh + kv) * HD;
+        dst = (is_v ? a.vc : a.kc) + ((size_t)row * a.kvh + kv) * HD;
+      }
+    };
+    // the first row's loads are in flight while the angles are computed
+    const __half* src = nullptr;
+    __half* dst = nullptr;
+    int i = 0, h = 0;
+    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+    int r = tid / kLanes;
+    auto fetch = [&] {
+      if (r < rows) source(r, src, dst, i, h);
+      if (r < rows && src) {
+        lo = reinterpret_cast<const uint4*>(src)[li];
+        hi = reinterpret_cast<const uint4*>(src)[li + kLanes];
+      }
+    };
+    fetch();
+    for (int j = tid; j < kTok * kPairs; j += kAppendThreads) {
+      const int t = j / kPairs;
       if (slot[t] != 0xFFFFFFFFu) {
         double s, c;
         sincos((double)__fmul_rn((float)position[t], frequency), &s, &c);
@@ -113,63 +169,48 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
       }
     }
     __syncthreads();
-    const int heads = a.qh + 2 * a.kvh;
-    for (int r = tid / kLanes; r < kTok * heads; r += kRows) {
-      const int i = r / heads, h = r - i * heads;
-      const uint32_t row = slot[i];
-      if (row == 0xFFFFFFFFu) continue;
-      const size_t t = t0 + i;
-      if (h >= a.qh + a.kvh) {
-        const int kv = h - a.qh - a.kvh;
-        reinterpret_cast<uint4*>(a.vc + ((size_t)row * a.kvh + kv) * HD)[li] =
-            reinterpret_cast<const uint4*>(a.v + (t * a.kvh + kv) * HD)[li];
+    for (; r - (tid & 31) / kLanes < rows; r += kRows, fetch()) {  // whole warps
+      const bool rotates = h < a.qh + a.kvh;
+      const __half* w = h < a.qh ? a.qw : a.kw;
+      if (!__any_sync(0xffffffffu, r < rows && src && rotates)) {  // values
+        if (r < rows && src) {
+          reinterpret_cast<uint4*>(dst)[li] = lo;
+          reinterpret_cast<uint4*>(dst)[li + kLanes] = hi;
+        }
         continue;
       }
-      // the lanes of a head row stay together, two or four rows to a warp
-      const unsigned group = (kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1))
-                             << ((tid & 31) / kLanes * kLanes);
-      const bool is_q = h < a.qh;
-      if (is_q && !a.q) continue;
-      const __half* src = is_q ? a.q + (t * a.qh + h) * HD : a.k + (t * a.kvh + h - a.qh) * HD;
-      __half* dst = is_q ? a.q_out + (t * a.qh + h) * HD
-                         : a.kc + ((size_t)row * a.kvh + h - a.qh) * HD;
-      const uint4 raw = reinterpret_cast<const uint4*>(src)[li];
-      const __half* w = is_q ? a.qw : a.kw;
-      const __half2* hr = reinterpret_cast<const __half2*>(&raw);
-      float x[8];
+      float x[8], y[8];
+      widen8(lo, x);
+      widen8(hi, y);
+      if (a.kw) {  // all of the call's rows have weights, or none
+        float total = __fadd_rn(chunk_sq(lo, 0.f), chunk_sq(hi, 0.f));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = __half22float2(hr[e]);
-        x[2 * e] = f.x;
-        x[2 * e + 1] = f.y;
+        for (int o = kLanes / 2; o >= 1; o >>= 1)
+          total = __fadd_rn(total, __shfl_xor_sync(0xffffffffu, total, o));
+        const float scale = rms_scale(total, HD, a.eps);
+        float g[8];
+        widen8(reinterpret_cast<const uint4*>(w)[li], g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = norm_mul(x[e], scale, g[e]);
+        widen8(reinterpret_cast<const uint4*>(w)[li + kLanes], g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = norm_mul(y[e], scale, g[e]);
       }
-      if (w) {
-        const float scale =
-            rms_scale(canon_butterfly_mask(chunk_sq(raw, 0.f), kLanes, group), HD, a.eps);
-        const uint4 wr = reinterpret_cast<const uint4*>(w)[li];
-        const __half2* hw = reinterpret_cast<const __half2*>(&wr);
+      if (r < rows && src) {
+        if (rotates) {
+          float u[8], v[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 g = __half22float2(hw[e]);
-          x[2 * e] = norm_mul(x[2 * e], scale, g.x);
-          x[2 * e + 1] = norm_mul(x[2 * e + 1], scale, g.y);
+          for (int e = 0; e < 8; ++e) {
+            const float2 t = cs[i][8 * li + e];
+            u[e] = __fsub_rn(__fmul_rn(x[e], t.x), __fmul_rn(y[e], t.y));
+            v[e] = __fadd_rn(__fmul_rn(x[e], t.y), __fmul_rn(y[e], t.x));
+          }
+          lo = narrow8(u);
+          hi = narrow8(v);
         }
+        reinterpret_cast<uint4*>(dst)[li] = lo;
+        reinterpret_cast<uint4*>(dst)[li + kLanes] = hi;
       }
-      const bool first = li < kLanes / 2;
-      uint4 packed;
-      __half2* hp = reinterpret_cast<__half2*>(&packed);
-      float y[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float other = __shfl_xor_sync(group, x[e], kLanes / 2);
-        const float2 t2 = cs[i][8 * (first ? li : li - kLanes / 2) + e];
-        y[e] = first ? __fsub_rn(__fmul_rn(x[e], t2.x), __fmul_rn(other, t2.y))
-                     : __fadd_rn(__fmul_rn(other, t2.y), __fmul_rn(x[e], t2.x));
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        hp[e] = __halves2half2(__float2half_rn(y[2 * e]), __float2half_rn(y[2 * e + 1]));
-      reinterpret_cast<uint4*>(dst)[li] = packed;
     }
     __syncthreads();
   }
@@ -740,7 +781,7 @@ void paged_append(const Launch& l, const PagedAppend& p) {
   if (p.tokens == 0 || p.sequences == 0) return;
   AppendArgs a{p.q, p.k, p.v, p.qw, p.kw, p.q_out, p.key_cache, p.value_cache, p.starts,
                p.lengths, p.table, p.fault, p.tokens, p.sequences, p.qh, p.kvh, p.table_width,
-               p.page, p.pages, p.theta, p.eps};
+               p.page, p.pages, p.theta, p.eps, 1.f / (float)(p.qh + 2 * p.kvh)};
   if (p.hd == 128)
     launch_append<128>(l, a);
   else
