@@ -26,7 +26,7 @@ namespace {
 // values and the chunk that it rotates with: the first step of the canonical
 // sum of squares and the whole rotation stay inside a lane (with a chunk to a
 // lane and the partner fetched by shuffles, 5.7 K tokens of 32/8 heads took 55
-// us, XXX so). A block takes kTok tokens at a time and first fills a table of
+// us, 33 so). A block takes kTok tokens at a time and first fills a table of
 // their cosines and sines: the angles need double precision (numerics.cuh),
 // which a thread per (token, pair) pays once for all heads, and the
 // frequency's pow once for all of a block's tokens.
@@ -43,20 +43,39 @@ struct AppendArgs {
   float inverse_heads;  // 1 / (qh + 2 kvh), rows to a token
 };
 
-__device__ __forceinline__ void widen8(const uint4& raw, float (&x)[8]) {
+// Two FP32 values in one instruction, each rounded as by itself.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void widen8(const uint4& raw, uint64_t (&x)[4]) {
   const __half2* h = reinterpret_cast<const __half2*>(&raw);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float2 f = __half22float2(h[e]);
-    x[2 * e] = f.x;
-    x[2 * e + 1] = f.y;
+    x[e] = pair_of(f.x, f.y);
   }
 }
-__device__ __forceinline__ uint4 narrow8(const float (&x)[8]) {
+__device__ __forceinline__ uint4 narrow8(const uint64_t (&x)[4]) {
   uint4 packed;
   __half2* h = reinterpret_cast<__half2*>(&packed);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+  for (int e = 0; e < 4; ++e) {
+    float lo, hi;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x[e]));
+    h[e] = __floats2half2_rn(lo, hi);
+  }
   return packed;
 }
 
@@ -65,7 +84,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
   constexpr int kLanes = HD / 16;          // lanes of a head row
   constexpr int kRows = kAppendThreads / kLanes;
   constexpr int kPairs = HD / 2;
-  __shared__ float2 cs[kTok][kPairs];
+  __shared__ __align__(16) float cosines[kTok][kPairs], sines[kTok][kPairs];
   __shared__ uint32_t position[kTok];
   __shared__ uint32_t slot[kTok];          // cache row of the token
   const int tid = threadIdx.x;
@@ -165,51 +184,68 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
       if (slot[t] != 0xFFFFFFFFu) {
         double s, c;
         sincos((double)__fmul_rn((float)position[t], frequency), &s, &c);
-        cs[t][pair0] = make_float2((float)c, (float)s);
+        cosines[t][pair0] = (float)c;
+        sines[t][pair0] = (float)s;
       }
     }
     __syncthreads();
-    for (; r - (tid & 31) / kLanes < rows; r += kRows, fetch()) {  // whole warps
+    while (r - (tid & 31) / kLanes < rows) {  // whole warps
+      // this row's, while the next one's are on their way
+      const bool ok = r < rows && src;
       const bool rotates = h < a.qh + a.kvh;
       const __half* w = h < a.qh ? a.qw : a.kw;
-      if (!__any_sync(0xffffffffu, r < rows && src && rotates)) {  // values
-        if (r < rows && src) {
-          reinterpret_cast<uint4*>(dst)[li] = lo;
-          reinterpret_cast<uint4*>(dst)[li + kLanes] = hi;
+      __half* const to = dst;
+      const int token = i;
+      uint4 first = lo, second = hi;
+      r += kRows;
+      fetch();
+      if (!__any_sync(0xffffffffu, ok && rotates)) {  // values
+        if (ok) {
+          reinterpret_cast<uint4*>(to)[li] = first;
+          reinterpret_cast<uint4*>(to)[li + kLanes] = second;
         }
         continue;
       }
-      float x[8], y[8];
-      widen8(lo, x);
-      widen8(hi, y);
+      uint64_t x[4], y[4];
+      widen8(first, x);
+      widen8(second, y);
       if (a.kw) {  // all of the call's rows have weights, or none
-        float total = __fadd_rn(chunk_sq(lo, 0.f), chunk_sq(hi, 0.f));
+        float total = __fadd_rn(chunk_sq(first, 0.f), chunk_sq(second, 0.f));
 #pragma unroll
         for (int o = kLanes / 2; o >= 1; o >>= 1)
           total = __fadd_rn(total, __shfl_xor_sync(0xffffffffu, total, o));
-        const float scale = rms_scale(total, HD, a.eps);
-        float g[8];
+        const float one = rms_scale(total, HD, a.eps);
+        const uint64_t scale = pair_of(one, one);
+        uint64_t g[4];
         widen8(reinterpret_cast<const uint4*>(w)[li], g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = norm_mul(x[e], scale, g[e]);
+        for (int e = 0; e < 4; ++e) x[e] = mul2(mul2(x[e], scale), g[e]);
         widen8(reinterpret_cast<const uint4*>(w)[li + kLanes], g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = norm_mul(y[e], scale, g[e]);
+        for (int e = 0; e < 4; ++e) y[e] = mul2(mul2(y[e], scale), g[e]);
       }
-      if (r < rows && src) {
+      if (ok) {
         if (rotates) {
-          float u[8], v[8];
+          uint64_t u[4], v[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float2 t = cs[i][8 * li + e];
-            u[e] = __fsub_rn(__fmul_rn(x[e], t.x), __fmul_rn(y[e], t.y));
-            v[e] = __fadd_rn(__fmul_rn(x[e], t.y), __fmul_rn(y[e], t.x));
+          for (int q = 0; q < 2; ++q) {
+            const float4 c = *reinterpret_cast<const float4*>(&cosines[token][8 * li + 4 * q]);
+            const float4 s = *reinterpret_cast<const float4*>(&sines[token][8 * li + 4 * q]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint64_t ce = e ? pair_of(c.z, c.w) : pair_of(c.x, c.y);
+              const uint64_t se = e ? pair_of(s.z, s.w) : pair_of(s.x, s.y);
+              const uint64_t minus = e ? pair_of(-s.z, -s.w) : pair_of(-s.x, -s.y);
+              const int k = 2 * q + e;
+              u[k] = add2(mul2(x[k], ce), mul2(y[k], minus));
+              v[k] = add2(mul2(x[k], se), mul2(y[k], ce));
+            }
           }
-          lo = narrow8(u);
-          hi = narrow8(v);
+          first = narrow8(u);
+          second = narrow8(v);
         }
-        reinterpret_cast<uint4*>(dst)[li] = lo;
-        reinterpret_cast<uint4*>(dst)[li + kLanes] = hi;
+        reinterpret_cast<uint4*>(to)[li] = first;
+        reinterpret_cast<uint4*>(to)[li + kLanes] = second;
       }
     }
     __syncthreads();
@@ -218,8 +254,9 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 
 template <int HD>
 void launch_append(const Launch& l, const AppendArgs& a) {
-  // Four tokens to a block amortise the table's barriers; few tokens take a
-  // block each, since latency is then all there is.
+  // Four tokens to a block share its barriers (one 42 us, two 33.9, four 32.7
+  // for 5.7 K tokens); few tokens take a block each, since latency is then all
+  // there is.
   if (a.tokens <= 2 * l.sm_count) {
     launch_kernel(l, dim3(a.tokens), dim3(kAppendThreads), 0, paged_append_kernel<HD, 1>, a);
   } else {
