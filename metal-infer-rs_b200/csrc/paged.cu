@@ -54,10 +54,8 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
+__device__ __forceinline__ void split(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
 }
 __device__ __forceinline__ void widen8(const uint4& raw, uint64_t (&x)[4]) {
   const __half2* h = reinterpret_cast<const __half2*>(&raw);
@@ -73,7 +71,7 @@ __device__ __forceinline__ uint4 narrow8(const uint64_t (&x)[4]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     float lo, hi;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x[e]));
+    split(x[e], lo, hi);
     h[e] = __floats2half2_rn(lo, hi);
   }
   return packed;
@@ -233,12 +231,18 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
             const float4 s = *reinterpret_cast<const float4*>(&sines[token][8 * li + 4 * q]);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+              // The sums are scalar: a paired addition behind a paired product
+              // is fused with it, and the product's rounding is lost.
               const uint64_t ce = e ? pair_of(c.z, c.w) : pair_of(c.x, c.y);
               const uint64_t se = e ? pair_of(s.z, s.w) : pair_of(s.x, s.y);
-              const uint64_t minus = e ? pair_of(-s.z, -s.w) : pair_of(-s.x, -s.y);
               const int k = 2 * q + e;
-              u[k] = add2(mul2(x[k], ce), mul2(y[k], minus));
-              v[k] = add2(mul2(x[k], se), mul2(y[k], ce));
+              float xc[2], xs[2], yc[2], ys[2];
+              split(mul2(x[k], ce), xc[0], xc[1]);
+              split(mul2(x[k], se), xs[0], xs[1]);
+              split(mul2(y[k], ce), yc[0], yc[1]);
+              split(mul2(y[k], se), ys[0], ys[1]);
+              u[k] = pair_of(__fsub_rn(xc[0], ys[0]), __fsub_rn(xc[1], ys[1]));
+              v[k] = pair_of(__fadd_rn(xs[0], yc[0]), __fadd_rn(xs[1], yc[1]));
             }
           }
           first = narrow8(u);
