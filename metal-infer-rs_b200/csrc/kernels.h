@@ -271,7 +271,10 @@ struct PackedAttention {
   uint32_t* fault = nullptr;
   int tokens = 0, keys = 0, sequences = 0, qh = 1, kvh = 1, hd = 128, causal = 1;
 };
-void packed_attention(const Launch& l, const PackedAttention& p);
+// Bytes of device scratch of a packed_attention launch (may be 0; nothing is
+// kept in it from one launch to the next).
+size_t packed_attention_workspace(const PackedAttention& p, int sm_count);
+void packed_attention(const Launch& l, const PackedAttention& p, void* workspace);
 // One token per row of logits [rows, n] under that row's options.
 struct SampleBatch {
   const __half* logits = nullptr;

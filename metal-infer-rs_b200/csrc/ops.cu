@@ -967,8 +967,11 @@ mi_status mi_batch_packed_attention(mi_batch* b, const mi_tensor* query, const m
     p.key_starts = key_starts->u32();
     p.fault = ctx->fault;
     p.causal = causal != 0;
+    Out ws;
+    if (const size_t bytes = k::packed_attention_workspace(p, ctx->sm_count))
+      ws.t = new_tensor(ctx, {(bytes + 3) / 4}, MI_F32);
     ProfileScope ps(ctx, "packed_attention");
-    k::packed_attention(launch_of(ctx), p);
+    k::packed_attention(launch_of(ctx), p, ws.t ? ws.t->base() : nullptr);
   });
 }
 

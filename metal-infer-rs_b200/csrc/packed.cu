@@ -63,6 +63,7 @@ struct PackedArgs {
   int head_tiles;   // row tiles to cover the group
   int span;         // tokens of a row tile
   float scale_log2; // log2(e) / sqrt(HD)
+  const struct Plan* plan;
 };
 
 template <int HD>
@@ -295,15 +296,121 @@ __device__ __forceinline__ void exp2_poly2(uint64_t x, float& lo, float& hi) {
   hi = __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23));
 }
 
-// What a CTA works on.
-struct Work {
+// What a CTA works on: two row tiles.
+struct alignas(16) Work {
   int q0, q1;      // the sequence's query rows
   int k0, keys;    // its first key row, its keys
-  int token;       // first token (of the sequence) of row tile 0
+  int token;       // first token (of the sequence) of row tile 0, -1: nothing
   int blocks[2];   // key tiles that row tile 0 / 1 sees
+  int pad;
 };
+static_assert(sizeof(Work) == 32, "two 16-byte words");
 
-template <int HD>
+// The row tiles from token t on of sequence s.
+__device__ __forceinline__ Work work_of(const PackedArgs& a, int key_tile, int s, long long t) {
+  Work w{0, 0, 0, 0, -1, {0, 0}, 0};
+  w.q0 = (int)a.query_starts[s];
+  w.q1 = (int)a.query_starts[s + 1];
+  w.k0 = (int)a.key_starts[s];
+  w.keys = (int)a.key_starts[s + 1] - w.k0;
+  const int n = w.q1 - w.q0;
+  w.token = t < n ? (int)t : -1;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int last = min((long long)n, t + (i + 1) * a.span) - 1;  // last token of the row tile
+    if (w.token < 0 || last < t + i * a.span) continue;
+    const long long seen = a.causal ? (long long)w.keys - (n - 1 - last) : w.keys;
+    w.blocks[i] = seen > 0 ? (int)((seen + key_tile - 1) / key_tile) : 0;
+  }
+  return w;
+}
+// Sequence s owns the places floor(start_s / (2 span)) + s and on, which leaves
+// it room for its tiles whatever the lengths are.
+__device__ __forceinline__ long long first_place(const PackedArgs& a, int s) {
+  return (long long)(a.query_starts[s] / (uint32_t)(2 * a.span)) + s;
+}
+__device__ __forceinline__ bool bad_starts(const PackedArgs& a, int s) {
+  const uint32_t qb = a.query_starts[s], qe = a.query_starts[s + 1];
+  const uint32_t kb = a.key_starts[s], ke = a.key_starts[s + 1];
+  return qb > qe || qe > (uint32_t)a.tokens || kb > ke || ke > (uint32_t)a.keys;
+}
+
+// ---- the order of the work ------------------------------------------------------
+// All sequences' row tiles, the ones that see most keys first (a counting sort
+// by key tiles): the CTAs that start last are then the shortest. Without it the
+// longest prompt's tiles may come last: 10 prompts of 20 to 2500 tokens took
+// 100 us, XXX so. The order among equals depends on timing, the results do not.
+struct Plan {
+  uint32_t count;
+  uint32_t pad[7];
+  Work work[1];
+};
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanBins = 2048;  // longer ones share the last
+
+__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedArgs a, Plan* plan,
+                                                                   int places, int key_tile) {
+  __shared__ uint32_t bins[kPlanBins];
+  __shared__ uint32_t sums[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < kPlanBins; i += kPlanThreads) bins[i] = 0;
+  pdl_wait();
+  pdl_trigger();
+  bool bad = false;
+  for (int s = tid; s < a.sequences; s += kPlanThreads) bad |= bad_starts(a, s);
+  if (__syncthreads_or(bad)) {
+    if (tid == 0) {
+      report_fault(a.fault, kFaultStarts);
+      plan->count = 0;
+    }
+    return;
+  }
+  auto work_at = [&](int place) {
+    int lo = 0, hi = a.sequences;  // the last sequence that begins at or before it
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (first_place(a, mid) <= place) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo == 0) return Work{0, 0, 0, 0, -1, {0, 0}, 0};
+    return work_of(a, key_tile, lo - 1, (place - first_place(a, lo - 1)) * 2 * a.span);
+  };
+  auto bin_of = [&](const Work& w) {  // longest first
+    return kPlanBins - 1 - min(kPlanBins - 1, max(w.blocks[0], w.blocks[1]));
+  };
+  for (int i = tid; i < places; i += kPlanThreads) {
+    const Work w = work_at(i);
+    if (w.token >= 0) atomicAdd(&bins[bin_of(w)], 1u);
+  }
+  __syncthreads();
+  // sums before each bin, two bins to a thread
+  const uint32_t b0 = bins[2 * tid], b1 = bins[2 * tid + 1];
+  uint32_t x = b0 + b1;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) sums[warp] = x;
+  __syncthreads();
+  uint32_t base = 0, all = 0;
+  for (int q = 0; q < 32; ++q) {
+    if (q < warp) base += sums[q];
+    all += sums[q];
+  }
+  bins[2 * tid] = base + x - b0 - b1;
+  bins[2 * tid + 1] = base + x - b1;
+  if (tid == 0) plan->count = all;
+  __syncthreads();
+  for (int i = tid; i < places; i += kPlanThreads) {
+    const Work w = work_at(i);
+    if (w.token >= 0) plan->work[atomicAdd(&bins[bin_of(w)], 1u)] = w;
+  }
+}
+static_assert(kPlanBins == 2 * kPlanThreads, "two bins to a thread");
+
+// kPlanned: the work comes in the plan's order, else each CTA looks for its place.
+template <int HD, bool kPlanned>
 __global__ void __launch_bounds__(kThreads, 1)
     packed_kernel(const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ CUtensorMap map_k,
@@ -325,59 +432,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* kv_full = bars + 10;   // [kStages]
   uint64_t* kv_empty = kv_full + kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kStages);
-  Work* work = reinterpret_cast<Work*>(tmem_slot + 2);
+  Work* work = reinterpret_cast<Work*>(bars + 24);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kv = blockIdx.x / a.head_tiles;
   const int head0 = (blockIdx.x % a.head_tiles) * a.heads;  // first head of the group in the tile
 
-  pdl_trigger();
-  pdl_wait();
-
-  // ---- which tokens ------------------------------------------------------------
-  // Sequence s owns the places floor(start_s / (2 span)) + s and on, which
-  // leaves it room for its tiles whatever the lengths are; a place's sequence
-  // is the last one that begins at or before it. Late places first: with a
-  // causal mask they are the longest.
-  const int place = (int)gridDim.y - 1 - (int)blockIdx.y;
-  const int pair = 2 * a.span;
-  bool bad = false;
-  int begun = 0;
-  for (int s = tid; s < a.sequences; s += kThreads) {
-    const uint32_t qb = a.query_starts[s], qe = a.query_starts[s + 1];
-    const uint32_t kb = a.key_starts[s], ke = a.key_starts[s + 1];
-    bad |= qb > qe || qe > (uint32_t)a.tokens || kb > ke || ke > (uint32_t)a.keys;
-    begun += (unsigned long long)qb / pair + s <= (unsigned long long)place;
-  }
-  if (tid == 0) tmem_slot[1] = 0;
-  if (__syncthreads_or(bad)) {
-    if (tid == 0) report_fault(a.fault, kFaultStarts);
-    return;
-  }
-  begun = __reduce_add_sync(0xffffffffu, begun);
-  if (lane == 0 && begun) atomicAdd(tmem_slot + 1, (uint32_t)begun);
-  __syncthreads();
   if (tid == 0) {
-    const int s = (int)tmem_slot[1] - 1;
-    Work w{0, 0, 0, 0, 0, {0, 0}};
-    if (s >= 0) {
-      w.q0 = (int)a.query_starts[s];
-      w.q1 = (int)a.query_starts[s + 1];
-      w.k0 = (int)a.key_starts[s];
-      w.keys = (int)a.key_starts[s + 1] - w.k0;
-      const long long t = (long long)(place - (w.q0 / pair + s)) * pair;
-      w.token = t < w.q1 - w.q0 ? (int)t : -1;
-      for (int i = 0; i < 2 && w.token >= 0; ++i) {
-        const int n = w.q1 - w.q0;
-        const int last = min(n, w.token + (i + 1) * a.span) - 1;  // last token of the row tile
-        if (last < w.token + i * a.span) continue;
-        const long long seen = a.causal ? (long long)w.keys - (n - 1 - last) : w.keys;
-        w.blocks[i] = seen > 0 ? (int)((seen + kKeys - 1) / kKeys) : 0;
-      }
-    } else {
-      w.token = -1;
-    }
-    *work = w;
     pipe::mbar_init(q_full, 1);
     pipe::mbar_init(lead, 4);
     for (int i = 0; i < 2; ++i) {
@@ -391,10 +452,47 @@ __global__ void __launch_bounds__(kThreads, 1)
       pipe::mbar_init(kv_empty + i, 2);  // both tiles' issuers
     }
     pipe::fence_mbar_init();
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_q)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_k)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_v)) : "memory");
+    tmem_slot[1] = 0;
   }
-  __syncthreads();
-  const Work w = *work;
-  if (w.token < 0) return;  // a place without tokens
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- which tokens ------------------------------------------------------------
+  Work w;
+  if constexpr (kPlanned) {
+    if (blockIdx.y >= a.plan->count) return;
+    const uint4* src = reinterpret_cast<const uint4*>(&a.plan->work[blockIdx.y]);
+    reinterpret_cast<uint4*>(&w)[0] = src[0];
+    reinterpret_cast<uint4*>(&w)[1] = src[1];
+  } else {
+    // A place's sequence is the last one that begins at or before it. Late
+    // places first: with a causal mask they are the longest of their prompt.
+    const int place = (int)gridDim.y - 1 - (int)blockIdx.y;
+    bool bad = false;
+    int begun = 0;
+    for (int s = tid; s < a.sequences; s += kThreads) {
+      bad |= bad_starts(a, s);
+      begun += first_place(a, s) <= place;
+    }
+    if (__syncthreads_or(bad)) {
+      if (tid == 0) report_fault(a.fault, kFaultStarts);
+      return;
+    }
+    begun = __reduce_add_sync(0xffffffffu, begun);
+    if (lane == 0 && begun) atomicAdd(tmem_slot + 1, (uint32_t)begun);
+    __syncthreads();
+    if (tid == 0) {
+      const int s = (int)tmem_slot[1] - 1;
+      *work = s < 0 ? Work{0, 0, 0, 0, -1, {0, 0}, 0}
+                    : work_of(a, kKeys, s, (place - first_place(a, s)) * 2 * a.span);
+    }
+    __syncthreads();
+    w = *work;
+    if (w.token < 0) return;  // a place without tokens
+  }
   const int blocks = max(w.blocks[0], w.blocks[1]);
   if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -662,12 +760,31 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Heads of a row tile, its tokens, and the places of a call's row tile pairs.
+struct Shape {
+  int head_tiles, heads, span;
+  long long places;
+  bool planned;
+};
+Shape shape_of(const PackedAttention& p, int sm_count) {
+  Shape s;
+  const int group = p.qh / p.kvh;
+  s.head_tiles = (group + kTile - 1) / kTile;
+  s.heads = (group + s.head_tiles - 1) / s.head_tiles;
+  s.span = kTile / s.heads;
+  s.places = (long long)p.tokens / (2 * s.span) + p.sequences;
+  // One sequence's tiles are in order as they are, and so is what fits the GPU
+  // about at once: the plan is a launch of some 4 us.
+  s.planned = p.sequences > 1 && s.places * p.kvh * s.head_tiles > 2 * sm_count;
+  return s;
+}
+
 template <int HD>
-void launch_packed(const Launch& l, PackedArgs a) {
+void launch_packed(const Launch& l, PackedArgs a, const Shape& s, void* workspace) {
   using C = Packed<HD>;
-  a.head_tiles = (a.group + kTile - 1) / kTile;
-  a.heads = (a.group + a.head_tiles - 1) / a.head_tiles;
-  a.span = kTile / a.heads;
+  a.head_tiles = s.head_tiles;
+  a.heads = s.heads;
+  a.span = s.span;
   CUtensorMap mq, mk, mv;
   const uint64_t dq[4] = {(uint64_t)HD, (uint64_t)a.group, (uint64_t)a.kvh, (uint64_t)a.tokens};
   const uint32_t bq[4] = {64, (uint32_t)a.heads, 1, (uint32_t)a.span};
@@ -676,20 +793,29 @@ void launch_packed(const Launch& l, PackedArgs a) {
   if (!make_f16_map(&mq, a.q, 4, dq, bq) || !make_f16_map(&mk, a.k, 3, dk, bk) ||
       !make_f16_map(&mv, a.v, 3, dk, bk))
     fail(MI_ERR_KERNEL, "packed attention: tensor map encoding failed");
-  auto kernel = packed_kernel<HD>;
+  auto kernel = s.planned ? packed_kernel<HD, true> : packed_kernel<HD, false>;
   allow_dynamic_smem(kernel, C::kBytes);
-  // a place for every pair of row tiles, whatever the lengths are
-  const long long places = (long long)a.tokens / (2 * a.span) + a.sequences;
-  if (places > 65535)
+  if (s.places > 65535)
     fail(MI_ERR_SHAPE, "invalid tensor shape: %d tokens of %d sequences are too many for one call",
          a.tokens, a.sequences);
-  launch_kernel(l, dim3(a.kvh * a.head_tiles, (unsigned)places), dim3(kThreads), C::kBytes, kernel,
-                mq, mk, mv, a);
+  if (s.planned) {
+    Plan* plan = static_cast<Plan*>(workspace);
+    launch_kernel(l, dim3(1), dim3(kPlanThreads), 0, packed_plan_kernel, a, plan, (int)s.places,
+                  C::kKeys);
+    a.plan = plan;
+  }
+  launch_kernel(l, dim3(a.kvh * a.head_tiles, (unsigned)s.places), dim3(kThreads), C::kBytes,
+                kernel, mq, mk, mv, a);
 }
 
 }  // namespace
 
-void packed_attention(const Launch& l, const PackedAttention& p) {
+size_t packed_attention_workspace(const PackedAttention& p, int sm_count) {
+  const Shape s = shape_of(p, sm_count);
+  return s.planned ? sizeof(Plan) + (size_t)s.places * sizeof(Work) : 0;
+}
+
+void packed_attention(const Launch& l, const PackedAttention& p, void* workspace) {
   if (p.tokens == 0 || p.sequences == 0) return;
   PackedArgs a{};
   a.q = p.q;
@@ -707,10 +833,11 @@ void packed_attention(const Launch& l, const PackedAttention& p) {
   a.causal = p.causal;
   a.group = p.qh / p.kvh;
   a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)p.hd));
+  const Shape s = shape_of(p, l.sm_count);
   if (p.hd == 128)
-    launch_packed<128>(l, a);
+    launch_packed<128>(l, a, s, workspace);
   else
-    launch_packed<64>(l, a);
+    launch_packed<64>(l, a, s, workspace);
 }
 
 }  // namespace k
