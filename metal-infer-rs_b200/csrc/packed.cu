@@ -262,6 +262,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -306,13 +311,25 @@ struct alignas(16) Work {
 };
 static_assert(sizeof(Work) == 32, "two 16-byte words");
 
-// The row tiles from token t on of sequence s.
-__device__ __forceinline__ Work work_of(const PackedArgs& a, int key_tile, int s, long long t) {
-  Work w{0, 0, 0, 0, -1, {0, 0}, 0};
-  w.q0 = (int)a.query_starts[s];
-  w.q1 = (int)a.query_starts[s + 1];
-  w.k0 = (int)a.key_starts[s];
-  w.keys = (int)a.key_starts[s + 1] - w.k0;
+// The starts of a sequence and its successor.
+struct Starts {
+  uint32_t q0, q1, k0, k1;
+  __device__ Starts(const PackedArgs& a, int s)
+      : q0(a.query_starts[s]), q1(a.query_starts[s + 1]), k0(a.key_starts[s]),
+        k1(a.key_starts[s + 1]) {}
+  __device__ bool bad(const PackedArgs& a) const {
+    return q0 > q1 || q1 > (uint32_t)a.tokens || k0 > k1 || k1 > (uint32_t)a.keys;
+  }
+};
+// Sequence s owns the places floor(start_s / (2 span)) + s and on, which leaves
+// it room for its tiles whatever the lengths are.
+__device__ __forceinline__ long long first_place(const PackedArgs& a, uint32_t start, int s) {
+  return (long long)(start / (uint32_t)(2 * a.span)) + s;
+}
+// The row tiles from token t on of a sequence.
+__device__ __forceinline__ Work work_of(const PackedArgs& a, int key_tile, const Starts& st,
+                                        long long t) {
+  Work w{(int)st.q0, (int)st.q1, (int)st.k0, (int)(st.k1 - st.k0), -1, {0, 0}, 0};
   const int n = w.q1 - w.q0;
   w.token = t < n ? (int)t : -1;
 #pragma unroll
@@ -324,17 +341,6 @@ __device__ __forceinline__ Work work_of(const PackedArgs& a, int key_tile, int s
   }
   return w;
 }
-// Sequence s owns the places floor(start_s / (2 span)) + s and on, which leaves
-// it room for its tiles whatever the lengths are.
-__device__ __forceinline__ long long first_place(const PackedArgs& a, int s) {
-  return (long long)(a.query_starts[s] / (uint32_t)(2 * a.span)) + s;
-}
-__device__ __forceinline__ bool bad_starts(const PackedArgs& a, int s) {
-  const uint32_t qb = a.query_starts[s], qe = a.query_starts[s + 1];
-  const uint32_t kb = a.key_starts[s], ke = a.key_starts[s + 1];
-  return qb > qe || qe > (uint32_t)a.tokens || kb > ke || ke > (uint32_t)a.keys;
-}
-
 // ---- the order of the work ------------------------------------------------------
 // All sequences' row tiles, the ones that see most keys first (a counting sort
 // by key tiles): the CTAs that start last are then the shortest. Without it the
@@ -357,7 +363,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedA
   pdl_wait();
   pdl_trigger();
   bool bad = false;
-  for (int s = tid; s < a.sequences; s += kPlanThreads) bad |= bad_starts(a, s);
+  for (int s = tid; s < a.sequences; s += kPlanThreads) bad |= Starts(a, s).bad(a);
   if (__syncthreads_or(bad)) {
     if (tid == 0) {
       report_fault(a.fault, kFaultStarts);
@@ -369,11 +375,12 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedA
     int lo = 0, hi = a.sequences;  // the last sequence that begins at or before it
     while (lo < hi) {
       const int mid = (lo + hi) / 2;
-      if (first_place(a, mid) <= place) lo = mid + 1;
+      if (first_place(a, a.query_starts[mid], mid) <= place) lo = mid + 1;
       else hi = mid;
     }
     if (lo == 0) return Work{0, 0, 0, 0, -1, {0, 0}, 0};
-    return work_of(a, key_tile, lo - 1, (place - first_place(a, lo - 1)) * 2 * a.span);
+    const Starts st(a, lo - 1);
+    return work_of(a, key_tile, st, (place - first_place(a, st.q0, lo - 1)) * 2 * a.span);
   };
   auto bin_of = [&](const Work& w) {  // longest first
     return kPlanBins - 1 - min(kPlanBins - 1, max(w.blocks[0], w.blocks[1]));
@@ -455,45 +462,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_q)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_k)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_v)) : "memory");
-    tmem_slot[1] = 0;
+    work->token = -1;
   }
-  pdl_wait();
-  pdl_trigger();
-
-  // ---- which tokens ------------------------------------------------------------
-  Work w;
-  if constexpr (kPlanned) {
-    if (blockIdx.y >= a.plan->count) return;
-    const uint4* src = reinterpret_cast<const uint4*>(&a.plan->work[blockIdx.y]);
-    reinterpret_cast<uint4*>(&w)[0] = src[0];
-    reinterpret_cast<uint4*>(&w)[1] = src[1];
-  } else {
-    // A place's sequence is the last one that begins at or before it. Late
-    // places first: with a causal mask they are the longest of their prompt.
-    const int place = (int)gridDim.y - 1 - (int)blockIdx.y;
-    bool bad = false;
-    int begun = 0;
-    for (int s = tid; s < a.sequences; s += kThreads) {
-      bad |= bad_starts(a, s);
-      begun += first_place(a, s) <= place;
-    }
-    if (__syncthreads_or(bad)) {
-      if (tid == 0) report_fault(a.fault, kFaultStarts);
-      return;
-    }
-    begun = __reduce_add_sync(0xffffffffu, begun);
-    if (lane == 0 && begun) atomicAdd(tmem_slot + 1, (uint32_t)begun);
-    __syncthreads();
-    if (tid == 0) {
-      const int s = (int)tmem_slot[1] - 1;
-      *work = s < 0 ? Work{0, 0, 0, 0, -1, {0, 0}, 0}
-                    : work_of(a, kKeys, s, (place - first_place(a, s)) * 2 * a.span);
-    }
-    __syncthreads();
-    w = *work;
-    if (w.token < 0) return;  // a place without tokens
-  }
-  const int blocks = max(w.blocks[0], w.blocks[1]);
   if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      pipe::smem_u32(tmem_slot)),
@@ -501,9 +471,45 @@ __global__ void __launch_bounds__(kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if constexpr (!kPlanned) __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- which tokens ------------------------------------------------------------
+  Work w;
+  bool bad = false;
+  if constexpr (kPlanned) {
+    w.token = -1;
+    if (blockIdx.y < a.plan->count) {
+      const uint4* src = reinterpret_cast<const uint4*>(&a.plan->work[blockIdx.y]);
+      reinterpret_cast<uint4*>(&w)[0] = src[0];
+      reinterpret_cast<uint4*>(&w)[1] = src[1];
+    }
+  } else {
+    // A place lies in one sequence or in none. Late places first: with a causal
+    // mask they are the longest of their prompt.
+    const int place = (int)gridDim.y - 1 - (int)blockIdx.y;
+    for (int s = tid; s < a.sequences; s += kThreads) {
+      const Starts st(a, s);
+      bad |= st.bad(a);
+      const long long f = first_place(a, st.q0, s);
+      if (f <= place && place < first_place(a, st.q1, s + 1))
+        *work = work_of(a, kKeys, st, (place - f) * 2 * a.span);
+    }
+  }
   fence_before();
-  __syncthreads();
+  bad = __syncthreads_or(bad);
   fence_after();
+  if constexpr (!kPlanned) w = *work;
+  if (bad || w.token < 0) {  // starts that do not rise or leave their rows, or nothing to do
+    if (bad && tid == 0) report_fault(a.fault, kFaultStarts);
+    if (warp == 8)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot),
+                   "r"(512)
+                   : "memory");
+    return;
+  }
+  const int blocks = max(w.blocks[0], w.blocks[1]);
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -713,8 +719,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       float la, lb;
       split(l2, la, lb);
       const float inv = 1.f / (la + lb);
-      bool odd = false;  // something that is not finite
-#pragma unroll 1
+      uint64_t odd2 = 0;  // stays 0 while all is finite: a sum of 0 * value
+      const uint64_t inv2 = pair_of(inv, inv);
+      // The rows go through this tile's query tile in shared memory, which its
+      // products have read, so that they leave as whole lines: a row to a
+      // thread touches a line with every 16 bytes (5,100 clocks to a CTA, 1,XXX so).
+      uint8_t* stage = smem + t * C::kQBytes + (warp & 3) * 32 * (HD * 2);
+      constexpr int kChunks = HD / 8;
+#pragma unroll
       for (int c = 0; c < HD; c += 32) {
         uint32_t o[32];
         tmem_ld32(o, to + c);
@@ -726,16 +738,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           __half2* hv = reinterpret_cast<__half2*>(&v);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = __uint_as_float(o[q * 8 + 2 * e]) * inv;
-            const float y = __uint_as_float(o[q * 8 + 2 * e + 1]) * inv;
-            odd |= !(fabsf(x) <= 65504.f) || !(fabsf(y) <= 65504.f);
+            const uint64_t z = mul2(pair_of(__uint_as_float(o[q * 8 + 2 * e]),
+                                            __uint_as_float(o[q * 8 + 2 * e + 1])),
+                                    inv2);
+            odd2 = fma2(z, 0, odd2);
+            float x, y;
+            split(z, x, y);
             hv[e] = __floats2half2_rn(x, y);
           }
           if (visible == 0) v = make_uint4(0, 0, 0, 0);
-          if (valid) reinterpret_cast<uint4*>(a.out + at + c)[q] = v;
+          const int chunk = c / 8 + q;
+          *reinterpret_cast<uint4*>(stage + lane * (HD * 2) + ((chunk ^ (lane & 7)) << 4)) = v;
         }
       }
-      unsigned again = __ballot_sync(0xffffffffu, odd && visible > 0);
+      __syncwarp();
+      const unsigned long long mine_at = valid ? (unsigned long long)at : ~0ull;
+#pragma unroll 4
+      for (int r = lane / kChunks; r < 32; r += 32 / kChunks) {
+        const unsigned long long to_row = __shfl_sync(0xffffffffu, mine_at, r);
+        const int chunk = lane % kChunks;
+        if (to_row != ~0ull)
+          reinterpret_cast<uint4*>(a.out + to_row)[chunk] = *reinterpret_cast<const uint4*>(
+              stage + r * (HD * 2) + ((chunk ^ (r & 7)) << 4));
+      }
+      __syncwarp();
+      float odd0, odd1;
+      split(odd2, odd0, odd1);
+      unsigned again = __ballot_sync(0xffffffffu, !(odd0 + odd1 == 0.f) && visible > 0);
       while (again) {
         const int who = __ffs(again) - 1;
         again &= again - 1;
