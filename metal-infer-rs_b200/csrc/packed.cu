@@ -6,8 +6,10 @@
 //
 // Tensor-bound: 4 d operations per visible (query, key) pair and head on the
 // tcgen05 pipe, with the exponentials (16 per clock and SM) close behind at
-// head_dim 128 and ahead of it at 64; a quarter of them run as polynomials on
-// the FMA pipe (none 557 us, half 574, a quarter 532).
+// head_dim 128 and ahead of it at 64. A long prompt runs at the board's power
+// limit (8192 tokens: 1.55 of 1.965 GHz), so instructions cost clock: a quarter
+// of the exponentials as polynomials on the FMA pipe shortened the softmax and
+// lost 3% all the same.
 //
 // A CTA takes two row tiles of one sequence and KV head. The rows of a tile
 // are the query heads of the group for up to 128 / group tokens, so a short
@@ -49,7 +51,6 @@ constexpr int kTile = 128;     // rows of a row tile
 constexpr int kThreads = 384;
 constexpr uint64_t kWaitNs = 200ull * 1000 * 1000;
 constexpr int kLeadBlocks = 4; // key tiles from which row tile 1 starts after row tile 0
-constexpr int kPolyOf4 = 1;    // of four pairs of weights, those on the FMA pipe
 constexpr float kGrowth = 8.f; // log2 of the weights' largest value
 
 struct PackedArgs {
@@ -131,6 +132,23 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint32_
       return false;
     }
   return true;
+}
+// The same by a whole warp, with one answer for all of its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* fault) {
+  return __all_sync(0xffffffffu, wait_for(bar, parity, fault));
+}
+// Whether a wait would return at once. Asked early, the answer comes while the
+// asking warp works: even a wait that is over costs 150 to 200 clocks.
+__device__ __forceinline__ bool is_over(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n"
+      " mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(pipe::smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 __device__ __forceinline__ void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(pipe::smem_u32(bar)) : "memory");
@@ -277,30 +295,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x of two values on the FMA pipe, x <= 126: x = n + f with n the nearest
-// integer (the low bits of x + 1.5 2^23), 2^f by a degree-4 polynomial (least
-// largest relative error on [-1/2, 1/2], fitted: 2.6e-6), n added to the
-// exponent. x is held at -126 from below, whose power FP16 rounds to 0.
-__device__ __forceinline__ void exp2_poly2(uint64_t x, float& lo, float& hi) {
-  float a, b;
-  split(x, a, b);
-  x = pair_of(fmaxf(a, -126.f), fmaxf(b, -126.f));
-  const uint64_t magic = pair_of(12582912.f, 12582912.f);
-  const uint64_t t = add2(x, magic);
-  const uint64_t n = add2(t, pair_of(-12582912.f, -12582912.f));
-  const uint64_t f = fma2(n, pair_of(-1.f, -1.f), x);
-  uint64_t p = pair_of(0.009570101276f, 0.009570101276f);
-  p = fma2(p, f, pair_of(0.05591785908f, 0.05591785908f));
-  p = fma2(p, f, pair_of(0.2402474433f, 0.2402474433f));
-  p = fma2(p, f, pair_of(0.6931217909f, 0.6931217909f));
-  p = fma2(p, f, pair_of(0.9999992847f, 0.9999992847f));
-  float ta, tb;
-  split(p, a, b);
-  split(t, ta, tb);
-  lo = __int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23));
-  hi = __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23));
-}
-
 // What a CTA works on: two row tiles.
 struct alignas(16) Work {
   int q0, q1;      // the sequence's query rows
@@ -345,7 +339,7 @@ __device__ __forceinline__ Work work_of(const PackedArgs& a, int key_tile, const
 // All sequences' row tiles, the ones that see most keys first (a counting sort
 // by key tiles): the CTAs that start last are then the shortest. Without it the
 // longest prompt's tiles may come last: 10 prompts of 20 to 2500 tokens took
-// 100 us, XXX so. The order among equals depends on timing, the results do not.
+// 100 us, 96 so, the plan's launch included. The order among equals depends on timing, the results do not.
 struct Plan {
   uint32_t count;
   uint32_t pad[7];
@@ -558,8 +552,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = wait_for(q_full, 0, a.fault);
       // The tiles' softmaxes share the exponential unit; begun together they
       // would stay in step, both at their exponentials and then neither. Tile
-      // 1 begins when tile 0 has its first maximum (8192 tokens: 567 us in step,
-      // 532 so).
+      // 1 begins when tile 0 has its first maximum (head_dim 64, prompts over
+      // prefixes: 136 us in step, 128 so; no difference at 128).
       if (t == 1 && min(w.blocks[0], w.blocks[1]) >= kLeadBlocks)
         ok = ok && wait_for(lead, 0, a.fault);
       // stage n: the scores of key tile n, then the values of n - 1
@@ -617,9 +611,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m = -INFINITY;
     uint64_t l2 = 0;  // two partial sums
     const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2);
-    bool ok = true;
+    bool ok = true, scored = false;
     for (int i = 0; i < mine; ++i) {
-      ok = wait_for(s_full + t, i & 1, a.fault);
+      if (!__all_sync(0xffffffffu, scored)) ok = warp_wait(s_full + t, i & 1, a.fault);
       if (!ok) break;
       fence_after();
       uint32_t s[kKeys];
@@ -659,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         m = base;
         if (i > 0) {
           l2 = fma2(l2, pair_of(factor, factor), 0);
-          ok = wait_for(o_full + t, (i - 1) & 1, a.fault);
+          ok = warp_wait(o_full + t, (i - 1) & 1, a.fault);
           if (!ok) break;
           fence_after();
 #pragma unroll 1
@@ -676,6 +670,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (i == 0 && t == 0 && lane == 0) arrive(lead);
+      // P is free once the product of the step before is done
+      const bool free = i == 0 || is_over(o_full + t, (i - 1) & 1);
       const float base = m == -INFINITY ? 0.f : -m;
       const uint64_t base2 = pair_of(base, base);
       uint32_t p[kKeys / 2];
@@ -684,25 +680,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t x = fma2(pair_of(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])),
                                 scale2, base2);
         float w0, w1;
-        if (e % 4 < kPolyOf4) {
-          exp2_poly2(x, w0, w1);
-        } else {
-          split(x, w0, w1);
-          w0 = exp2_fast(w0);
-          w1 = exp2_fast(w1);
-        }
+        split(x, w0, w1);
+        w0 = exp2_fast(w0);
+        w1 = exp2_fast(w1);
         // the sum takes the weights before their rounding to FP16, which is
         // off by half a step at most and to either side
         l2 = add2(l2, pair_of(w0, w1));
         const __half2 h = __floats2half2_rn(w0, w1);
         p[e] = *reinterpret_cast<const uint32_t*>(&h);
       }
-      // P is free once the product of the step before is done
-      if (i > 0) {
-        ok = wait_for(o_full + t, (i - 1) & 1, a.fault);
-        if (!ok) break;
-        fence_after();
-      }
+      if (!__all_sync(0xffffffffu, free)) ok = warp_wait(o_full + t, (i - 1) & 1, a.fault);
+      if (!ok) break;
+      fence_after();
+      scored = i + 1 < mine && is_over(s_full + t, (i + 1) & 1);
 #pragma unroll
       for (int c = 0; c + 32 <= kKeys / 2; c += 32) tmem_st32(tp + c, p + c);
       if constexpr (kKeys % 64 != 0) tmem_st8(tp + kKeys / 2 - 8, p + kKeys / 2 - 8);
@@ -714,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- output ---------------------------------------------------------------------
     const size_t stride = (size_t)a.kvh * HD;
     const size_t at = ((size_t)(w.q0 + token) * a.qh + (size_t)kv * a.group + head) * HD;
-    if (mine > 0 && ok && wait_for(o_full + t, (mine - 1) & 1, a.fault)) {
+    if (mine > 0 && ok && warp_wait(o_full + t, (mine - 1) & 1, a.fault)) {
       fence_after();
       float la, lb;
       split(l2, la, lb);
@@ -723,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t inv2 = pair_of(inv, inv);
       // The rows go through this tile's query tile in shared memory, which its
       // products have read, so that they leave as whole lines: a row to a
-      // thread touches a line with every 16 bytes (5,100 clocks to a CTA, 1,XXX so).
+      // thread touches a line with every 16 bytes (5,100 clocks to a CTA, 2,900 so).
       uint8_t* stage = smem + t * C::kQBytes + (warp & 3) * 32 * (HD * 2);
       constexpr int kChunks = HD / 8;
 #pragma unroll

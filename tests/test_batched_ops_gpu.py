@@ -812,3 +812,25 @@ def test_refusals(ctx):
     huge = ctx.tensor_from_device(few.data_ptr(), [2, 2 ** 22 + 1], F16)
     refused(mi.ERR_SHAPE, "logits a row", sample_with(x=huge, o=u(2)))
     refused(mi.ERR_INVALID_ARGUMENT, "NULL", lambda b: mi._check(mi.lib().mi_batch_sample(b._h, *[None] * 7)))
+
+
+def test_offsets_beyond_32_bits(ctx):
+    # caches of more than 2^32 values: the pages at their end
+    rng = np.random.default_rng(41)
+    page, kvh, hd, n = 16, 8, 128, 77
+    pages = 2 ** 32 // (page * kvh * hd) + 8
+    kc, vc = ctx.empty([pages, page, kvh, hd], F16), ctx.empty([pages, page, kvh, hd], F16)
+    table = (pages - 1 - np.arange(5)[None]).astype(np.uint32)
+    q, k, v = normal(rng, n, 16, hd), normal(rng, n, kvh, hd), normal(rng, n, kvh, hd)
+    out = up(ctx, np.zeros((1, 16, hd), np.float16))
+    small = [ctx.empty([8, page, kvh, hd], F16) for _ in range(2)]
+    low = (7 - np.arange(5)[None]).astype(np.uint32)
+    results = []
+    for a, b, t in ((kc, vc, table), (*small, low)):
+        rotated = up(ctx, np.zeros_like(q))
+        tt, tl, ts = up(ctx, t), up(ctx, np.array([n], np.uint32)), up(ctx, np.array([0, n], np.uint32))
+        one(ctx, lambda bt: bt.paged_append(up(ctx, q), up(ctx, k), up(ctx, v), None, None, ts, tl, tt, a, b, rotated, 1e6))
+        one(ctx, lambda bt: bt.paged_attention(up(ctx, down(rotated)[-1:]), a, b, tl, tt, out))
+        results.append(down(out).view(np.uint16).copy())
+    np.testing.assert_array_equal(results[0], results[1])
+    assert np.any(results[0])
