@@ -436,8 +436,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   Work* work = reinterpret_cast<Work*>(bars + 24);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kv = blockIdx.x / a.head_tiles;
-  const int head0 = (blockIdx.x % a.head_tiles) * a.heads;  // first head of the group in the tile
+  // heads of one place side by side: their key tiles are near each other
+  const int columns = a.kvh * a.head_tiles;
+  const int place_y = (int)(blockIdx.x / (uint32_t)columns);
+  const int kv = (int)(blockIdx.x % (uint32_t)columns) / a.head_tiles;
+  const int head0 = (int)(blockIdx.x % (uint32_t)a.head_tiles) * a.heads;  // first of the group
 
   if (tid == 0) {
     pipe::mbar_init(q_full, 1);
@@ -474,15 +477,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool bad = false;
   if constexpr (kPlanned) {
     w.token = -1;
-    if (blockIdx.y < a.plan->count) {
-      const uint4* src = reinterpret_cast<const uint4*>(&a.plan->work[blockIdx.y]);
+    if (place_y < (int)a.plan->count) {
+      const uint4* src = reinterpret_cast<const uint4*>(&a.plan->work[place_y]);
       reinterpret_cast<uint4*>(&w)[0] = src[0];
       reinterpret_cast<uint4*>(&w)[1] = src[1];
     }
   } else {
     // A place lies in one sequence or in none. Late places first: with a causal
     // mask they are the longest of their prompt.
-    const int place = (int)gridDim.y - 1 - (int)blockIdx.y;
+    const int place = (int)(gridDim.x / (uint32_t)columns) - 1 - place_y;
     for (int s = tid; s < a.sequences; s += kThreads) {
       const Starts st(a, s);
       bad |= st.bad(a);
@@ -814,7 +817,8 @@ void launch_packed(const Launch& l, PackedArgs a, const Shape& s, void* workspac
     fail(MI_ERR_KERNEL, "packed attention: tensor map encoding failed");
   auto kernel = s.planned ? packed_kernel<HD, true> : packed_kernel<HD, false>;
   allow_dynamic_smem(kernel, C::kBytes);
-  if (s.places > 65535)
+  const long long grid = s.places * a.kvh * a.head_tiles;
+  if (grid > 0x7FFFFFFF)
     fail(MI_ERR_SHAPE, "invalid tensor shape: %d tokens of %d sequences are too many for one call",
          a.tokens, a.sequences);
   if (s.planned) {
@@ -823,7 +827,7 @@ void launch_packed(const Launch& l, PackedArgs a, const Shape& s, void* workspac
                   C::kKeys);
     a.plan = plan;
   }
-  launch_kernel(l, dim3(a.kvh * a.head_tiles, (unsigned)s.places), dim3(kThreads), C::kBytes,
+  launch_kernel(l, dim3((unsigned)grid), dim3(kThreads), C::kBytes,
                 kernel, mq, mk, mv, a);
 }
 

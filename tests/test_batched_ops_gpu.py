@@ -834,3 +834,83 @@ def test_offsets_beyond_32_bits(ctx):
         results.append(down(out).view(np.uint16).copy())
     np.testing.assert_array_equal(results[0], results[1])
     assert np.any(results[0])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_large_groups(ctx, hd):
+    # more query heads to a KV head than a row tile or a product has places
+    rng = np.random.default_rng(42)
+    lengths = [37, 90]
+    table, pages = paged(rng, lengths, 16)
+    q, kc, vc = normal(rng, 2, 200, hd), normal(rng, pages, 16, 1, hd), normal(rng, pages, 16, 1, hd)
+    check_paged(q, kc, vc, lengths, table, 16, run_paged(ctx, q, kc, vc, lengths, table))
+    qs, ks = starts([5, 3]), starts([5, 103])
+    q, k, v = normal(rng, 8, 200, hd), normal(rng, 108, 1, hd), normal(rng, 108, 1, hd)
+    check_packed(q, k, v, qs, ks, True, run_packed(ctx, q, k, v, qs, ks, True))
+
+
+def test_many_sequences(ctx):
+    # more sequences than a block has threads, prompts of every small length
+    rng = np.random.default_rng(43)
+    lengths = [i % 7 for i in range(1500)]
+    table, pages = paged(rng, lengths, 4)
+    q, kc, vc = normal(rng, 1500, 2, 64), normal(rng, pages, 4, 1, 64), normal(rng, pages, 4, 1, 64)
+    check_paged(q, kc, vc, lengths, table, 4, run_paged(ctx, q, kc, vc, lengths, table))
+    qs = ks = starts(lengths)
+    q, k, v = normal(rng, qs[-1], 2, 64), normal(rng, qs[-1], 1, 64), normal(rng, qs[-1], 1, 64)
+    check_packed(q, k, v, qs, ks, True, run_packed(ctx, q, k, v, qs, ks, True))
+    kc, vc = np.zeros((pages, 4, 1, 64), np.float16), np.zeros((pages, 4, 1, 64), np.float16)
+    _, _, got = run_append(ctx, None, k, v, None, None, qs, lengths, table, kc, vc)
+    for s in range(0, 1500, 97):
+        np.testing.assert_array_equal(got.reshape(-1, 1, 64)[rows_of(table, s, lengths[s], 4)], v[qs[s]:qs[s + 1]])
+
+
+@pytest.mark.parametrize("n", [1000003, 2 ** 22])
+@pytest.mark.parametrize("kind", ["normal", "equal", "lowest"])
+def test_sample_counts_beyond_16_bits(ctx, kind, n):
+    rng = np.random.default_rng(44)
+    options = [OPTIONS[0] + (0.37,), OPTIONS[8] + (UNIFORMS[-1],), (1.0, n // 2, 0.9, 0.0, 0.99)]
+    bits = np.stack([logits_of(kind, rng, n) for _ in options])
+    want = np.array([sample64(b, *o) for b, o in zip(bits, options)], np.uint32)
+    np.testing.assert_array_equal(run_sample(ctx, bits, options), want)
+    # as many rows as make a CTA take a whole one
+    many = run_sample(ctx, np.tile(bits, (8, 1)), options * 8) if n < 2 ** 22 else np.tile(want, 8)
+    np.testing.assert_array_equal(many, np.tile(want, 8))
+
+
+def test_a_captured_step_of_all_ops(ctx):
+    rng = np.random.default_rng(45)
+    page, hd, qh, kvh, width = 16, 128, 8, 2, 20
+    prompts = [150, 3, 90]
+    st = starts(prompts)
+    table = rng.permutation(3 * width).reshape(3, width).astype(np.uint32)
+    q, k, v = (normal(rng, st[-1], h, hd) for h in (qh, kvh, kvh))
+    logits = normal(rng, 40, 3000)
+    kc, vc = ctx.empty([3 * width, page, kvh, hd], F16), ctx.empty([3 * width, page, kvh, hd], F16)
+    t = {n: up(ctx, x) for n, x in dict(
+        q=q, k=k, v=v, st=st.astype(np.uint32), n=np.array(prompts, np.uint32), table=table, last=q[st[1:] - 1],
+        logits=logits, temp=np.full(40, 0.8, np.float32), top_k=np.full(40, 50, np.uint32),
+        top_p=np.full(40, 0.9, np.float32), min_p=np.zeros(40, np.float32),
+        u=rng.random(40).astype(np.float32)).items()}
+    rotated, packed_out, paged_out, tokens = (up(ctx, np.zeros_like(q)), up(ctx, np.zeros_like(q)),
+                                              up(ctx, np.zeros((3, qh, hd), np.float16)), ctx.empty([40], U32))
+
+    def step(b):
+        b.paged_append(t["q"], t["k"], t["v"], None, None, t["st"], t["n"], t["table"], kc, vc, rotated, 1e6)
+        b.packed_attention(t["q"], t["k"], t["v"], t["st"], t["st"], True, packed_out)
+        b.paged_attention(t["last"], kc, vc, t["n"], t["table"], paged_out)
+        b.sample(t["logits"], t["temp"], t["top_k"], t["top_p"], t["min_p"], t["u"], tokens)
+
+    outs = (rotated, packed_out, paged_out, tokens)
+    one(ctx, step)
+    eager = [down(o).copy() for o in outs]
+    graph = Graph().capture(ctx, step)
+    for _ in range(3):
+        for o in outs:
+            o.write(np.zeros_like(down(o)))
+        graph.replay(ctx.stream())
+        ctx.synchronize()
+        for o, e in zip(outs, eager):
+            np.testing.assert_array_equal(down(o).view(np.uint16), e.view(np.uint16))
+    graph.close()
+    check_packed(q, k, v, st, st, True, eager[1])
