@@ -17,14 +17,14 @@
 //
 // A CTA counts 16 bits to a key (128 KB of shared memory). The shared-memory
 // additions set the pace, so a row that shares the GPU with many others has
-// one CTA and nothing to add up between CTAs; where rows are few, a cluster of
-// 8 CTAs takes a row: each counts an eighth of it, then adds up the keys of
-// its own over the cluster's histograms (blocks of 64 keys by turns, as a
-// row's values share a few exponents). Measured, 96 rows of 151,936: 115 us
-// with 4 CTAs to a row, 120 with every CTA reading the whole row for its own
-// keys, 47 so; one row 15 us with 8 CTAs. Of the 65,000 to 70,000 clocks of a
-// row's CTA the additions take 37,000 (4,750 warp-wide ones on 32 banks), the
-// weights 11,000 and the search for the token's index 7,000.
+// one CTA and nothing to add up between CTAs; where rows are fewer, a cluster
+// of 2, 4 or 8 CTAs takes a row: each counts its share of it, then adds up the
+// keys of its own over the cluster's histograms (blocks of 64 keys by turns,
+// as a row's values share a few exponents). Measured, 96 rows of 151,936: 115
+// us with 4 CTAs to a row, 120 with every CTA reading the whole row for its
+// own keys, 45 so; one row 15 to 19 us. Of the 65,000 to 70,000 clocks of a
+// row's only CTA the additions take 37,000 (4,750 warp-wide ones on 32 banks),
+// the weights 11,000 and the search for the token's index 7,000.
 
 #include <cooperative_groups.h>
 
@@ -51,9 +51,9 @@ constexpr int kSegment = 49152;
 constexpr uint32_t kLarge = 65535 - kSegment;
 constexpr int kLargeMax = kSampleBatchMax / (int)kLarge + 1;
 
-// A thread has groups of eight keys: one where a cluster shares the row, and
-// 8 of a CTA's own, 1,024 groups apart, so that the few exponents that hold
-// most of a row keep all warps busy.
+// A thread has a group of eight keys in each of its rounds: 8 where the CTA
+// has the row to itself, 1,024 groups apart, so that the few exponents that
+// hold most of a row keep all warps busy; fewer where a cluster shares it.
 template <int kCtas>
 constexpr int kRounds = kGroups / kThreads / kCtas;
 
@@ -61,7 +61,7 @@ template <int kCtas>
 struct Shared {
   uint32_t hist[65536 / 2];  // two 16-bit counts to a word
   double mass[kRounds<kCtas>][kThreads];  // sum of a thread's candidates, per round
-  double warp_sums[kRounds<kCtas> * kWarps];
+  double warp_sums[kCtas == 1 ? kRounds<1> * kWarps : kWarps];
   double total;
   double blocks_before[kCtas == 1 ? 1 : kBlocks];
   double step[64];           // weight of one step of an exponent's values (sign in front)
@@ -205,19 +205,22 @@ __device__ __forceinline__ T row_exclusive(Shared<kCtas>& sh, int rank,
     for (int r = 0; r < kR; ++r) before[r] += sums[r * kWarps + warp];
     return *reinterpret_cast<T*>(&sh.total);
   } else {
-    // eight threads to a block; block b of the row is block b / kCtas of CTA
-    // b % kCtas. Each CTA adds up all blocks.
-    T x = v[0];
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      const T y = __shfl_up_sync(0xffffffffu, x, o, 8);
-      if (tid % 8 >= o) x += y;
-    }
-    T up = __shfl_up_sync(0xffffffffu, x, 1, 8);
-    if (tid % 8 == 0) up = T(0);
+    // eight threads to a block, 128 blocks to a round; block b of the row is
+    // block b / kCtas of CTA b % kCtas. Each CTA adds up all blocks.
     T* own = reinterpret_cast<T*>(sh.block_sums);
     T* all = reinterpret_cast<T*>(sh.blocks_before);
-    if (tid % 8 == 7) own[tid / 8] = x;
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      T x = v[r];
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        const T y = __shfl_up_sync(0xffffffffu, x, o, 8);
+        if (tid % 8 >= o) x += y;
+      }
+      before[r] = __shfl_up_sync(0xffffffffu, x, 1, 8);
+      if (tid % 8 == 0) before[r] = T(0);
+      if (tid % 8 == 7) own[r * (kThreads / 8) + tid / 8] = x;
+    }
     row_sync<kCtas>();
     T z = of_rank<kCtas>(own, tid % kCtas)[tid / kCtas];
 #pragma unroll
@@ -240,7 +243,9 @@ __device__ __forceinline__ T row_exclusive(Shared<kCtas>& sh, int rank,
     if (warp) earlier += base;
     all[tid] = earlier;
     __syncthreads();
-    before[0] = all[tid / 8 * kCtas + rank] + up;
+#pragma unroll
+    for (int r = 0; r < kR; ++r)
+      before[r] += all[(r * (kThreads / 8) + tid / 8) * kCtas + rank];
     return total;
   }
 }
@@ -283,7 +288,6 @@ __device__ __forceinline__ bool row_first(Shared<kCtas>& sh, int rank, bool has,
 template <int kCtas>
 __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleBatch p) {
   constexpr int kR = kRounds<kCtas>;
-  static_assert(kCtas == 1 || kR == 1, "a thread of a cluster has one group");
   extern __shared__ __align__(16) uint8_t smem[];
   Shared<kCtas>& sh = *reinterpret_cast<Shared<kCtas>*>(smem);
   const int rank = kCtas == 1 ? 0 : (int)(blockIdx.x % kCtas);
@@ -397,7 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
     const double most = key_value(top);
     // this thread's group of a round, in descending order of keys
     auto group_of = [&](int r) -> uint32_t {
-      return kCtas == 1 ? r * kThreads + tid : (tid / 8 * kCtas + rank) * 8 + tid % 8;
+      return kCtas == 1 ? r * kThreads + tid
+                        : ((r * (kThreads / 8) + tid / 8) * kCtas + rank) * 8 + tid % 8;
     };
     // Counts of a group's keys, over the cluster.
     auto counts = [&](uint32_t k0, uint32_t (&c)[8]) {
@@ -425,11 +430,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
           }
         }
     };
-    // A cluster's thread has one group and adds up its counts once.
+    // A thread with one group adds up its counts over the cluster once.
     uint32_t group_counts[8];
-    if constexpr (kCtas > 1) counts(group_of(0) * 8, group_counts);
+    if constexpr (kR == 1) counts(group_of(0) * 8, group_counts);
     auto group = [&](int r, uint32_t (&c)[8]) {
-      if constexpr (kCtas > 1) {
+      if constexpr (kR == 1) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) c[e] = group_counts[e];
       } else {
@@ -743,10 +748,17 @@ void launch_sample(const Launch& l, const SampleBatch& p) {
 
 void sample_batch(const Launch& l, const SampleBatch& p) {
   if (p.rows == 0) return;
-  // Clusters of 8 while the rows fit the GPU at once so, one CTA to a row
-  // otherwise.
-  if (p.rows * 8 <= l.sm_count)
+  // As many CTAs to a row as fit the GPU at once, up to 8. Clusters of 8 and 4
+  // leave SMs of a GPC empty, which the eighth below stands for (18 rows of
+  // 151,936: 28 us with 8, 25 with 4; 36: 34 with 4, 32 with 2; 75 and more:
+  // 45 with 1).
+  const int sms = l.sm_count - l.sm_count / 8;
+  if (p.rows * 8 <= sms)
     launch_sample<8>(l, p);
+  else if (p.rows * 4 <= sms)
+    launch_sample<4>(l, p);
+  else if (p.rows * 2 <= l.sm_count)
+    launch_sample<2>(l, p);
   else
     launch_sample<1>(l, p);
 }

@@ -533,9 +533,12 @@ def test_sample_matches_its_definition(ctx, kind, n):
     rng = np.random.default_rng(n)
     options = [o + (u,) for o in OPTIONS for u in UNIFORMS]
     bits = np.stack([logits_of(kind, rng, n) for _ in options])
-    got = run_sample(ctx, bits, options)
-    want = [sample64(b, *o) for b, o in zip(bits, options)]
-    np.testing.assert_array_equal(got, np.array(want, np.uint32))
+    want = np.array([sample64(b, *o) for b, o in zip(bits, options)], np.uint32)
+    # as many rows as share the GPU among one, two, four or eight CTAs to a row
+    for rows in (60, 20, 7, 120):
+        pick = (np.arange(rows) * 7) % 60
+        got = run_sample(ctx, bits[pick], [options[i] for i in pick])
+        np.testing.assert_array_equal(got, want[pick])
 
 
 @pytest.mark.parametrize("n,kind", [(151936, "normal"), (151937, "equal"), (262144, "two values"), (524224, "normal"),
