@@ -116,7 +116,7 @@ struct mi_context {
   };
   std::vector<Profile> pending_profiles;
   std::vector<mi_kernel_profile> profiles;
-  // Reusable zero-initialised scratch for split reductions (grown on demand).
+  // Reusable scratch of ops on the context's stream (grown on demand).
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
   // Mapped host word that kernels write when they refuse a device-side

@@ -786,6 +786,17 @@ Pages require_pages(const mi_context* ctx, const mi_tensor* key_cache,
   return p;
 }
 
+// Scratch of one op. Calls on the context's stream follow one another and share
+// the context's; a captured call keeps memory of its own, so that graphs share
+// it neither with each other nor with later calls.
+void* op_scratch(mi_context* ctx, size_t bytes, Out& own) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  MI_CUDA(cudaStreamIsCapturing(ctx->stream, &status));
+  if (status == cudaStreamCaptureStatusNone) return context_scratch(ctx, bytes);
+  own.t = new_tensor(ctx, {(bytes + 3) / 4}, MI_F32);
+  return own.t->base();
+}
+
 void require_starts(const mi_context* ctx, const mi_tensor* starts, const char* what) {
   require_tensor(ctx, starts, MI_U32, 1, what);
   require_aligned(starts, 4, what);
@@ -920,12 +931,10 @@ mi_status mi_batch_paged_attention(mi_batch* b, const mi_tensor* query,
     p.table_width = (int)pg.width;
     p.page = (int)pg.page;
     p.pages = (uint32_t)pg.pages;
-    // stream-ordered scratch of this call: a captured call keeps its own, so
-    // two graphs never share it
-    Out ws;
-    ws.t = new_tensor(ctx, {k::paged_attention_workspace(ctx->sm_count, p.hd) / 4}, MI_F32);
+    Out own;
+    void* scratch = op_scratch(ctx, k::paged_attention_workspace(ctx->sm_count, p.hd), own);
     ProfileScope ps(ctx, "paged_attention");
-    k::paged_attention(launch_of(ctx), p, ws.t->base());
+    k::paged_attention(launch_of(ctx), p, scratch);
   });
 }
 
@@ -967,11 +976,12 @@ mi_status mi_batch_packed_attention(mi_batch* b, const mi_tensor* query, const m
     p.key_starts = key_starts->u32();
     p.fault = ctx->fault;
     p.causal = causal != 0;
-    Out ws;
+    Out own;
+    void* scratch = nullptr;
     if (const size_t bytes = k::packed_attention_workspace(p, ctx->sm_count))
-      ws.t = new_tensor(ctx, {(bytes + 3) / 4}, MI_F32);
+      scratch = op_scratch(ctx, bytes, own);
     ProfileScope ps(ctx, "packed_attention");
-    k::packed_attention(launch_of(ctx), p, ws.t ? ws.t->base() : nullptr);
+    k::packed_attention(launch_of(ctx), p, scratch);
   });
 }
 

@@ -281,8 +281,8 @@ void launch_append(const Launch& l, const AppendArgs& a) {
 // result layout transposed (movmatrix).
 //
 // The work is cut evenly whatever the lengths are: all (sequence, KV head,
-// head tile) units are laid end to end, each its tiles of 64 keys and kUnitCost
-// empty places for what its end costs, and CTA c of C takes the places
+// head tile) units are laid end to end, each its tiles of 64 or 128 keys and
+// kUnitCost empty places for what its end costs, and CTA c of C takes the places
 // [c N / C, (c + 1) N / C). (Without them the CTAs that met the many units of
 // short sequences set the time: 64 sequences of 1 to 8192 took 78 us, 57 with
 // them.) A unit that lies inside a CTA is
@@ -291,14 +291,13 @@ void launch_append(const Launch& l, const AppendArgs& a) {
 // timing. A CTA has at most two pieces: one that continues a unit from the
 // CTA before it (slot 0), one that a later CTA continues (slot 1).
 //
-// Each of a CTA's four warps owns 16 keys of a tile, with its own ring of
+// Each of a CTA's four warps owns a quarter of a tile, with its own ring of
 // cp.async stages (rows past the length are filled with zeros, so stale
 // values never enter a product) and its own running maximum and sum; the
 // warps meet only at a unit's end, where each leaves its state in the ring
 // stage that it has just used up. Two CTAs to an SM keep about 130 KB of
 // loads in flight.
-constexpr int kTileKeys = 64;
-constexpr int kUnitCost = 2;
+constexpr int kUnitCost = 1;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kHeadsMax = 16;
@@ -314,18 +313,22 @@ struct PagedArgs {
   int group;        // query heads per KV head
   int head_tiles;   // head tiles of a group
   int heads;        // heads of a tile (the last may have fewer)
+  int page_shift;   // log2 of the page size, -1 where it has none
   uint32_t pages;
   float scale_log2; // log2(e) / sqrt(HD)
 };
 
 template <int HD, int NT>
 struct PagedShape {
-  // CTAs to an SM, what their registers allow; head_dim 64 has half the bytes
-  // to a step of the same length, so more warps keep the loads coming (4
-  // against 2: 256 sequences of 100 to 1500 take 62 us against 63)
-  static constexpr int kCtas = HD == 128 ? 2 : NT == 1 ? 4 : 3;
+  // k16 tiles of keys of a warp's step, keys of a CTA's tile. At head_dim 64 a
+  // step of 32 keys has the bytes of 16 at 128 and pays the maximum's shuffles
+  // and the loop once for them (256 sequences of 100 to 1500: 63 us with 16
+  // keys and four CTAs to an SM, 58 so).
+  static constexpr int kSteps = HD == 128 ? 1 : 2;
+  static constexpr int kTileKeys = kWarps * kSteps * 16;
+  static constexpr int kCtas = 2;  // to an SM
   static constexpr int kStages = 3;
-  static constexpr int kStageBytes = 2 * 16 * HD * 2;  // a warp's keys and values
+  static constexpr int kStageBytes = 2 * kSteps * 16 * HD * 2;  // a warp's keys and values
   static constexpr int kBytes = kWarps * kStages * kStageBytes;
 };
 constexpr size_t piece_floats(int hd) { return kHeadsMax * hd + 2 * kHeadsMax; }
@@ -387,17 +390,19 @@ struct Cursor {
   uint32_t len;
 };
 // Places of a unit of n keys.
+template <int kTileKeys>
 __device__ __forceinline__ uint32_t unit_places(uint32_t n) {
   return n ? (n + kTileKeys - 1) / kTileKeys + kUnitCost : 0;
 }
 
 // NT: 8-head column tiles. kRuns: the page size is a multiple of 16, so a
-// warp's 16 keys lie in one page (one table entry and one address to a stage).
+// 16 keys of a step lie in one page (one table entry and one address for them).
 template <int HD, int NT, bool kRuns>
 __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
     paged_attention_kernel(const PagedArgs a) {
   using S = PagedShape<HD, NT>;
-  constexpr int kStages = S::kStages;
+  constexpr int kStages = S::kStages, kSteps = S::kSteps, kTileKeys = S::kTileKeys;
+  constexpr int kRowsStep = 16 * kSteps;  // keys of a warp's step
   constexpr int kK = HD / 16;      // k16 steps of a score, m16 tiles of an output column
   constexpr int kChunks = HD / 8;  // 16-byte chunks of a row
   // row of a state in the ring: padded against bank conflicts where it fits
@@ -421,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
     const int s = tid * run + i;
     if (s < a.sequences) {
       const uint32_t n = paged_length(a, s);
-      mine += unit_places(n);
+      mine += unit_places<kTileKeys>(n);
       if (n == 0 && s % gridDim.x == blockIdx.x && a.lengths[s] != 0)
         report_fault(a.fault, kFaultLength);
     }
@@ -456,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
       const int s = tid * run + i;
       if (s >= a.sequences) break;
       const uint32_t n = paged_length(a, s);
-      const uint32_t places = unit_places(n);
+      const uint32_t places = unit_places<kTileKeys>(n);
       const unsigned long long next = at + (unsigned long long)places * units;
       if (at <= begin && begin < next) {
         const unsigned long long w = begin - at;
@@ -492,12 +497,13 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
 
   const uint32_t ring = pipe::smem_u32(smem) + warp * kStages * S::kStageBytes;
   const uint32_t row_stride = a.kvh * HD;
-  // Cache row of this warp's key lane % 16 of a tile (its first one, kRuns);
-  // all ones where there is none.
+  // Cache row of this warp's key `lane` of a tile (kRuns: of key 16 lane, the
+  // first of a run); all ones where there is none.
   auto row_of = [&](const Cursor& c) -> uint32_t {
-    const uint32_t p = (uint32_t)c.tile * kTileKeys + warp * 16 + (kRuns ? 0 : lane & 15);
-    if (p >= c.len) return 0xFFFFFFFFu;
-    const uint32_t pi = p / (uint32_t)a.page;
+    const int key = kRuns ? (lane < kSteps ? lane * 16 : kRowsStep) : lane;
+    const uint32_t p = (uint32_t)c.tile * kTileKeys + warp * kRowsStep + key;
+    if (key >= kRowsStep || p >= c.len) return 0xFFFFFFFFu;
+    const uint32_t pi = a.page_shift >= 0 ? p >> a.page_shift : p / (uint32_t)a.page;
     const uint32_t pg = a.table[(size_t)c.s * a.table_width + pi];
     if (pg >= a.pages) {
       report_fault(a.fault, kFaultPage);
@@ -512,29 +518,35 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
     const int kv = c.unit / a.head_tiles;
     const size_t head = (size_t)kv * HD + chunk * 8;
     if constexpr (kRuns) {
-      // rows past the length are not read
-      const int left = rows == 0xFFFFFFFFu ? 0
-                                           : (int)c.len - c.tile * kTileKeys - warp * 16 - row0;
-      const size_t off = rows == 0xFFFFFFFFu ? head : (size_t)(rows + row0) * row_stride + head;
+      const int last = (int)c.len - c.tile * kTileKeys - warp * kRowsStep - row0;
 #pragma unroll
-      for (int i = 0; i < 16 / kRowsPerPass; ++i) {
-        const int r = i * kRowsPerPass;
-        const uint32_t bytes = r < left ? 16 : 0;
-        const size_t at = r < left ? off + (size_t)r * row_stride : head;
-        const uint32_t d = dst + r * (HD * 2) + ((chunk ^ ((r + row0) & 7)) << 4);
-        cp_async16_zfill(d, a.kc + at, bytes);
-        cp_async16_zfill(d + 16 * HD * 2, a.vc + at, bytes);
+      for (int run = 0; run < kSteps; ++run) {
+        const uint32_t first_row = __shfl_sync(0xffffffffu, rows, run);
+        const bool none = first_row == 0xFFFFFFFFu;
+        // rows past the length are not read
+        const int left = none ? 0 : last - run * 16;
+        const size_t off = none ? head : (size_t)(first_row + row0) * row_stride + head;
+#pragma unroll
+        for (int i = 0; i < 16 / kRowsPerPass; ++i) {
+          const int r = i * kRowsPerPass;
+          const uint32_t bytes = r < left ? 16 : 0;
+          const size_t at = r < left ? off + (size_t)r * row_stride : head;
+          const uint32_t d =
+              dst + (run * 16 + r) * (HD * 2) + ((chunk ^ ((r + row0) & 7)) << 4);
+          cp_async16_zfill(d, a.kc + at, bytes);
+          cp_async16_zfill(d + kRowsStep * HD * 2, a.vc + at, bytes);
+        }
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 16 / kRowsPerPass; ++i) {
+      for (int i = 0; i < kRowsStep / kRowsPerPass; ++i) {
         const int r = i * kRowsPerPass;
         const uint32_t row = __shfl_sync(0xffffffffu, rows, r + row0);
         const uint32_t bytes = row != 0xFFFFFFFFu ? 16 : 0;
         const size_t at = row != 0xFFFFFFFFu ? (size_t)row * row_stride + head : head;
         const uint32_t d = dst + r * (HD * 2) + ((chunk ^ ((r + row0) & 7)) << 4);
         cp_async16_zfill(d, a.kc + at, bytes);
-        cp_async16_zfill(d + 16 * HD * 2, a.vc + at, bytes);
+        cp_async16_zfill(d + kRowsStep * HD * 2, a.vc + at, bytes);
       }
     }
   };
@@ -596,29 +608,37 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
       cp_async_wait<kStages - 1>();
       __syncwarp();
       const uint32_t kbase = ring + stage * S::kStageBytes;
-      const uint32_t vbase = kbase + 16 * HD * 2;
+      const uint32_t vbase = kbase + kRowsStep * HD * 2;
 
-      // scores of 16 keys x 8 NT heads
-      float sc[NT][4] = {};
+      // scores of 16 kSteps keys x 8 NT heads
+      float sc[kSteps][NT][4] = {};
 #pragma unroll
-      for (int kk = 0; kk < kK; ++kk) {
-        uint32_t k4[4];
-        ldsm4(k4, kbase + key_k * (HD * 2) + (((2 * kk + chunk_k) ^ (key_k & 7)) << 4));
+      for (int u = 0; u < kSteps; ++u)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816(sc[n], k4, qf[n][kk][0], qf[n][kk][1]);
-      }
-      const uint32_t p0 = (uint32_t)comp.tile * kTileKeys + warp * 16 + (lane >> 2);
-      const bool seen0 = p0 < comp.len, seen1 = p0 + 8 < comp.len;
-      uint32_t pf[NT][2];
+        for (int kk = 0; kk < kK; ++kk) {
+          uint32_t k4[4];
+          ldsm4(k4, kbase + (u * 16 + key_k) * (HD * 2) +
+                        (((2 * kk + chunk_k) ^ (key_k & 7)) << 4));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816(sc[u][n], k4, qf[n][kk][0], qf[n][kk][1]);
+        }
+      const uint32_t p0 = (uint32_t)comp.tile * kTileKeys + warp * kRowsStep + (lane >> 2);
+      uint32_t pf[kSteps][NT][2];
       bool moved = false;
       float f[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          sc[n][e] = seen0 ? sc[n][e] * a.scale_log2 : -INFINITY;
-          sc[n][e + 2] = seen1 ? sc[n][e + 2] * a.scale_log2 : -INFINITY;
-          float x = fmaxf(sc[n][e], sc[n][e + 2]);
+          float x = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < kSteps; ++u) {
+            float& s0 = sc[u][n][e];
+            float& s1 = sc[u][n][e + 2];
+            s0 = p0 + u * 16 < comp.len ? s0 * a.scale_log2 : -INFINITY;
+            s1 = p0 + u * 16 + 8 < comp.len ? s1 * a.scale_log2 : -INFINITY;
+            x = fmaxf(x, fmaxf(s0, s1));
+          }
 #pragma unroll
           for (int sh = 4; sh < 32; sh <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, sh));
           const float top = fmaxf(m[n][e], x);
@@ -626,18 +646,25 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
           moved |= top > m[n][e];
           m[n][e] = top;
           const float z = top == -INFINITY ? 0.f : top;
-          sc[n][e] = exp2_fast(sc[n][e] - z);
-          sc[n][e + 2] = exp2_fast(sc[n][e + 2] - z);
+#pragma unroll
+          for (int u = 0; u < kSteps; ++u) {
+            sc[u][n][e] = exp2_fast(sc[u][n][e] - z);
+            sc[u][n][e + 2] = exp2_fast(sc[u][n][e + 2] - z);
+          }
+          l[n][e] *= f[n][e];
         }
-        // weights rounded to FP16 for the product; the sum takes the rounded
-        // ones, so a row of equal values keeps its value
-        const __half2 h0 = __floats2half2_rn(sc[n][0], sc[n][1]);
-        const __half2 h1 = __floats2half2_rn(sc[n][2], sc[n][3]);
-        const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
-        l[n][0] = l[n][0] * f[n][0] + (g0.x + g1.x);
-        l[n][1] = l[n][1] * f[n][1] + (g0.y + g1.y);
-        pf[n][0] = transpose8(*reinterpret_cast<const uint32_t*>(&h0));
-        pf[n][1] = transpose8(*reinterpret_cast<const uint32_t*>(&h1));
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) {
+          // weights rounded to FP16 for the product; the sum takes the rounded
+          // ones, so a row of equal values keeps its value
+          const __half2 h0 = __floats2half2_rn(sc[u][n][0], sc[u][n][1]);
+          const __half2 h1 = __floats2half2_rn(sc[u][n][2], sc[u][n][3]);
+          const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
+          l[n][0] += g0.x + g1.x;
+          l[n][1] += g0.y + g1.y;
+          pf[u][n][0] = transpose8(*reinterpret_cast<const uint32_t*>(&h0));
+          pf[u][n][1] = transpose8(*reinterpret_cast<const uint32_t*>(&h1));
+        }
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -651,12 +678,15 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
           }
       }
 #pragma unroll
-      for (int kk = 0; kk < kK; ++kk) {
-        uint32_t v4[4];
-        ldsm4_trans(v4, vbase + key_v * (HD * 2) + (((2 * kk + chunk_v) ^ (key_v & 7)) << 4));
+      for (int u = 0; u < kSteps; ++u)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816(o[kk][n], v4, pf[n][0], pf[n][1]);
-      }
+        for (int kk = 0; kk < kK; ++kk) {
+          uint32_t v4[4];
+          ldsm4_trans(v4, vbase + (u * 16 + key_v) * (HD * 2) +
+                              (((2 * kk + chunk_v) ^ (key_v & 7)) << 4));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816(o[kk][n], v4, pf[u][n][0], pf[u][n][1]);
+        }
       __syncwarp();
 
       const bool unit_done = comp.tile + 1 == comp.tiles;
@@ -791,7 +821,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a) {
   }
 }
 
-constexpr int kCtasMax = 4;
+constexpr int kCtasMax = 2;
 
 template <int HD, int NT, bool kRuns>
 void launch_paged(const Launch& l, const PagedArgs& a) {
@@ -853,6 +883,9 @@ void paged_attention(const Launch& l, const PagedAttention& p, void* workspace) 
   a.table_width = p.table_width;
   a.page = p.page;
   a.group = p.qh / p.kvh;
+  a.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (p.page == 1 << i) a.page_shift = i;
   a.pages = p.pages;
   a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)p.hd));
   if (p.hd == 128)

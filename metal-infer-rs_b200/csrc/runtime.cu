@@ -116,8 +116,15 @@ mi_tensor* view(const mi_tensor* t, const std::vector<size_t>& shape, size_t ext
 void* context_scratch(mi_context* ctx, size_t bytes) {
   if (bytes > ctx->scratch_bytes) {
     if (ctx->scratch) MI_CUDA(cudaFreeAsync(ctx->scratch, ctx->stream));
+    ctx->scratch = nullptr;
+    ctx->scratch_bytes = 0;
     size_t alloc = std::max<size_t>(bytes, 1 << 20);
-    MI_CUDA(cudaMallocAsync(&ctx->scratch, alloc, ctx->stream));
+    cudaError_t err = cudaMallocAsync(&ctx->scratch, alloc, ctx->stream);
+    if (err != cudaSuccess) {
+      ctx->scratch = nullptr;
+      fail(MI_ERR_RESOURCE, "device allocation of %zu bytes failed: %s", alloc,
+           cudaGetErrorString(err));
+    }
     ctx->scratch_bytes = alloc;
   }
   return ctx->scratch;
