@@ -22,9 +22,10 @@
 // keys of its own over the cluster's histograms (blocks of 64 keys by turns,
 // as a row's values share a few exponents). Measured, 96 rows of 151,936: 115
 // us with 4 CTAs to a row, 120 with every CTA reading the whole row for its
-// own keys, 45 so; one row 15 to 19 us. Of the 65,000 to 70,000 clocks of a
-// row's only CTA the additions take 37,000 (4,750 warp-wide ones on 32 banks),
-// the weights 11,000 and the search for the token's index 7,000.
+// own keys, 45 so; one row 15 to 19 us. Of the 62,000 to 68,000 clocks of a
+// row's only CTA the additions take 34,000 (4,750 warp-wide ones of 7 clocks:
+// 32 places in 32 banks meet three to four deep), the weights 11,000 and the
+// search for the token's index 6,500.
 
 #include <cooperative_groups.h>
 
@@ -355,12 +356,32 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
             if (lane == 0) add(d & 0xffffu, 256);
             continue;
           }
+          uint32_t d[4], most = 0;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t d = keys_of(u[e]);
-            least = __viaddmin_u16x2(d, 0xFC00FC00u, least);
-            add(d & 0xffffu, 1);
-            add(d >> 16, 1);
+            d[e] = keys_of(u[e]);
+            least = __viaddmin_u16x2(d[e], 0xFC00FC00u, least);
+            most = __viaddmax_u16x2(d[e], 0xFC00FC00u, most);
+          }
+          // less kFirst, keys of infinities and NaN are the ones from kEnd - kFirst on
+          const bool finite =
+              most < (kEnd - kFirst) << 16 && (most & 0xffffu) < kEnd - kFirst;
+          if (__all_sync(0xffffffffu, finite)) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              // word d / 2, and 1 or 2^16: 1 turned by 16 (d mod 2) bits
+              char* const hist = reinterpret_cast<char*>(sh.hist);
+              atomicAdd(reinterpret_cast<uint32_t*>(hist + ((d[e] << 1) & 0x1FFFCu)),
+                        __funnelshift_l(1u, 1u, d[e] << 4));
+              atomicAdd(reinterpret_cast<uint32_t*>(hist + ((d[e] >> 15) & 0x1FFFCu)),
+                        __funnelshift_l(1u, 1u, (d[e] >> 12) & 16u));
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              add(d[e] & 0xffffu, 1);
+              add(d[e] >> 16, 1);
+            }
           }
         }
       }
@@ -374,6 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
               const uint32_t n = (c >> (16 * h)) & 0xffffu;
               if (n > kLarge) {
                 const uint32_t at = atomicAdd(&sh.large, 1u);
+                if (at >= kLargeMax) continue;  // more counts than the row has: cannot be
                 sh.large_key[at] = 2 * i + h;
                 sh.large_count[at] = n;
                 reinterpret_cast<uint16_t*>(sh.hist)[2 * i + h] = 0;
@@ -421,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
       }
       if (large)
         for (int r = 0; r < kCtas; ++r) {
-          const uint32_t n = *of_rank<kCtas>(&sh.large, r);
+          const uint32_t n = min(*of_rank<kCtas>(&sh.large, r), (uint32_t)kLargeMax);
           for (uint32_t i = 0; i < n; ++i) {
             const uint32_t k = of_rank<kCtas>(sh.large_key, r)[i] - k0;
 #pragma unroll
