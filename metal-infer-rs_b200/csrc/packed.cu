@@ -65,6 +65,7 @@ struct PackedArgs {
   int span;         // tokens of a row tile
   float scale_log2; // log2(e) / sqrt(HD)
   const struct Plan* plan;
+  float* parts;     // states of the parts of split work
 };
 
 template <int HD>
@@ -301,7 +302,7 @@ struct alignas(16) Work {
   int k0, keys;    // its first key row, its keys
   int token;       // first token (of the sequence) of row tile 0, -1: nothing
   int blocks[2];   // key tiles that row tile 0 / 1 sees
-  int pad;
+  int part;        // where a part's state goes, -1: the work is whole
 };
 static_assert(sizeof(Work) == 32, "two 16-byte words");
 
@@ -323,7 +324,7 @@ __device__ __forceinline__ long long first_place(const PackedArgs& a, uint32_t s
 // The row tiles from token t on of a sequence.
 __device__ __forceinline__ Work work_of(const PackedArgs& a, int key_tile, const Starts& st,
                                         long long t) {
-  Work w{(int)st.q0, (int)st.q1, (int)st.k0, (int)(st.k1 - st.k0), -1, {0, 0}, 0};
+  Work w{(int)st.q0, (int)st.q1, (int)st.k0, (int)(st.k1 - st.k0), -1, {0, 0}, -1};
   const int n = w.q1 - w.q0;
   w.token = t < n ? (int)t : -1;
 #pragma unroll
@@ -340,11 +341,32 @@ __device__ __forceinline__ Work work_of(const PackedArgs& a, int key_tile, const
 // by key tiles): the CTAs that start last are then the shortest. Without it the
 // longest prompt's tiles may come last: 10 prompts of 20 to 2500 tokens took
 // 100 us, 96 so, the plan's launch included. The order among equals depends on timing, the results do not.
-struct Plan {
-  uint32_t count;
-  uint32_t pad[7];
-  Work work[1];
+struct alignas(16) Join {
+  Work w;          // the whole work
+  int part, parts; // its parts' states
+  int pad[2];
 };
+struct Plan {
+  uint32_t count, joins;
+  uint32_t pad[6];
+  Work work[1];
+  __host__ __device__ Join* join(int works) { return reinterpret_cast<Join*>(work + works); }
+  __host__ __device__ const Join* join(int works) const {
+    return reinterpret_cast<const Join*>(work + works);
+  }
+};
+__device__ __forceinline__ Work work_at_place(const PackedArgs& a, int key_tile, int place) {
+  int lo = 0, hi = a.sequences;  // the last sequence that begins at or before it
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (first_place(a, a.query_starts[mid], mid) <= place) lo = mid + 1;
+    else hi = mid;
+  }
+  if (lo == 0) return Work{0, 0, 0, 0, -1, {0, 0}, -1};
+  const Starts st(a, lo - 1);
+  return work_of(a, key_tile, st, (place - first_place(a, st.q0, lo - 1)) * 2 * a.span);
+}
+
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanBins = 2048;  // longer ones share the last
 
@@ -365,17 +387,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedA
     }
     return;
   }
-  auto work_at = [&](int place) {
-    int lo = 0, hi = a.sequences;  // the last sequence that begins at or before it
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (first_place(a, a.query_starts[mid], mid) <= place) lo = mid + 1;
-      else hi = mid;
-    }
-    if (lo == 0) return Work{0, 0, 0, 0, -1, {0, 0}, 0};
-    const Starts st(a, lo - 1);
-    return work_of(a, key_tile, st, (place - first_place(a, st.q0, lo - 1)) * 2 * a.span);
-  };
+  auto work_at = [&](int place) { return work_at_place(a, key_tile, place); };
   auto bin_of = [&](const Work& w) {  // longest first
     return kPlanBins - 1 - min(kPlanBins - 1, max(w.blocks[0], w.blocks[1]));
   };
@@ -410,8 +422,149 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedA
 }
 static_assert(kPlanBins == 2 * kPlanThreads, "two bins to a thread");
 
-// kPlanned: the work comes in the plan's order, else each CTA looks for its place.
-template <int HD, bool kPlanned>
+// ---- work split along its keys ------------------------------------------------------
+// Few queries over many keys are a few row tiles with very much each: their
+// keys are then cut into parts of about equal work for all SMs (a part is work
+// like any other over keys of its own), which leave their rows' maxima, sums
+// and unnormalised outputs, and a last kernel joins them in order. 64 queries
+// of 32/8 heads over 65,536 keys take 855 us in one piece, 103 so.
+constexpr int kPartLeast = 8;  // key tiles of a part at least
+
+__global__ void __launch_bounds__(kPlanThreads) packed_split_kernel(const PackedArgs a, Plan* plan,
+                                                                    int places, int works,
+                                                                    int key_tile, int columns,
+                                                                    int sm_count) {
+  __shared__ unsigned long long total;
+  __shared__ uint32_t count, states, joins;
+  const int tid = threadIdx.x;
+  if (tid == 0) {
+    total = 0;
+    count = states = joins = 0;
+  }
+  pdl_wait();
+  pdl_trigger();
+  bool bad = false;
+  for (int s = tid; s < a.sequences; s += kPlanThreads) bad |= Starts(a, s).bad(a);
+  if (__syncthreads_or(bad)) {
+    if (tid == 0) {
+      report_fault(a.fault, kFaultStarts);
+      plan->count = plan->joins = 0;
+    }
+    return;
+  }
+  for (int i = tid; i < places; i += kPlanThreads) {
+    const Work w = work_at_place(a, key_tile, i);
+    if (w.token >= 0) atomicAdd(&total, (unsigned long long)max(w.blocks[0], w.blocks[1]));
+  }
+  __syncthreads();
+  const unsigned long long even = (total * columns + sm_count - 1) / sm_count;
+  const int most = (int)max(even, (unsigned long long)kPartLeast);
+  for (int i = tid; i < places; i += kPlanThreads) {
+    Work w = work_at_place(a, key_tile, i);
+    if (w.token < 0) continue;
+    const int blocks = max(w.blocks[0], w.blocks[1]);
+    int parts = max(1, (blocks + most - 1) / most);
+    const int per = (blocks + parts - 1) / parts;
+    if (blocks > 0) parts = (blocks + per - 1) / per;
+    const uint32_t at = atomicAdd(&count, (uint32_t)parts);
+    if (at + parts > (uint32_t)works) continue;  // more than there is work for: cannot be
+    if (parts == 1) {
+      plan->work[at] = w;
+      continue;
+    }
+    const int state = (int)atomicAdd(&states, (uint32_t)parts);
+    plan->join(works)[atomicAdd(&joins, 1u)] = Join{w, state, parts, {0, 0}};
+    for (int q = 0; q < parts; ++q) {
+      Work v = w;
+      v.k0 += q * per * key_tile;
+      v.keys -= q * per * key_tile;
+      for (int t = 0; t < 2; ++t)
+        v.blocks[t] = max(0, min(w.blocks[t], (q + 1) * per) - q * per);
+      v.part = state + q;
+      plan->work[at + q] = v;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    plan->count = min(count, (uint32_t)works);
+    plan->joins = joins;
+  }
+}
+
+// Floats of a part's state: (maximum, sum) and output of 2 x 128 rows.
+constexpr size_t part_floats(int hd) { return 2 * kTile * (2 + (size_t)hd); }
+
+// What a row is: token and head of the group, keys that it sees.
+struct RowOf {
+  int token, head, visible;
+  bool valid;
+  __device__ RowOf(const PackedArgs& a, const Work& w, int head0, int t, int row) {
+    const int n = w.q1 - w.q0;
+    token = w.token + t * a.span + row / a.heads;
+    head = head0 + row % a.heads;
+    valid = row < a.heads * a.span && token < n && head < a.group;
+    const long long seen = a.causal ? (long long)w.keys - (n - 1 - token) : w.keys;
+    visible = valid && seen > 0 ? (int)seen : 0;
+  }
+};
+
+// A row to a warp.
+template <int HD>
+__global__ void __launch_bounds__(256) packed_join_kernel(const PackedArgs a, int works) {
+  constexpr int kV = HD / 32;
+  pdl_wait();
+  pdl_trigger();
+  const int columns = a.kvh * a.head_tiles;
+  const int index = (int)(blockIdx.x / (uint32_t)columns);
+  if (index >= (int)a.plan->joins) return;
+  const Join j = a.plan->join(works)[index];
+  const int column = (int)(blockIdx.x % (uint32_t)columns);
+  const int lane = threadIdx.x & 31;
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int t = r / kTile, row = r % kTile;
+  const int kv = column / a.head_tiles;
+  const RowOf me(a, j.w, column % a.head_tiles * a.heads, t, row);
+  if (!me.valid) return;
+  const size_t at =
+      ((size_t)(j.w.q0 + me.token) * a.qh + (size_t)kv * a.group + me.head) * HD;
+  auto state = [&](int q) {
+    return a.parts + ((size_t)(j.part + q) * columns + column) * part_floats(HD);
+  };
+  float top = -INFINITY;
+  for (int q = lane; q < j.parts; q += 32) top = fmaxf(top, state(q)[2 * r]);
+  top = warp_max(top);
+  float acc[kV] = {}, total = 0.f;
+#pragma unroll 4
+  for (int q = 0; q < j.parts; ++q) {
+    const float* s = state(q);
+    const float2 ml = *reinterpret_cast<const float2*>(s + 2 * r);
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // sees nothing of this part
+    const float w = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top);
+    total += w * ml.y;
+    const float* o = s + 4 * kTile + (size_t)r * HD + lane * kV;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) acc[e] += w * o[e];
+  }
+  bool odd = false;
+  const float inv = 1.f / total;
+#pragma unroll
+  for (int e = 0; e < kV; ++e) {
+    acc[e] = me.visible > 0 ? acc[e] * inv : 0.f;
+    odd |= !(acc[e] * 0.f == 0.f);
+    a.out[at + lane * kV + e] = __float2half_rn(acc[e]);
+  }
+  if (__any_sync(0xffffffffu, odd) && me.visible > 0) {
+    const size_t stride = (size_t)a.kvh * HD;
+    attention_row<HD>(a.q + at, a.k + (size_t)j.w.k0 * stride + kv * HD,
+                      a.v + (size_t)j.w.k0 * stride + kv * HD, stride, me.visible, a.scale_log2,
+                      a.out + at);
+  }
+}
+
+// How a CTA comes by its work: it looks for its place, it is in the plan's
+// order, or it is in a plan that splits it.
+enum Mode { kOwnPlace, kPlanned, kSplit };
+template <int HD, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1)
     packed_kernel(const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ CUtensorMap map_k,
@@ -468,14 +621,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if constexpr (!kPlanned) __syncthreads();
+  if constexpr (kMode == kOwnPlace) __syncthreads();
   pdl_wait();
   pdl_trigger();
 
   // ---- which tokens ------------------------------------------------------------
   Work w;
   bool bad = false;
-  if constexpr (kPlanned) {
+  if constexpr (kMode != kOwnPlace) {
     w.token = -1;
     if (place_y < (int)a.plan->count) {
       const uint4* src = reinterpret_cast<const uint4*>(&a.plan->work[place_y]);
@@ -497,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   bad = __syncthreads_or(bad);
   fence_after();
-  if constexpr (!kPlanned) w = *work;
+  if constexpr (kMode == kOwnPlace) w = *work;
   if (bad || w.token < 0) {  // starts that do not rise or leave their rows, or nothing to do
     if (bad && tid == 0) report_fault(a.fault, kFaultStarts);
     if (warp == 8)
@@ -602,11 +755,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tp = ts + C::kP;
     const uint32_t to = tmem + lanes + C::kO + t * HD;
     const int n = w.q1 - w.q0;
-    const int token = w.token + t * a.span + row / a.heads;
-    const int head = head0 + row % a.heads;
-    const bool valid = row < a.heads * a.span && token < n && head < a.group;
-    const long long seen = a.causal ? (long long)w.keys - (n - 1 - token) : w.keys;
-    const int visible = valid && seen > 0 ? (int)seen : 0;
+    const RowOf me(a, w, head0, t, row);
+    const int token = me.token, head = me.head, visible = me.visible;
+    const bool valid = me.valid;
     // keys that every row of the tile sees
     const long long least =
         a.causal ? (long long)w.keys - (n - 1 - (w.token + t * a.span)) : w.keys;
@@ -711,62 +862,87 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_after();
       float la, lb;
       split(l2, la, lb);
-      const float inv = 1.f / (la + lb);
-      uint64_t odd2 = 0;  // stays 0 while all is finite: a sum of 0 * value
-      const uint64_t inv2 = pair_of(inv, inv);
-      // The rows go through this tile's query tile in shared memory, which its
-      // products have read, so that they leave as whole lines: a row to a
-      // thread touches a line with every 16 bytes (5,100 clocks to a CTA, 2,900 so).
-      uint8_t* stage = smem + t * C::kQBytes + (warp & 3) * 32 * (HD * 2);
-      constexpr int kChunks = HD / 8;
+      if (kMode == kSplit && w.part >= 0) {
+        float* state = a.parts + ((size_t)w.part * columns + blockIdx.x % (uint32_t)columns) *
+                                     part_floats(HD);
+        const int r = t * kTile + row;
+        if (valid) *reinterpret_cast<float2*>(state + 2 * r) = make_float2(m, la + lb);
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o, to + c);
+          tmem_wait_ld();
+          tie32(o);
+          float4* dst = reinterpret_cast<float4*>(state + 4 * kTile + (size_t)r * HD + c);
 #pragma unroll
-      for (int c = 0; c < HD; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(o, to + c);
-        tmem_wait_ld();
-        tie32(o);
+          for (int q = 0; q < 8; ++q)
+            if (valid)
+              dst[q] = make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]),
+                                   __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3]));
+        }
+      } else {
+        const float inv = 1.f / (la + lb);
+        uint64_t odd2 = 0;  // stays 0 while all is finite: a sum of 0 * value
+        const uint64_t inv2 = pair_of(inv, inv);
+        // The rows go through this tile's query tile in shared memory, which its
+        // products have read, so that they leave as whole lines: a row to a
+        // thread touches a line with every 16 bytes (5,100 clocks to a CTA, 2,900 so).
+        uint8_t* stage = smem + t * C::kQBytes + (warp & 3) * 32 * (HD * 2);
+        constexpr int kChunks = HD / 8;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint4 v;
-          __half2* hv = reinterpret_cast<__half2*>(&v);
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o, to + c);
+          tmem_wait_ld();
+          tie32(o);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint64_t z = mul2(pair_of(__uint_as_float(o[q * 8 + 2 * e]),
-                                            __uint_as_float(o[q * 8 + 2 * e + 1])),
-                                    inv2);
-            odd2 = fma2(z, 0, odd2);
-            float x, y;
-            split(z, x, y);
-            hv[e] = __floats2half2_rn(x, y);
+          for (int q = 0; q < 4; ++q) {
+            uint4 v;
+            __half2* hv = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint64_t z = mul2(pair_of(__uint_as_float(o[q * 8 + 2 * e]),
+                                              __uint_as_float(o[q * 8 + 2 * e + 1])),
+                                      inv2);
+              odd2 = fma2(z, 0, odd2);
+              float x, y;
+              split(z, x, y);
+              hv[e] = __floats2half2_rn(x, y);
+            }
+            if (visible == 0) v = make_uint4(0, 0, 0, 0);
+            const int chunk = c / 8 + q;
+            *reinterpret_cast<uint4*>(stage + lane * (HD * 2) + ((chunk ^ (lane & 7)) << 4)) = v;
           }
-          if (visible == 0) v = make_uint4(0, 0, 0, 0);
-          const int chunk = c / 8 + q;
-          *reinterpret_cast<uint4*>(stage + lane * (HD * 2) + ((chunk ^ (lane & 7)) << 4)) = v;
+        }
+        __syncwarp();
+        const unsigned long long mine_at = valid ? (unsigned long long)at : ~0ull;
+#pragma unroll 4
+        for (int r = lane / kChunks; r < 32; r += 32 / kChunks) {
+          const unsigned long long to_row = __shfl_sync(0xffffffffu, mine_at, r);
+          const int chunk = lane % kChunks;
+          if (to_row != ~0ull)
+            reinterpret_cast<uint4*>(a.out + to_row)[chunk] = *reinterpret_cast<const uint4*>(
+                stage + r * (HD * 2) + ((chunk ^ (r & 7)) << 4));
+        }
+        __syncwarp();
+        float odd0, odd1;
+        split(odd2, odd0, odd1);
+        unsigned again = __ballot_sync(0xffffffffu, !(odd0 + odd1 == 0.f) && visible > 0);
+        while (again) {
+          const int who = __ffs(again) - 1;
+          again &= again - 1;
+          const int seen_w = __shfl_sync(0xffffffffu, visible, who);
+          const unsigned long long at_w = __shfl_sync(0xffffffffu, (unsigned long long)at, who);
+          attention_row<HD>(a.q + at_w, a.k + (size_t)w.k0 * stride + kv * HD,
+                            a.v + (size_t)w.k0 * stride + kv * HD, stride, seen_w, a.scale_log2,
+                            a.out + at_w);
         }
       }
-      __syncwarp();
-      const unsigned long long mine_at = valid ? (unsigned long long)at : ~0ull;
-#pragma unroll 4
-      for (int r = lane / kChunks; r < 32; r += 32 / kChunks) {
-        const unsigned long long to_row = __shfl_sync(0xffffffffu, mine_at, r);
-        const int chunk = lane % kChunks;
-        if (to_row != ~0ull)
-          reinterpret_cast<uint4*>(a.out + to_row)[chunk] = *reinterpret_cast<const uint4*>(
-              stage + r * (HD * 2) + ((chunk ^ (r & 7)) << 4));
-      }
-      __syncwarp();
-      float odd0, odd1;
-      split(odd2, odd0, odd1);
-      unsigned again = __ballot_sync(0xffffffffu, !(odd0 + odd1 == 0.f) && visible > 0);
-      while (again) {
-        const int who = __ffs(again) - 1;
-        again &= again - 1;
-        const int seen_w = __shfl_sync(0xffffffffu, visible, who);
-        const unsigned long long at_w = __shfl_sync(0xffffffffu, (unsigned long long)at, who);
-        attention_row<HD>(a.q + at_w, a.k + (size_t)w.k0 * stride + kv * HD,
-                          a.v + (size_t)w.k0 * stride + kv * HD, stride, seen_w, a.scale_log2,
-                          a.out + at_w);
-      }
+    } else if (kMode == kSplit && mine == 0 && w.part >= 0) {
+      float* state = a.parts + ((size_t)w.part * columns + blockIdx.x % (uint32_t)columns) *
+                                   part_floats(HD);
+      if (valid)
+        *reinterpret_cast<float2*>(state + 2 * (t * kTile + row)) = make_float2(-INFINITY, 0.f);
     } else if (mine == 0 && valid) {
       for (int c = 0; c < HD / 8; ++c)
         reinterpret_cast<uint4*>(a.out + at)[c] = make_uint4(0, 0, 0, 0);
@@ -782,11 +958,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Keys of a sequence, times the share of SMs without work, from which a split
+// pays (32/8 heads of 128, in one piece and split: 64 queries over 2,048 keys 34
+// and 27 us, over 65,536 855 and 103; 512 over 2,048 35 and 53; 900 over 8,192
+// 120 and 146).
+constexpr int kSplitKeys = 1800;
+
 // Heads of a row tile, its tokens, and the places of a call's row tile pairs.
 struct Shape {
   int head_tiles, heads, span;
   long long places;
-  bool planned;
+  Mode mode;
+  int works;  // a split plan's most
 };
 Shape shape_of(const PackedAttention& p, int sm_count) {
   Shape s;
@@ -797,8 +980,22 @@ Shape shape_of(const PackedAttention& p, int sm_count) {
   s.places = (long long)p.tokens / (2 * s.span) + p.sequences;
   // One sequence's tiles are in order as they are, and so is what fits the GPU
   // about at once: the plan is a launch of some 4 us.
-  s.planned = p.sequences > 1 && s.places * p.kvh * s.head_tiles > 2 * sm_count;
+  const long long items = s.places * p.kvh * s.head_tiles;
+  s.mode = p.sequences > 1 && items > 2 * sm_count ? kPlanned : kOwnPlace;
+  // Less work than SMs, and keys enough that sharing them with the idle ones
+  // outweighs the split's two launches and its states.
+  if (items < sm_count && (long long)p.keys / p.sequences * (sm_count - items) / sm_count >=
+                              kSplitKeys)
+    s.mode = kSplit;
+  s.works = (int)std::min<long long>(s.places + sm_count / (p.kvh * s.head_tiles) + 1, 1 << 20);
   return s;
+}
+
+// Bytes of the plan, to a multiple of 16.
+size_t plan_bytes(const Shape& s) {
+  if (s.mode == kSplit)
+    return sizeof(Plan) + (size_t)s.works * sizeof(Work) + (size_t)s.places * sizeof(Join);
+  return sizeof(Plan) + (size_t)s.places * sizeof(Work);
 }
 
 template <int HD>
@@ -815,27 +1012,40 @@ void launch_packed(const Launch& l, PackedArgs a, const Shape& s, void* workspac
   if (!make_f16_map(&mq, a.q, 4, dq, bq) || !make_f16_map(&mk, a.k, 3, dk, bk) ||
       !make_f16_map(&mv, a.v, 3, dk, bk))
     fail(MI_ERR_KERNEL, "packed attention: tensor map encoding failed");
-  auto kernel = s.planned ? packed_kernel<HD, true> : packed_kernel<HD, false>;
+  auto kernel = s.mode == kSplit     ? packed_kernel<HD, kSplit>
+                : s.mode == kPlanned ? packed_kernel<HD, kPlanned>
+                                     : packed_kernel<HD, kOwnPlace>;
   allow_dynamic_smem(kernel, C::kBytes);
-  const long long grid = s.places * a.kvh * a.head_tiles;
+  const int columns = a.kvh * a.head_tiles;
+  const long long grid = (s.mode == kSplit ? s.works : s.places) * (long long)columns;
   if (grid > 0x7FFFFFFF)
     fail(MI_ERR_SHAPE, "invalid tensor shape: %d tokens of %d sequences are too many for one call",
          a.tokens, a.sequences);
-  if (s.planned) {
-    Plan* plan = static_cast<Plan*>(workspace);
+  Plan* plan = static_cast<Plan*>(workspace);
+  a.plan = plan;
+  if (s.mode == kPlanned)
     launch_kernel(l, dim3(1), dim3(kPlanThreads), 0, packed_plan_kernel, a, plan, (int)s.places,
                   C::kKeys);
-    a.plan = plan;
+  if (s.mode == kSplit) {
+    a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan_bytes(s));
+    launch_kernel(l, dim3(1), dim3(kPlanThreads), 0, packed_split_kernel, a, plan, (int)s.places,
+                  s.works, C::kKeys, columns, l.sm_count);
   }
-  launch_kernel(l, dim3((unsigned)grid), dim3(kThreads), C::kBytes,
-                kernel, mq, mk, mv, a);
+  launch_kernel(l, dim3((unsigned)grid), dim3(kThreads), C::kBytes, kernel, mq, mk, mv, a);
+  if (s.mode == kSplit)
+    launch_kernel(l, dim3((unsigned)s.places * columns, 2 * kTile / 8), dim3(256), 0,
+                  packed_join_kernel<HD>, a, s.works);
 }
 
 }  // namespace
 
 size_t packed_attention_workspace(const PackedAttention& p, int sm_count) {
   const Shape s = shape_of(p, sm_count);
-  return s.planned ? sizeof(Plan) + (size_t)s.places * sizeof(Work) : 0;
+  if (s.mode == kOwnPlace) return 0;
+  size_t bytes = plan_bytes(s);
+  if (s.mode == kSplit)
+    bytes += (size_t)s.works * p.kvh * s.head_tiles * part_floats(p.hd) * sizeof(float);
+  return bytes;
 }
 
 void packed_attention(const Launch& l, const PackedAttention& p, void* workspace) {

@@ -268,6 +268,34 @@ def test_packed_attention_long(ctx, hd, qh, kvh, queries, prefix):
     np.testing.assert_array_equal(got.view(np.uint16), run_packed(ctx, q, k, v, qs, ks, True).view(np.uint16))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("hd,qh,kvh,queries,keys", [
+    (128, 8, 2, [7], [5000]), (64, 8, 2, [7], [5000]), (128, 4, 1, [1, 3], [9000, 100]),
+    (128, 6, 2, [40, 0, 5], [4100, 0, 2000]), (64, 7, 1, [90, 5], [40, 4500]), (128, 16, 8, [64], [2549])])
+def test_packed_attention_few_queries_over_many_keys(ctx, hd, qh, kvh, queries, keys, causal):
+    # work that is split along its keys and joined
+    rng = np.random.default_rng(17)
+    qs, ks = starts(queries), starts(keys)
+    q, k, v = normal(rng, qs[-1], qh, hd), normal(rng, ks[-1], kvh, hd), normal(rng, ks[-1], kvh, hd)
+    got = run_packed(ctx, q, k, v, qs, ks, causal)
+    check_packed(q, k, v, qs, ks, causal, got)
+    np.testing.assert_array_equal(got.view(np.uint16), run_packed(ctx, q, k, v, qs, ks, causal).view(np.uint16))
+
+
+@pytest.mark.parametrize("stale", [np.nan, np.inf])
+def test_packed_attention_split_ignores_masked_values(ctx, stale):
+    rng = np.random.default_rng(18)
+    qs, ks = starts([20, 6]), starts([3000, 40])
+    q, k, v = normal(rng, 26, 4, 128), normal(rng, 3300, 2, 128), normal(rng, 3300, 2, 128)
+    k[3040:], v[3040:] = stale, stale
+    v[2990:3000] = stale   # seen by the last ten queries of the first sequence alone
+    got = run_packed(ctx, q, k, v, qs, ks, True)
+    clean = np.where(np.isfinite(v), v, 0)
+    check_packed(q[:10], k, clean, [0, 10], [0, 2990], True, got[:10])
+    check_packed(q[20:], k[3000:3040], clean[3000:3040], [0, 6], [0, 40], True, got[20:])
+    assert not np.any(np.isfinite(got[10:20]))
+
+
 def test_packed_attention_large_scores(ctx):
     rng = np.random.default_rng(12)
     qs = ks = starts([150, 260])
