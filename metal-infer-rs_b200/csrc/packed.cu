@@ -340,7 +340,8 @@ __device__ __forceinline__ Work work_of(const PackedArgs& a, int key_tile, const
 // All sequences' row tiles, the ones that see most keys first (a counting sort
 // by key tiles): the CTAs that start last are then the shortest. Without it the
 // longest prompt's tiles may come last: 10 prompts of 20 to 2500 tokens took
-// 100 us, 96 so, the plan's launch included. The order among equals depends on timing, the results do not.
+// 100 us, 96 so, the plan's launch included. The order among equals depends on
+// timing, the results do not.
 struct alignas(16) Join {
   Work w;          // the whole work
   int part, parts; // its parts' states
@@ -866,7 +867,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         float* state = a.parts + ((size_t)w.part * columns + blockIdx.x % (uint32_t)columns) *
                                      part_floats(HD);
         const int r = t * kTile + row;
-        if (valid) *reinterpret_cast<float2*>(state + 2 * r) = make_float2(m, la + lb);
+        // a row that saw only scores of -inf is done again, as its values count
+        const float sum = m == -INFINITY && visible > 0 ? __int_as_float(0x7fc00000) : la + lb;
+        if (valid) *reinterpret_cast<float2*>(state + 2 * r) = make_float2(m, sum);
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           uint32_t o[32];

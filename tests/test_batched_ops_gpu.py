@@ -296,6 +296,22 @@ def test_packed_attention_split_ignores_masked_values(ctx, stale):
     assert not np.any(np.isfinite(got[10:20]))
 
 
+@pytest.mark.parametrize("hidden", [0.0, np.inf])
+def test_packed_attention_split_with_scores_of_minus_infinity(ctx, hidden):
+    # keys of weight 0 that the rows see: they leave the others' result alone
+    # where their values are finite, and 0 * inf is NaN, in any part
+    rng = np.random.default_rng(19)
+    q, k, v = normal(rng, 9, 2, 128), normal(rng, 4000, 1, 128), normal(rng, 4000, 1, 128)
+    q[:, :, 0] = 1
+    k[:2000, :, 0] = -np.inf
+    v[7] += hidden
+    got = run_packed(ctx, q, k, v, [0, 9], [0, 4000], True)
+    if hidden:
+        assert np.all(np.isnan(got))
+    else:
+        check_packed(q, k[2000:], v[2000:], [0, 9], [0, 2000], True, got)
+
+
 def test_packed_attention_large_scores(ctx):
     rng = np.random.default_rng(12)
     qs = ks = starts([150, 260])
