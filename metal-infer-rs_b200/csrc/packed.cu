@@ -14,8 +14,7 @@
 // A CTA takes two row tiles of one sequence and KV head. The rows of a tile
 // are the query heads of the group for up to 128 / group tokens, so a short
 // prompt still fills a tile and a key tile is read once for the whole group.
-// Roles (warp 11 only fills its warpgroup; registers go from the last warpgroup
-// to the softmax):
+// Roles (registers go from the last warpgroup to the softmax):
 //   warps 0-3, 4-7  softmax of row tile 0 / 1, one row to a thread: scores from
 //                   TMEM, the running maximum and sum in registers, FP16
 //                   weights to TMEM; in the end the output
@@ -25,6 +24,9 @@
 //                   each tile has an issuer, and K and V come under one barrier
 //   warp 10         TMA: the query tiles once, then a ring of stages, stage n
 //                   holding K tile n and V tile n - 1, which are used together
+//   warp 11         zeros over the rows behind a sequence's last value: what
+//                   stands there (other sequences, padding) has weight 0, and
+//                   0 * NaN would send the row to attention_row
 // TMEM holds S, P and O of both tiles with P beside S, so the next key tile's
 // scores are computed while the softmax of this one runs and the products
 // leave its chain: 80 keys to a tile at head_dim 128 (2 (80 + 40 + 128)
@@ -84,7 +86,8 @@ struct Packed {
 
 // One row by one warp, from the formula, over the first `visible` keys and
 // reading no others: rows whose products met infinities or NaN that they do
-// not see (0 * NaN in a tile's masked places) are computed again this way.
+// not see (0 * NaN among the keys behind a causal row) are computed again this
+// way.
 template <int HD>
 __device__ __noinline__ void attention_row(const __half* q, const __half* k, const __half* v,
                                            size_t stride, int visible, float scale_log2,
@@ -586,6 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* lead = bars + 9;       // tile 0 has its first maximum
   uint64_t* kv_full = bars + 10;   // [kStages]
   uint64_t* kv_empty = kv_full + kStages;
+  uint64_t* tail_full = bars + 20; // the last V tile, before its end is zero
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kStages);
   Work* work = reinterpret_cast<Work*>(bars + 24);
 
@@ -599,6 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     pipe::mbar_init(q_full, 1);
     pipe::mbar_init(lead, 4);
+    pipe::mbar_init(tail_full, 1);
     for (int i = 0; i < 2; ++i) {
       pipe::mbar_init(s_full + i, 1);
       pipe::mbar_init(s_free + i, 4);
@@ -662,10 +667,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int blocks = max(w.blocks[0], w.blocks[1]);
   const uint32_t tmem = *tmem_slot;
+  // rows of the CTA's last V tile that are its sequence's, 0: all
+  const int tail = blocks > 0 && blocks == (w.keys + kKeys - 1) / kKeys ? w.keys % kKeys : 0;
 
   if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 11) {
-    // no role
+    if (tail && warp_wait(tail_full, 0, a.fault)) {
+      const int st = blocks % kStages;
+      uint8_t* at = ring + (2 * st + 1) * C::kTileBytes + tail * 128;
+      for (int h = 0; h < kHalves; ++h)
+        for (int i = lane; i < (kKeys - tail) * 8; i += 32)
+          reinterpret_cast<uint4*>(at + h * (kKeys * 128))[i] = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive(kv_full + st);
+    }
   } else if (warp == 10) {
     if (lane == 0 && blocks > 0) {
       // ---- TMA ------------------------------------------------------------------
@@ -679,18 +695,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int st = n % kStages;
         if (!wait_for(kv_empty + st, ((n / kStages) & 1) ^ 1, a.fault)) break;
         uint8_t* at = ring + 2 * st * C::kTileBytes;
-        pipe::mbar_expect_tx(kv_full + st,
-                             ((n < blocks ? 1u : 0u) + (n > 0 ? 1u : 0u)) * C::kTileBytes);
+        // a V tile with an end is full when that is zero
+        uint64_t* full = n == blocks && tail ? tail_full : kv_full + st;
+        pipe::mbar_expect_tx(full, ((n < blocks ? 1u : 0u) + (n > 0 ? 1u : 0u)) * C::kTileBytes);
         for (int h = 0; h < kHalves; ++h) {
           if (n < blocks)
-            tma_3d(at + h * (kKeys * 128), &map_k, kv_full + st, h * 64, kv, w.k0 + n * kKeys);
+            tma_3d(at + h * (kKeys * 128), &map_k, full, h * 64, kv, w.k0 + n * kKeys);
           if (n > 0)
-            tma_3d(at + C::kTileBytes + h * (kKeys * 128), &map_v, kv_full + st, h * 64, kv,
+            tma_3d(at + C::kTileBytes + h * (kKeys * 128), &map_v, full, h * 64, kv,
                    w.k0 + (n - 1) * kKeys);
         }
       }
       // the copies land before the CTA leaves
       wait_for(q_full, 0, a.fault);
+      if (n > blocks && tail) wait_for(tail_full, 0, a.fault);
       for (int i = max(0, n - kStages); i < n; ++i)
         wait_for(kv_full + i % kStages, (i / kStages) & 1, a.fault);
     }
