@@ -427,24 +427,29 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedA
 static_assert(kPlanBins == 2 * kPlanThreads, "two bins to a thread");
 
 // ---- work split along its keys ------------------------------------------------------
-// Few queries over many keys are a few row tiles with very much each: their
-// keys are then cut into parts of about equal work for all SMs (a part is work
-// like any other over keys of its own), which leave their rows' maxima, sums
-// and unnormalised outputs, and a last kernel joins them in order. 64 queries
-// of 32/8 heads over 65,536 keys take 855 us in one piece, 103 so.
-constexpr int kPartLeast = 8;  // key tiles of a part at least
+// Few queries over many keys are a few row tiles with very much each, and a few
+// waves of row tiles over long prefixes leave most SMs without work in the last
+// wave. The work that does not fill a wave (the shortest) is cut along its keys
+// into as many parts as there are places left in that wave (a part is work like
+// any other over keys of its own), which leave their rows' maxima, sums and
+// unnormalised outputs, and a last kernel joins them in order. With 32/8 heads
+// of 128, 64 queries over 65,536 keys take 855 us in one piece and 88 so, 1,300
+// over 9,300 (1.1 waves) 224 and 170, 1,200 over 5,200 120 and 94.
+constexpr int kPartLeast = 8;       // key tiles of a part at least
+constexpr int kSplitPlaces = 512;  // of a call that is split, at most (each is ranked among all)
+constexpr int kSplitRest = 512;    // SMs and one, at most
 
 __global__ void __launch_bounds__(kPlanThreads) packed_split_kernel(const PackedArgs a, Plan* plan,
                                                                     int places, int works,
                                                                     int key_tile, int columns,
                                                                     int sm_count) {
-  __shared__ unsigned long long total;
+  // Never more works than `works`, nor parts than states: the parts have `room`.
+  __shared__ int length[kSplitPlaces];  // key tiles of a place's work, -1: none
+  __shared__ int rest[kSplitRest];      // of the works that are cut, from long to short
   __shared__ uint32_t count, states, joins;
-  const int tid = threadIdx.x;
-  if (tid == 0) {
-    total = 0;
-    count = states = joins = 0;
-  }
+  __shared__ int part_most;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) count = states = joins = 0;
   pdl_wait();
   pdl_trigger();
   bool bad = false;
@@ -456,29 +461,51 @@ __global__ void __launch_bounds__(kPlanThreads) packed_split_kernel(const Packed
     }
     return;
   }
-  for (int i = tid; i < places; i += kPlanThreads) {
-    const Work w = work_at_place(a, key_tile, i);
-    if (w.token >= 0) atomicAdd(&total, (unsigned long long)max(w.blocks[0], w.blocks[1]));
+  Work w;  // of place `tid`
+  w.token = -1;
+  if (tid < places) w = work_at_place(a, key_tile, tid);
+  const int mine = w.token < 0 ? -1 : max(w.blocks[0], w.blocks[1]);
+  if (tid < kSplitPlaces) length[tid] = mine;
+  const int n = __syncthreads_count(w.token >= 0);
+  // its place in the order from long to short
+  int order = 0;
+  if (tid < places)
+    for (int j = 0; j < places; ++j)
+      order += length[j] > mine || (length[j] == mine && j < tid);
+  // the works that fill whole waves, and the places of the wave behind them
+  const int waves = (int)((long long)n * columns / sm_count);
+  const int whole = (int)((long long)waves * sm_count / columns);
+  const int room = (int)(((long long)(waves + 1) * sm_count - (long long)whole * columns) / columns);
+  if (w.token >= 0 && order >= whole) rest[order - whole] = mine;
+  __syncthreads();
+  if (warp == 0) {  // the least length of a part at which all parts have room
+    const int many = n - whole;  // <= sm_count / columns + 1
+    auto parts_of = [&](int most) {
+      uint32_t parts = 0;
+      for (int i = lane; i < many; i += 32) parts += max(1, (rest[i] + most - 1) / most);
+      return (int)__reduce_add_sync(0xffffffffu, parts);
+    };
+    int lo = kPartLeast, hi = many > 0 ? max(kPartLeast, rest[0]) : kPartLeast;
+    while (lo < hi) {
+      const int most = (lo + hi) / 2;
+      if (parts_of(most) <= room) hi = most;
+      else lo = most + 1;
+    }
+    if (lane == 0) part_most = lo;
   }
   __syncthreads();
-  const unsigned long long even = (total * columns + sm_count - 1) / sm_count;
-  const int most = (int)max(even, (unsigned long long)kPartLeast);
-  for (int i = tid; i < places; i += kPlanThreads) {
-    Work w = work_at_place(a, key_tile, i);
-    if (w.token < 0) continue;
-    const int blocks = max(w.blocks[0], w.blocks[1]);
-    int parts = max(1, (blocks + most - 1) / most);
-    const int per = (blocks + parts - 1) / parts;
-    if (blocks > 0) parts = (blocks + per - 1) / per;
-    const uint32_t at = atomicAdd(&count, (uint32_t)parts);
-    if (at + parts > (uint32_t)works) continue;  // more than there is work for: cannot be
-    if (parts == 1) {
-      plan->work[at] = w;
-      continue;
-    }
-    const int state = (int)atomicAdd(&states, (uint32_t)parts);
-    plan->join(works)[atomicAdd(&joins, 1u)] = Join{w, state, parts, {0, 0}};
-    for (int q = 0; q < parts; ++q) {
+  const int most = part_most;
+  if (w.token >= 0 && order < whole) {
+    plan->work[order] = w;
+  } else if (w.token >= 0) {
+    int parts = max(1, (mine + most - 1) / most);
+    const int per = (mine + parts - 1) / parts;
+    if (mine > 0) parts = (mine + per - 1) / per;
+    const int at = whole + (int)atomicAdd(&count, (uint32_t)parts);
+    const int state = parts > 1 ? (int)atomicAdd(&states, (uint32_t)parts) : 0;
+    if (parts == 1) plan->work[at] = w;
+    else plan->join(works)[atomicAdd(&joins, 1u)] = Join{w, state, parts, {0, 0}};
+    for (int q = 0; parts > 1 && q < parts; ++q) {
       Work v = w;
       v.k0 += q * per * key_tile;
       v.keys -= q * per * key_tile;
@@ -490,10 +517,11 @@ __global__ void __launch_bounds__(kPlanThreads) packed_split_kernel(const Packed
   }
   __syncthreads();
   if (tid == 0) {
-    plan->count = min(count, (uint32_t)works);
+    plan->count = whole + count;
     plan->joins = joins;
   }
 }
+static_assert(kSplitPlaces <= kPlanThreads, "a place to a thread");
 
 // Floats of a part's state: (maximum, sum) and output of 2 x 128 rows.
 constexpr size_t part_floats(int hd) { return 2 * kTile * (2 + (size_t)hd); }
@@ -979,18 +1007,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Keys of a sequence, times the share of SMs without work, from which a split
-// pays (32/8 heads of 128, in one piece and split: 64 queries over 2,048 keys 34
-// and 27 us, over 65,536 855 and 103; 512 over 2,048 35 and 53; 900 over 8,192
-// 120 and 146).
+// From how many keys, saved on the longest way through a call, its split pays
+// for two launches, the parts' beginnings and their states, some 15 us in all
+// (32/8 heads of 128, in one piece and split: 64 queries over 2,048 keys 34 and
+// 28 us; 32 over 1,024 16 and 20; 512 over 2,048 35 and 40; 1,300 over 2,600 55
+// and 63).
 constexpr int kSplitKeys = 1800;
+constexpr int kSplitWaves = 8;  // the wave that is cut is a small part of more
 
 // Heads of a row tile, its tokens, and the places of a call's row tile pairs.
 struct Shape {
   int head_tiles, heads, span;
   long long places;
   Mode mode;
-  int works;  // a split plan's most
+  int works, states, joins;  // a split plan's most
 };
 Shape shape_of(const PackedAttention& p, int sm_count) {
   Shape s;
@@ -1001,21 +1031,33 @@ Shape shape_of(const PackedAttention& p, int sm_count) {
   s.places = (long long)p.tokens / (2 * s.span) + p.sequences;
   // One sequence's tiles are in order as they are, and so is what fits the GPU
   // about at once: the plan is a launch of some 4 us.
-  const long long items = s.places * p.kvh * s.head_tiles;
+  const long long columns = p.kvh * s.head_tiles;
+  const long long items = s.places * columns;
   s.mode = p.sequences > 1 && items > 2 * sm_count ? kPlanned : kOwnPlace;
-  // Less work than SMs, and keys enough that sharing them with the idle ones
-  // outweighs the split's two launches and its states.
-  if (items < sm_count && (long long)p.keys / p.sequences * (sm_count - items) / sm_count >=
-                              kSplitKeys)
+  // The lengths are not known here: a sequence is taken to fill half of its last
+  // place, and to see its share of the keys, less those that its own queries add
+  // one by one.
+  const long long likely =
+      std::max(1ll, p.sequences == 1 ? (p.tokens + 2ll * s.span - 1) / (2 * s.span)
+                                     : s.places - p.sequences / 2) * columns;
+  const long long waves = likely / sm_count;
+  const long long cut = likely - waves * sm_count;
+  const long long parts = cut > 0 ? sm_count / cut : 1;
+  long long seen = (long long)p.keys / p.sequences;
+  if (p.causal && waves > 0) seen -= p.tokens / p.sequences;
+  if (waves < kSplitWaves && s.places <= kSplitPlaces && sm_count < kSplitRest && parts > 1 &&
+      seen - seen / parts >= kSplitKeys)
     s.mode = kSplit;
-  s.works = (int)std::min<long long>(s.places + sm_count / (p.kvh * s.head_tiles) + 1, 1 << 20);
+  s.works = (int)std::min<long long>(s.places + sm_count / columns + 2, 1 << 20);
+  s.states = (int)(sm_count / columns + 2);
+  s.joins = (int)std::min<long long>(s.places, s.states / 2);
   return s;
 }
 
 // Bytes of the plan, to a multiple of 16.
 size_t plan_bytes(const Shape& s) {
   if (s.mode == kSplit)
-    return sizeof(Plan) + (size_t)s.works * sizeof(Work) + (size_t)s.places * sizeof(Join);
+    return sizeof(Plan) + (size_t)s.works * sizeof(Work) + (size_t)s.joins * sizeof(Join);
   return sizeof(Plan) + (size_t)s.places * sizeof(Work);
 }
 
@@ -1054,7 +1096,7 @@ void launch_packed(const Launch& l, PackedArgs a, const Shape& s, void* workspac
   }
   launch_kernel(l, dim3((unsigned)grid), dim3(kThreads), C::kBytes, kernel, mq, mk, mv, a);
   if (s.mode == kSplit)
-    launch_kernel(l, dim3((unsigned)s.places * columns, 2 * kTile / 8), dim3(256), 0,
+    launch_kernel(l, dim3((unsigned)s.joins * columns, 2 * kTile / 8), dim3(256), 0,
                   packed_join_kernel<HD>, a, s.works);
 }
 
@@ -1065,7 +1107,7 @@ size_t packed_attention_workspace(const PackedAttention& p, int sm_count) {
   if (s.mode == kOwnPlace) return 0;
   size_t bytes = plan_bytes(s);
   if (s.mode == kSplit)
-    bytes += (size_t)s.works * p.kvh * s.head_tiles * part_floats(p.hd) * sizeof(float);
+    bytes += (size_t)s.states * p.kvh * s.head_tiles * part_floats(p.hd) * sizeof(float);
   return bytes;
 }
 

@@ -282,6 +282,19 @@ def test_packed_attention_few_queries_over_many_keys(ctx, hd, qh, kvh, queries, 
     np.testing.assert_array_equal(got.view(np.uint16), run_packed(ctx, q, k, v, qs, ks, causal).view(np.uint16))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("hd,qh,kvh,queries,prefix", [
+    (64, 32, 4, [700, 500], 3000), (128, 24, 8, [1100, 1000], 4200), (128, 32, 4, [1210], 2700)])
+def test_packed_attention_waves_with_little_in_the_last(ctx, hd, qh, kvh, queries, prefix, causal):
+    # whole waves of work, and the rest split along its keys
+    rng = np.random.default_rng(20)
+    qs, ks = starts(queries), starts([n + prefix for n in queries])
+    q, k, v = normal(rng, qs[-1], qh, hd), normal(rng, ks[-1], kvh, hd), normal(rng, ks[-1], kvh, hd)
+    got = run_packed(ctx, q, k, v, qs, ks, causal)
+    check_packed(q, k, v, qs, ks, causal, got, heads=[0, qh - 1])
+    np.testing.assert_array_equal(got.view(np.uint16), run_packed(ctx, q, k, v, qs, ks, causal).view(np.uint16))
+
+
 @pytest.mark.parametrize("stale", [np.nan, np.inf])
 def test_packed_attention_split_ignores_masked_values(ctx, stale):
     rng = np.random.default_rng(18)
