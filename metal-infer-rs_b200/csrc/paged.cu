@@ -26,10 +26,10 @@ namespace {
 // values and the chunk that it rotates with: the first step of the canonical
 // sum of squares and the whole rotation stay inside a lane (with a chunk to a
 // lane and the partner fetched by shuffles, 5.7 K tokens of 32/8 heads took 55
-// us, 33 so). A block takes kTok tokens at a time and first fills a table of
+// us, 32 so). A block takes kTok tokens at a time and first fills a table of
 // their cosines and sines: the angles need double precision (numerics.cuh),
-// which a thread per (token, pair) pays once for all heads, and the
-// frequency's pow once for all of a block's tokens.
+// which a thread per (token, pair) pays once for all heads, and a thread per
+// pair the frequency's pow once for all of a block's tokens.
 constexpr int kAppendThreads = 256;
 
 struct AppendArgs {
@@ -83,14 +83,14 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
   constexpr int kRows = kAppendThreads / kLanes;
   constexpr int kPairs = HD / 2;
   __shared__ __align__(16) float cosines[kTok][kPairs], sines[kTok][kPairs];
+  __shared__ float frequencies[kPairs];
   __shared__ uint32_t position[kTok];
   __shared__ uint32_t slot[kTok];          // cache row of the token
   const int tid = threadIdx.x;
   const int li = tid % kLanes;
   const int pair0 = tid % kPairs;
-  float frequency = 0.f;
-  if (tid < kTok * kPairs)
-    frequency = (float)pow((double)a.theta, (double)__fdiv_rn(-(float)(pair0 * 2), (float)HD));
+  if (tid < kPairs)
+    frequencies[tid] = (float)pow((double)a.theta, (double)__fdiv_rn(-(float)(tid * 2), (float)HD));
   pdl_trigger();
   pdl_wait();
 
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
       const int t = j / kPairs;
       if (slot[t] != 0xFFFFFFFFu) {
         double s, c;
-        sincos((double)__fmul_rn((float)position[t], frequency), &s, &c);
+        sincos((double)__fmul_rn((float)position[t], frequencies[pair0]), &s, &c);
         cosines[t][pair0] = (float)c;
         sines[t][pair0] = (float)s;
       }
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 template <int HD>
 void launch_append(const Launch& l, const AppendArgs& a) {
   // Four tokens to a block share its barriers (one 42 us, two 33.9, four 32.7
-  // for 5.7 K tokens); few tokens take a block each, since latency is then all
+  // for 5.7 K tokens, before the pow was shared); few tokens take a block each, since latency is then all
   // there is.
   if (a.tokens <= 2 * l.sm_count) {
     launch_kernel(l, dim3(a.tokens), dim3(kAppendThreads), 0, paged_append_kernel<HD, 1>, a);
