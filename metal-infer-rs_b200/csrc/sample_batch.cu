@@ -387,22 +387,24 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
       }
       if (b < w1) {  // more to come: room in every count
         __syncthreads();
-        for (int i = tid; i < 65536 / 2; i += kThreads) {
-          const uint32_t c = sh.hist[i];
-          if ((c & 0xffffu) > kLarge || c >> 16 > kLarge) {
+        uint4* const words = reinterpret_cast<uint4*>(sh.hist);
+        uint32_t most = 0;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t n = (c >> (16 * h)) & 0xffffu;
-              if (n > kLarge) {
-                const uint32_t at = atomicAdd(&sh.large, 1u);
-                if (at >= kLargeMax) continue;  // more counts than the row has: cannot be
-                sh.large_key[at] = 2 * i + h;
-                sh.large_count[at] = n;
-                reinterpret_cast<uint16_t*>(sh.hist)[2 * i + h] = 0;
-              }
-            }
-          }
+        for (int i = tid; i < 65536 / 8; i += kThreads) {
+          const uint4 c = words[i];
+          most = __vmaxu2(most, __vmaxu2(__vmaxu2(c.x, c.y), __vmaxu2(c.z, c.w)));
         }
+        if ((most & 0xffffu) > kLarge || most >> 16 > kLarge)
+          for (int i = tid; i < 65536 / 8; i += kThreads)
+            for (int h = 0; h < 8; ++h) {
+              uint16_t& n = reinterpret_cast<uint16_t*>(words + i)[h];
+              if (n <= kLarge) continue;
+              const uint32_t at = atomicAdd(&sh.large, 1u);
+              if (at >= kLargeMax) continue;  // more counts than the row has: cannot be
+              sh.large_key[at] = 8 * i + h;
+              sh.large_count[at] = n;
+              n = 0;
+            }
         __syncthreads();
       }
     }
