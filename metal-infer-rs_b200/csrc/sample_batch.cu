@@ -15,17 +15,18 @@
 // neighbouring keys share an exponent, so their weights are one exponential
 // and powers of another.
 //
-// A CTA counts 16 bits to a key (128 KB of shared memory). The shared-memory
-// additions set the pace, so a row that shares the GPU with many others has
-// one CTA and nothing to add up between CTAs; where rows are fewer, a cluster
-// of 2, 4 or 8 CTAs takes a row: each counts its share of it, then adds up the
-// keys of its own over the cluster's histograms (blocks of 64 keys by turns,
-// as a row's values share a few exponents). Measured, 96 rows of 151,936: 115
-// us with 4 CTAs to a row, 120 with every CTA reading the whole row for its
-// own keys, 45 so; one row 15 to 19 us. Of the 62,000 to 68,000 clocks of a
-// row's only CTA the additions take 34,000 (4,750 warp-wide ones of 7 clocks:
-// 32 places in 32 banks meet three to four deep), the weights 11,000 and the
-// search for the token's index 6,500.
+// A CTA counts 16 bits to a key (128 KB of shared memory). Counting sets the
+// pace, so a row that shares the GPU with many others has one CTA and nothing
+// to add up between CTAs; where rows are fewer, a cluster of 2, 4 or 8 CTAs
+// takes a row: each counts its share of it, then adds up the keys of its own
+// over the cluster's histograms (blocks of 64 keys by turns, as a row's values
+// share a few exponents). Measured, 96 rows of 151,936: 115 us with 4 CTAs to a
+// row, 120 with every CTA reading the whole row for its own keys, 40 so; one
+// row 15 to 19 us. Of the some 60,000 clocks of a row's only CTA counting takes
+// 27,000 (21,000 without the additions: a key's word and half are ten integer
+// instructions to two values), the weights 10,000, their sums 5,000, the borders
+// of top_p and the crossing 5,000 each and the search for the token's index
+// 7,000.
 
 #include <cooperative_groups.h>
 
@@ -348,13 +349,15 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
         for (int k = 0; k < kMany; ++k) {
           const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
           // a stretch of one value (a mask) is one addition
-          const uint32_t one = __shfl_sync(0xffffffffu, u[0], 0);
-          const bool same = u[0] == one && u[1] == one && u[2] == one && u[3] == one;
-          if (__all_sync(0xffffffffu, same) && (one & 0xffffu) == one >> 16) {
-            const uint32_t d = keys_of(one);
-            least = __viaddmin_u16x2(d, 0xFC00FC00u, least);
-            if (lane == 0) add(d & 0xffffu, 256);
-            continue;
+          const bool same = ((u[0] ^ u[1]) | (u[2] ^ u[3]) | (u[0] ^ u[2])) == 0;
+          if (__all_sync(0xffffffffu, same)) {
+            const uint32_t one = __shfl_sync(0xffffffffu, u[0], 0);
+            if (__all_sync(0xffffffffu, u[0] == one) && (one & 0xffffu) == one >> 16) {
+              const uint32_t d = keys_of(one);
+              least = __viaddmin_u16x2(d, 0xFC00FC00u, least);
+              if (lane == 0) add(d & 0xffffu, 256);
+              continue;
+            }
           }
           uint32_t d[4], most = 0;
 #pragma unroll
@@ -718,26 +721,27 @@ __global__ void __launch_bounds__(kThreads, 1) sample_batch_kernel(const SampleB
     }
     for (int q = 0; q < warp; ++q) rest -= (int)sh.equals[q];
     if (rest >= 0 && rest < (int)equals) {
-      for (int i = a; i < b; i += 32) {
-        uint4 v[1];
+      for (int i = a; i < b; i += 4 * 32) {
+        uint4 v[4];
         x.load(v, i + lane, 32, b);
-        uint32_t mask = equal(v[0]);
-        int n = __popc(mask), upto = n;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += y;
-        }
-        const int all = __shfl_sync(0xffffffffu, upto, 31);
-        if (rest < all) {
+        for (int k = 0; k < 4; ++k) {
+          uint32_t mask = equal(v[k]);
+          int n = __popc(mask), upto = n;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+          }
+          const int all = __shfl_sync(0xffffffffu, upto, 31);
           int j = rest - (upto - n);  // of this lane's equals
           if (j >= 0 && j < n) {
             for (; j > 0; --j) mask &= mask - 1;
-            p.tokens[row] = 8 * (i + lane) + __ffs(mask) - 1 - x.from;
+            p.tokens[row] = 8 * (i + 32 * k + lane) + __ffs(mask) - 1 - x.from;
           }
-          break;
+          rest -= all;
         }
-        rest -= all;
+        if (rest < 0) break;
       }
     }
   }
@@ -774,8 +778,8 @@ void sample_batch(const Launch& l, const SampleBatch& p) {
   if (p.rows == 0) return;
   // As many CTAs to a row as fit the GPU at once, up to 8. Clusters of 8 and 4
   // leave SMs of a GPC empty, which the eighth below stands for (18 rows of
-  // 151,936: 28 us with 8, 25 with 4; 36: 34 with 4, 32 with 2; 75 and more:
-  // 45 with 1).
+  // 151,936: 28 us with 8, 25 with 4; 36: 34 with 4, 30 with 2; 75 and more:
+  // 39 with 1).
   const int sms = l.sm_count - l.sm_count / 8;
   if (p.rows * 8 <= sms)
     launch_sample<8>(l, p);
