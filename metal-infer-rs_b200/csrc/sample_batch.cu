@@ -23,10 +23,10 @@
 // share a few exponents). Measured, 96 rows of 151,936: 115 us with 4 CTAs to a
 // row, 120 with every CTA reading the whole row for its own keys, 40 so; one
 // row 15 to 19 us. Of the some 60,000 clocks of a row's only CTA counting takes
-// 27,000 (21,000 without the additions: a key's word and half are ten integer
-// instructions to two values), the weights 10,000, their sums 5,000, the borders
-// of top_p and the crossing 5,000 each and the search for the token's index
-// 7,000.
+// 27,000 (21,000 without its additions; more loads at a time, loads a step
+// ahead and fewer instructions to a value change little), the weights 10,000,
+// their sums 5,000, the borders of top_p and the crossing 5,000 each and the
+// search for the token's index 7,000.
 
 #include <cooperative_groups.h>
 
