@@ -385,6 +385,20 @@ def test_packed_attention_reports_bad_starts(ctx):
     check_packed(q, k, v, [0, 10, 20], [0, 10, 20], True, run_packed(ctx, q, k, v, [0, 10, 20], [0, 10, 20], True))
 
 
+@pytest.mark.parametrize("queries,keys", [([40] * 50, [40] * 50), ([9, 5], [5000, 20])])
+def test_packed_attention_reports_bad_starts_in_every_order_of_work(ctx, queries, keys):
+    # work in a planned order, and work that is split along its keys
+    rng = np.random.default_rng(21)
+    qs, ks = starts(queries), starts(keys)
+    q, k, v = normal(rng, qs[-1], 16, 64), normal(rng, ks[-1], 8, 64), normal(rng, ks[-1], 8, 64)
+    for bad_q, bad_k in ((qs + (np.arange(len(qs)) == len(qs) - 1), ks), (qs, ks[::-1].copy()),
+                         (qs, np.where(np.arange(len(ks)) == 1, ks[-1] + 1, ks))):
+        with pytest.raises(mi.CoreError) as e:
+            run_packed(ctx, q, k, v, bad_q, bad_k, True)
+        assert e.value.status == mi.ERR_INVALID_ARGUMENT and "starts" in e.value.message
+    check_packed(q, k, v, qs, ks, True, run_packed(ctx, q, k, v, qs, ks, True), heads=[0, 15])
+
+
 def test_packed_attention_agrees_with_the_prefill_op(ctx):
     rng = np.random.default_rng(16)
     q, k, v = normal(rng, 100, 16, 128), normal(rng, 100, 8, 128), normal(rng, 100, 8, 128)
