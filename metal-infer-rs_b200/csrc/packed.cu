@@ -35,9 +35,21 @@
 // roles is 150 to 370 of them) where the products take 1,024.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the
-// last time (weights then stay below 2^8, far inside FP16, and the final
-// division by the sum of the same weights takes the factor out), once the
-// product of the step before is done.
+// last time, once the product of the step before is done. Weights are taken
+// over the row's maximum less 7 binary places, so that they lie below 2^15 and
+// use all of FP16's exponents: one is rounded by at most half a step, which is
+// 2^-11 of itself or, below 2^-14, 2^-25, and that is 2^-32 of the row's
+// largest. The final division by the sum of the same weights takes both factors
+// out.
+//
+// The tensor cores cut each product off at 2^-25 of the accumulator's power of
+// two before they add it (measured: beside a first key of weight 1, 131,071
+// keys of 2^-25.04 added nothing, of 2^-23.5 0.69 of their sum, and as many
+// equal keys lost 6e-4 of their mean, more than the output's rounding). So every
+// 8,240 keys (8,192 at head_dim 64) a row puts its output and its sum aside in
+// device memory, in FP32, and its accumulators start from 0: what products lose
+// then adds up to at most 2^-11.6 whatever the length (16,384 tokens of 32/8
+// heads of 128: 1,720 us without, 1,800 so).
 
 #include <cuda.h>
 
@@ -53,7 +65,9 @@ constexpr int kTile = 128;     // rows of a row tile
 constexpr int kThreads = 384;
 constexpr uint64_t kWaitNs = 200ull * 1000 * 1000;
 constexpr int kLeadBlocks = 4; // key tiles from which row tile 1 starts after row tile 0
-constexpr float kGrowth = 8.f; // log2 of the weights' largest value
+constexpr int kAsideKeys = 8192; // keys that are added up in TMEM at most, to whole key tiles
+constexpr float kLift = 7.f;    // log2 of a largest weight when the base is set
+constexpr float kGrowth = 15.f; // and what it may grow to
 
 struct PackedArgs {
   const __half *q, *k, *v;
@@ -68,6 +82,11 @@ struct PackedArgs {
   float scale_log2; // log2(e) / sqrt(HD)
   const struct Plan* plan;
   float* parts;     // states of the parts of split work
+  // Outputs put aside, for a CTA on every SM (more are never resident): a flag
+  // to a place that says whether it is taken, null where no row is that long.
+  uint32_t* taken;
+  float4* aside;    // [places][2][HD / 4 + 1][kTile]: output, then base and sum
+  int places;
 };
 
 template <int HD>
@@ -77,6 +96,7 @@ struct Packed {
   static constexpr uint32_t kTileBytes = kKeys * HD * 2;  // a K or V tile
   static constexpr int kStages = 4;                       // of a K and a V tile
   static constexpr int kBytes = 1024 /*align*/ + 2 * kQBytes + 2 * kStages * kTileBytes + 512;
+  static constexpr int kAside = (kAsideKeys + kKeys - 1) / kKeys;  // key tiles from 0 to aside
   // TMEM columns
   static constexpr uint32_t kS = HD == 128 ? 128 : 192;  // S_1's distance from S_0, which is at 0
   static constexpr uint32_t kP = kKeys;                  // P's distance from its S
@@ -114,13 +134,18 @@ __device__ __noinline__ void attention_row(const __half* q, const __half* k, con
 #pragma unroll
     for (int e = 0; e < kV; ++e) acc[e] *= keep;
     m = top;
+    // these keys' own sum first: one by one, small weights would be lost beside
+    // what the row has
     const int n = min(32, visible - j0);
+    float sum[kV] = {};
     for (int i = 0; i < n; ++i) {
       const float w = __shfl_sync(0xffffffffu, p, i);
       const __half* vr = v + (size_t)(j0 + i) * stride + lane * kV;
 #pragma unroll
-      for (int e = 0; e < kV; ++e) acc[e] += w * __half2float(vr[e]);
+      for (int e = 0; e < kV; ++e) sum[e] += w * __half2float(vr[e]);
     }
+#pragma unroll
+    for (int e = 0; e < kV; ++e) acc[e] += sum[e];
   }
 #pragma unroll
   for (int e = 0; e < kV; ++e) out[lane * kV + e] = __float2half_rn(acc[e] / l);
@@ -372,6 +397,9 @@ __device__ __forceinline__ Work work_at_place(const PackedArgs& a, int key_tile,
 }
 
 constexpr int kPlanThreads = 1024;
+__device__ __forceinline__ void free_places(const PackedArgs& a, int tid) {
+  for (int i = tid; a.taken && i < a.places; i += kPlanThreads) a.taken[i] = 0;
+}
 constexpr int kPlanBins = 2048;  // longer ones share the last
 
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedArgs a, Plan* plan,
@@ -382,6 +410,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedA
   for (int i = tid; i < kPlanBins; i += kPlanThreads) bins[i] = 0;
   pdl_wait();
   pdl_trigger();
+  free_places(a, tid);
   bool bad = false;
   for (int s = tid; s < a.sequences; s += kPlanThreads) bad |= Starts(a, s).bad(a);
   if (__syncthreads_or(bad)) {
@@ -452,6 +481,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_split_kernel(const Packed
   if (tid == 0) count = states = joins = 0;
   pdl_wait();
   pdl_trigger();
+  free_places(a, tid);
   bool bad = false;
   for (int s = tid; s < a.sequences; s += kPlanThreads) bad |= Starts(a, s).bad(a);
   if (__syncthreads_or(bad)) {
@@ -523,7 +553,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_split_kernel(const Packed
 }
 static_assert(kSplitPlaces <= kPlanThreads, "a place to a thread");
 
-// Floats of a part's state: (maximum, sum) and output of 2 x 128 rows.
+// Floats of a part's state: (base, sum) and output of 2 x 128 rows.
 constexpr size_t part_floats(int hd) { return 2 * kTile * (2 + (size_t)hd); }
 
 // What a row is: token and head of the group, keys that it sees.
@@ -593,10 +623,91 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const PackedArgs a, in
   }
 }
 
+// A free place for outputs put aside, by one thread: the SM's own, which the CTA
+// before this one has given back (any other free one would do).
+__device__ __forceinline__ int take_place(const PackedArgs& a) {
+  uint32_t sm;
+  asm volatile("mov.u32 %0, %%smid;" : "=r"(sm));
+  for (int n = 0; n < 4 * a.places; ++n) {
+    const int i = (int)((sm + n) % (uint32_t)a.places);
+    if (atomicCAS(a.taken + i, 0u, 1u) == 0u) {
+      __threadfence();
+      return i;
+    }
+  }
+  return -1;
+}
+// What a sum over base `from` is worth over base `to`.
+__device__ __forceinline__ float rebase(float from, float to) {
+  return from == to ? 1.f : from == -INFINITY ? 0.f : exp2_fast(from - to);
+}
+
+// A row's output and sum of weights go from the accumulators to the row's place
+// aside, on top of what is there, and in the end come back: `at` is that of its
+// first four values, `m` the base of the accumulators. Both are rare, and calls,
+// so that they take no registers from the softmax.
+template <int HD>
+__device__ __noinline__ void put_aside(uint32_t to, float4* at, bool first, float m, float l) {
+  float4* const stats = at + HD / 4 * kTile;
+  const float2 before = first ? make_float2(m, 0.f) : *reinterpret_cast<const float2*>(stats);
+  const float factor = rebase(before.x, m);
+  *reinterpret_cast<float2*>(stats) = make_float2(m, factor * before.y + l);
+#pragma unroll 1
+  for (int c = 0; c < HD; c += 64) {
+    float4 v[16] = {};
+    if (!first)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) v[q] = at[(c / 4 + q) * kTile];
+    uint32_t o[64];
+    tmem_ld32(o, to + c);
+    tmem_ld32(o + 32, to + c + 32);
+    tmem_wait_ld();
+    tie32(o);
+    tie32(o + 32);
+#pragma unroll
+    for (int q = 0; q < 16; ++q)
+      at[(c / 4 + q) * kTile] = make_float4(factor * v[q].x + __uint_as_float(o[4 * q]),
+                                            factor * v[q].y + __uint_as_float(o[4 * q + 1]),
+                                            factor * v[q].z + __uint_as_float(o[4 * q + 2]),
+                                            factor * v[q].w + __uint_as_float(o[4 * q + 3]));
+  }
+}
+// Returns the sum.
+template <int HD>
+__device__ __noinline__ float take_back(uint32_t to, const float4* at, float m, float l) {
+  const float2 before = *reinterpret_cast<const float2*>(at + HD / 4 * kTile);
+  const float factor = rebase(before.x, m);
+#pragma unroll 1
+  for (int c = 0; c < HD; c += 64) {
+    float4 v[16];
+#pragma unroll
+    for (int q = 0; q < 16; ++q) v[q] = at[(c / 4 + q) * kTile];
+    uint32_t o[64];
+    tmem_ld32(o, to + c);
+    tmem_ld32(o + 32, to + c + 32);
+    tmem_wait_ld();
+    tie32(o);
+    tie32(o + 32);
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      const float x[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        o[4 * q + e] = __float_as_uint(factor * x[e] + __uint_as_float(o[4 * q + e]));
+    }
+    tmem_st32(to + c, o);
+    tmem_st32(to + c + 32, o + 32);
+  }
+  tmem_wait_st();
+  return factor * before.y + l;
+}
+
 // How a CTA comes by its work: it looks for its place, it is in the plan's
-// order, or it is in a plan that splits it.
+// order, or it is in a plan that splits it. kLong: rows may be long enough to be
+// put aside (a call of more keys than that; the others' softmax is shorter by
+// its registers: 8192 tokens in 452 us, 460 with it).
 enum Mode { kOwnPlace, kPlanned, kSplit };
-template <int HD, Mode kMode>
+template <int HD, Mode kMode, bool kLong>
 __global__ void __launch_bounds__(kThreads, 1)
     packed_kernel(const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ CUtensorMap map_k,
@@ -620,6 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* tail_full = bars + 20; // the last V tile, before its end is zero
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kStages);
   Work* work = reinterpret_cast<Work*>(bars + 24);
+  int* place_slot = reinterpret_cast<int*>(bars + 28);  // of outputs put aside
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // heads of one place side by side: their key tiles are near each other
@@ -695,6 +807,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int blocks = max(w.blocks[0], w.blocks[1]);
   const uint32_t tmem = *tmem_slot;
+  if (kLong && blocks > C::kAside) {
+    if (tid == 0) *place_slot = take_place(a);
+    __syncthreads();
+    if (*place_slot < 0) {  // cannot be: there is one for every resident CTA
+      if (tid == 0) report_fault(a.fault, kFaultTimeout);
+      if (warp == 8)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                     : "memory");
+      return;
+    }
+  }
   // rows of the CTA's last V tile that are its sequence's, 0: all
   const int tail = blocks > 0 && blocks == (w.keys + kKeys - 1) / kKeys ? w.keys % kKeys : 0;
 
@@ -760,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (t == 1 && min(w.blocks[0], w.blocks[1]) >= kLeadBlocks)
         ok = ok && wait_for(lead, 0, a.fault);
       // stage n: the scores of key tile n, then the values of n - 1
-      int st = 0;
+      int st = 0, fresh = 0;  // `fresh`: the next key tile whose products start from 0
       uint32_t phase = 0;
       for (int n = 0; n <= blocks && ok; ++n) {
         ok = wait_for(kv_full + st, phase, a.fault);
@@ -783,7 +906,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int kk = 0; kk < kKeys / 16; ++kk)
               mma_ts(d_o, d_p + kk * 8, v_lo + (2 * st * C::kTileBytes + kk * 2048) / 16, idesc_o,
-                     n > 1 || kk != 0, one);
+                     n - 1 != fresh || kk != 0, one);
+            if (kLong && n - 1 == fresh) fresh += C::kAside;
             commit(o_full + t, one);
           }
         }
@@ -809,98 +933,114 @@ __global__ void __launch_bounds__(kThreads, 1)
     const long long least =
         a.causal ? (long long)w.keys - (n - 1 - (w.token + t * a.span)) : w.keys;
     const int mine = w.blocks[t];
-    float m = -INFINITY;
+    float m = -INFINITY;  // the row's base: its maximum when it was set, less kLift
     uint64_t l2 = 0;  // two partial sums
     const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2);
+    // this row's place aside
+    auto aside = [&] {
+      return a.aside + ((size_t)*place_slot * 2 + t) * (HD / 4 + 1) * kTile + row;
+    };
     bool ok = true, scored = false;
-    for (int i = 0; i < mine; ++i) {
-      if (!__all_sync(0xffffffffu, scored)) ok = warp_wait(s_full + t, i & 1, a.fault);
-      if (!ok) break;
-      fence_after();
-      uint32_t s[kKeys];
-#pragma unroll
-      for (int c = 0; c + 32 <= kKeys; c += 32) tmem_ld32(s + c, ts + c);
-      if constexpr (kKeys % 32 != 0) tmem_ld16(s + kKeys - 16, ts + kKeys - 16);
-      tmem_wait_ld();
-#pragma unroll
-      for (int c = 0; c + 32 <= kKeys; c += 32) tie32(s + c);
-      if constexpr (kKeys % 32 != 0) tie16(s + kKeys - 16);
-      fence_before();
-      __syncwarp();
-      if (lane == 0) arrive(s_free + t);
-      const int k0 = i * kKeys;
-      if (k0 + kKeys > least) {
-        const int left = visible - k0;
-#pragma unroll
-        for (int e = 0; e < kKeys; ++e)
-          if (e >= left) s[e] = 0xff800000u;  // -inf
+    // key tiles whose products one accumulator takes
+    for (int first = 0; ok && first < mine; first += kLong ? C::kAside : mine) {
+      if (kLong && first > 0) {
+        ok = warp_wait(o_full + t, (first - 1) & 1, a.fault);
+        if (!ok) break;
+        fence_after();
+        float la, lb;
+        split(l2, la, lb);
+        put_aside<HD>(to, aside(), first == C::kAside, m, la + lb);
+        l2 = 0;
       }
-      // a NaN or +inf that the row sees ends in the maximum
-      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      const int last = kLong ? min(mine, first + C::kAside) : mine;
+      for (int i = first; i < last; ++i) {
+        if (!__all_sync(0xffffffffu, scored)) ok = warp_wait(s_full + t, i & 1, a.fault);
+        if (!ok) break;
+        fence_after();
+        uint32_t s[kKeys];
 #pragma unroll
-      for (int e = 0; e < kKeys; e += 2)
-        tops[(e >> 1) & 3] = max3_nan(tops[(e >> 1) & 3], __uint_as_float(s[e]),
-                                      __uint_as_float(s[e + 1]));
-      float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], -INFINITY) * a.scale_log2;
-      if (!(top < INFINITY)) {  // the row ends as NaN, and is done again below
-        l2 = pair_of(__int_as_float(0x7fc00000), 0.f);
-        top = m;
-      }
-      // a maximum that grew past the bound moves the row's base
-      const bool grown = top > m + kGrowth || (m == -INFINITY && top > m);
-      if (__any_sync(0xffffffffu, grown)) {
-        const float base = grown ? top : m;
-        const float factor = !grown ? 1.f : m == -INFINITY ? 0.f : exp2_fast(m - base);
-        m = base;
-        if (i > 0) {
-          l2 = fma2(l2, pair_of(factor, factor), 0);
-          ok = warp_wait(o_full + t, (i - 1) & 1, a.fault);
-          if (!ok) break;
-          fence_after();
+        for (int c = 0; c + 32 <= kKeys; c += 32) tmem_ld32(s + c, ts + c);
+        if constexpr (kKeys % 32 != 0) tmem_ld16(s + kKeys - 16, ts + kKeys - 16);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c + 32 <= kKeys; c += 32) tie32(s + c);
+        if constexpr (kKeys % 32 != 0) tie16(s + kKeys - 16);
+        fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(s_free + t);
+        const int k0 = i * kKeys;
+        if (k0 + kKeys > least) {
+          const int left = visible - k0;
+#pragma unroll
+          for (int e = 0; e < kKeys; ++e)
+            if (e >= left) s[e] = 0xff800000u;  // -inf
+        }
+        // a NaN or +inf that the row sees ends in the maximum
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < kKeys; e += 2)
+          tops[(e >> 1) & 3] = max3_nan(tops[(e >> 1) & 3], __uint_as_float(s[e]),
+                                        __uint_as_float(s[e + 1]));
+        float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], -INFINITY) * a.scale_log2;
+        if (!(top < INFINITY)) {  // the row ends as NaN, and is done again below
+          l2 = pair_of(__int_as_float(0x7fc00000), 0.f);
+          top = m;
+        }
+        // a maximum that grew past the bound moves the row's base
+        const bool grown = top > m + kGrowth || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, grown)) {
+          const float base = grown ? top - kLift : m;
+          const float factor = !grown ? 1.f : m == -INFINITY ? 0.f : exp2_fast(m - base);
+          m = base;
+          if (i > first) {
+            l2 = fma2(l2, pair_of(factor, factor), 0);
+            ok = warp_wait(o_full + t, (i - 1) & 1, a.fault);
+            if (!ok) break;
+            fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(o, to + c);
-            tmem_wait_ld();
-            tie32(o);
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(o, to + c);
+              tmem_wait_ld();
+              tie32(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-            tmem_st32(to + c, o);
+              for (int e = 0; e < 32; ++e)
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+              tmem_st32(to + c, o);
+            }
           }
         }
-      }
-      if (i == 0 && t == 0 && lane == 0) arrive(lead);
-      // P is free once the product of the step before is done
-      const bool free = i == 0 || is_over(o_full + t, (i - 1) & 1);
-      const float base = m == -INFINITY ? 0.f : -m;
-      const uint64_t base2 = pair_of(base, base);
-      uint32_t p[kKeys / 2];
+        if (i == 0 && t == 0 && lane == 0) arrive(lead);
+        // P is free once the product of the step before is done
+        const bool free = i == first || is_over(o_full + t, (i - 1) & 1);
+        const float base = m == -INFINITY ? 0.f : -m;
+        const uint64_t base2 = pair_of(base, base);
+        uint32_t p[kKeys / 2];
 #pragma unroll
-      for (int e = 0; e < kKeys / 2; ++e) {
-        const uint64_t x = fma2(pair_of(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])),
-                                scale2, base2);
-        float w0, w1;
-        split(x, w0, w1);
-        w0 = exp2_fast(w0);
-        w1 = exp2_fast(w1);
-        // the sum takes the weights before their rounding to FP16, which is
-        // off by half a step at most and to either side
-        l2 = add2(l2, pair_of(w0, w1));
-        const __half2 h = __floats2half2_rn(w0, w1);
-        p[e] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-      if (!__all_sync(0xffffffffu, free)) ok = warp_wait(o_full + t, (i - 1) & 1, a.fault);
-      if (!ok) break;
-      fence_after();
-      scored = i + 1 < mine && is_over(s_full + t, (i + 1) & 1);
+        for (int e = 0; e < kKeys / 2; ++e) {
+          const uint64_t x = fma2(pair_of(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])),
+                                  scale2, base2);
+          float w0, w1;
+          split(x, w0, w1);
+          w0 = exp2_fast(w0);
+          w1 = exp2_fast(w1);
+          // the sum takes the weights before their rounding to FP16
+          l2 = add2(l2, pair_of(w0, w1));
+          const __half2 h = __floats2half2_rn(w0, w1);
+          p[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if (!__all_sync(0xffffffffu, free)) ok = warp_wait(o_full + t, (i - 1) & 1, a.fault);
+        if (!ok) break;
+        fence_after();
+        scored = i + 1 < mine && is_over(s_full + t, (i + 1) & 1);
 #pragma unroll
-      for (int c = 0; c + 32 <= kKeys / 2; c += 32) tmem_st32(tp + c, p + c);
-      if constexpr (kKeys % 64 != 0) tmem_st8(tp + kKeys / 2 - 8, p + kKeys / 2 - 8);
-      tmem_wait_st();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) arrive(p_full + t);
+        for (int c = 0; c + 32 <= kKeys / 2; c += 32) tmem_st32(tp + c, p + c);
+        if constexpr (kKeys % 64 != 0) tmem_st8(tp + kKeys / 2 - 8, p + kKeys / 2 - 8);
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(p_full + t);
+      }
     }
     // ---- output ---------------------------------------------------------------------
     const size_t stride = (size_t)a.kvh * HD;
@@ -909,6 +1049,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_after();
       float la, lb;
       split(l2, la, lb);
+      if (kLong && mine > C::kAside) {
+        la = take_back<HD>(to, aside(), m, la + lb);
+        lb = 0.f;
+      }
       if (kMode == kSplit && w.part >= 0) {
         float* state = a.parts + ((size_t)w.part * columns + blockIdx.x % (uint32_t)columns) *
                                      part_floats(HD);
@@ -999,6 +1143,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   fence_before();
   __syncthreads();
+  if (kLong && tid == 0 && blocks > C::kAside) {
+    __threadfence();
+    atomicExch(a.taken + *place_slot, 0u);
+  }
   if (warp == 8) {
     __syncwarp();
     fence_after();
@@ -1054,15 +1202,38 @@ Shape shape_of(const PackedAttention& p, int sm_count) {
   return s;
 }
 
+// Whether a row can be so long that its output is put aside.
+bool has_aside(const PackedAttention& p) {
+  return p.keys > kAsideKeys;
+}
+// Bytes of the flags of places, to a multiple of 16, and of the places.
+size_t taken_bytes(int sm_count) { return ((size_t)sm_count * sizeof(uint32_t) + 15) / 16 * 16; }
+size_t aside_bytes(int sm_count, int hd) {
+  return (size_t)sm_count * 2 * kTile * (hd + 4) * sizeof(float);
+}
+
 // Bytes of the plan, to a multiple of 16.
 size_t plan_bytes(const Shape& s) {
+  if (s.mode == kOwnPlace) return 0;
   if (s.mode == kSplit)
     return sizeof(Plan) + (size_t)s.works * sizeof(Work) + (size_t)s.joins * sizeof(Join);
   return sizeof(Plan) + (size_t)s.places * sizeof(Work);
 }
 
+// Bytes of the states of parts.
+size_t parts_bytes(const Shape& s, int columns, int hd) {
+  return s.mode == kSplit ? (size_t)s.states * columns * part_floats(hd) * sizeof(float) : 0;
+}
+
+template <int HD, bool kLong>
+auto kernel_of(Mode mode) {
+  return mode == kSplit     ? packed_kernel<HD, kSplit, kLong>
+         : mode == kPlanned ? packed_kernel<HD, kPlanned, kLong>
+                            : packed_kernel<HD, kOwnPlace, kLong>;
+}
+
 template <int HD>
-void launch_packed(const Launch& l, PackedArgs a, const Shape& s, void* workspace) {
+void launch_packed(const Launch& l, PackedArgs a, const Shape& s, bool aside, void* workspace) {
   using C = Packed<HD>;
   a.head_tiles = s.head_tiles;
   a.heads = s.heads;
@@ -1075,9 +1246,7 @@ void launch_packed(const Launch& l, PackedArgs a, const Shape& s, void* workspac
   if (!make_f16_map(&mq, a.q, 4, dq, bq) || !make_f16_map(&mk, a.k, 3, dk, bk) ||
       !make_f16_map(&mv, a.v, 3, dk, bk))
     fail(MI_ERR_KERNEL, "packed attention: tensor map encoding failed");
-  auto kernel = s.mode == kSplit     ? packed_kernel<HD, kSplit>
-                : s.mode == kPlanned ? packed_kernel<HD, kPlanned>
-                                     : packed_kernel<HD, kOwnPlace>;
+  auto kernel = aside ? kernel_of<HD, true>(s.mode) : kernel_of<HD, false>(s.mode);
   allow_dynamic_smem(kernel, C::kBytes);
   const int columns = a.kvh * a.head_tiles;
   const long long grid = (s.mode == kSplit ? s.works : s.places) * (long long)columns;
@@ -1086,6 +1255,14 @@ void launch_packed(const Launch& l, PackedArgs a, const Shape& s, void* workspac
          a.tokens, a.sequences);
   Plan* plan = static_cast<Plan*>(workspace);
   a.plan = plan;
+  if (aside) {
+    char* at = static_cast<char*>(workspace) + plan_bytes(s) + parts_bytes(s, columns, HD);
+    a.taken = reinterpret_cast<uint32_t*>(at);
+    a.aside = reinterpret_cast<float4*>(at + taken_bytes(l.sm_count));
+    a.places = l.sm_count;
+    if (s.mode == kOwnPlace)  // no plan that clears them
+      MI_CUDA(cudaMemsetAsync(a.taken, 0, taken_bytes(l.sm_count), l.stream));
+  }
   if (s.mode == kPlanned)
     launch_kernel(l, dim3(1), dim3(kPlanThreads), 0, packed_plan_kernel, a, plan, (int)s.places,
                   C::kKeys);
@@ -1104,10 +1281,8 @@ void launch_packed(const Launch& l, PackedArgs a, const Shape& s, void* workspac
 
 size_t packed_attention_workspace(const PackedAttention& p, int sm_count) {
   const Shape s = shape_of(p, sm_count);
-  if (s.mode == kOwnPlace) return 0;
-  size_t bytes = plan_bytes(s);
-  if (s.mode == kSplit)
-    bytes += (size_t)s.states * p.kvh * s.head_tiles * part_floats(p.hd) * sizeof(float);
+  size_t bytes = plan_bytes(s) + parts_bytes(s, p.kvh * s.head_tiles, p.hd);
+  if (has_aside(p)) bytes += taken_bytes(sm_count) + aside_bytes(sm_count, p.hd);
   return bytes;
 }
 
@@ -1131,9 +1306,9 @@ void packed_attention(const Launch& l, const PackedAttention& p, void* workspace
   a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)p.hd));
   const Shape s = shape_of(p, l.sm_count);
   if (p.hd == 128)
-    launch_packed<128>(l, a, s, workspace);
+    launch_packed<128>(l, a, s, has_aside(p), workspace);
   else
-    launch_packed<64>(l, a, s, workspace);
+    launch_packed<64>(l, a, s, has_aside(p), workspace);
 }
 
 }  // namespace k

@@ -1,0 +1,96 @@
+"""The ops of a ragged batch where their numbers, their order and their errors
+are easily wrong: many keys of small weight, several open batches, kernels that
+only large batches reach, first calls inside a capture.
+
+Tolerances of attention. A weight is held in FP16 over a base at which the
+row's largest is 2^7 or more: it is off by at most 2^-11 of itself or 2^-32 of
+the largest, which is at most the sum, so a mean over n keys moves by at most
+2 (2^-11 + n 2^-32) max|v|. The tensor cores cut a product off at 2^-25 of the
+accumulator's power of two and the sum of 16 at 2^-23: (2^-25 + 2^-27) max|v| a
+key, for the 8,240 keys at most that one accumulator takes. The weights are
+summed in FP32 by tiles of up to 128: (n / 80 + 128) 2^-24. Exponentials and
+joins add less than 2^-16, and the rounded output 2^-11.
+"""
+import numpy as np
+import pytest
+
+import metal_infer as mi
+from test_batched_ops_gpu import attention64, check, normal, run_packed, starts
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- weights far below a row's largest --------------------------------------------
+
+
+def small_weights(hd, exponent, n):
+    """A query, a first key of weight 1 and n - 1 others of about 2^-exponent;
+    the sum of the others' weights."""
+    q, first = np.zeros(hd, np.float16), np.zeros(hd, np.float16)
+    q[3] = 8
+    first[3] = exponent * np.log(2) * np.sqrt(hd) / 8
+    score = 8 * float(first[3]) / np.sqrt(hd)
+    return q, first, (n - 1) * np.exp(-score)
+
+
+def mean_bound(n):
+    """Of a mean over n keys whose values are at most 1."""
+    return (2 * (2.0 ** -11 + n * 2.0 ** -32) + min(n, 8240) * (2.0 ** -25 + 2.0 ** -27) + (n / 80 + 128) * 2.0 ** -24
+            + 2.0 ** -16 + 2.0 ** -11)
+
+
+@pytest.mark.parametrize("other", [1, -1])
+@pytest.mark.parametrize("exponent", [25.05, 24.5])
+@pytest.mark.parametrize("hd,queries", [(64, 37888), (128, 37888), (64, 7), (128, 7)])
+def test_packed_attention_sums_weights_far_below_the_largest(ctx, hd, queries, exponent, other):
+    # a thread that sees all keys, and parts joined
+    n = 131072
+    q, first, rest = small_weights(hd, exponent, n)
+    k, v = np.zeros((n, 1, hd), np.float16), np.full((n, 1, hd), other, np.float16)
+    k[0, 0], v[0] = first, 1
+    got = run_packed(ctx, np.tile(q, (queries, 1, 1)), k, v, [0, queries], [0, n], False).astype(np.float64)
+    want = (1 + other * rest) / (1 + rest)
+    assert np.abs(got - want).max() <= mean_bound(n), (got.min(), got.max(), want)
+
+
+@pytest.mark.parametrize("hd,queries", [(64, 7), (128, 200)])
+def test_packed_attention_sums_small_weights_in_rows_done_again(ctx, hd, queries):
+    # the last key's value is not a number, and the last query alone sees it: the
+    # rows before it meet it in the products and are computed a second time
+    n = 131072
+    q, first, rest = small_weights(hd, 25.05, n)
+    k, v = np.zeros((n, 1, hd), np.float16), np.full((n, 1, hd), -1, np.float16)
+    k[0, 0], v[0], v[n - 1] = first, 1, np.nan
+    got = run_packed(ctx, np.tile(q, (queries, 1, 1)), k, v, [0, queries], [0, n], True).astype(np.float64)
+    seen = rest / (n - 1) * (n - 1 - np.arange(queries - 1, 0, -1))
+    want = ((1 - seen) / (1 + seen))[:, None]
+    assert np.abs(got[:-1, 0] - want).max() <= mean_bound(n)
+    assert np.all(np.isnan(got[-1]))
+
+
+@pytest.mark.parametrize("hd,qh,kvh,queries,keys,causal", [
+    (128, 16, 8, [2400, 2300], [20000, 9500], True),     # in a planned order
+    (64, 16, 8, [2400, 2300], [20000, 9500], False),
+    (128, 4, 1, [70, 300], [100, 66000], True),          # split, its parts as long
+    (64, 8, 8, [1480], [25000], True),                   # one sequence
+])
+def test_packed_attention_rows_longer_than_an_accumulator_takes(ctx, hd, qh, kvh, queries, keys, causal):
+    # scores that grow along the keys, so that what was put aside is weighed
+    # down again and again; NaN behind the last sequence
+    rng = np.random.default_rng(51)
+    qs, ks = starts(queries), starts(keys)
+    q, k, v = normal(rng, qs[-1], qh, hd) * np.float16(3), normal(rng, ks[-1] + 60, kvh, hd), normal(rng, ks[-1] + 60, kvh, hd)
+    for s, n in enumerate(keys):
+        k[ks[s]:ks[s + 1]] *= np.linspace(0.2, 1, n).astype(np.float16)[:, None, None]
+    k[ks[-1]:], v[ks[-1]:] = np.nan, np.nan
+    got = run_packed(ctx, q, k, v, qs, ks, causal)
+    assert np.all(np.isfinite(got))
+    for s, (n, m) in enumerate(zip(queries, keys)):
+        for i in {0, 1, n // 2, n - 2, n - 1}:
+            for h in (0, qh - 1):
+                row, g = qs[s] + i, h // (qh // kvh)
+                seen = m - (n - 1 - i) if causal else m
+                want, tol = attention64(q[row:row + 1, h], k[ks[s]:ks[s + 1], g], v[ks[s]:ks[s + 1], g], [seen])
+                big = np.abs(v[ks[s]:ks[s] + seen, g].astype(float)).max()
+                check(got[row:row + 1, h], want, tol + big * mean_bound(seen), (s, i, h))
+    np.testing.assert_array_equal(got.view(np.uint16), run_packed(ctx, q, k, v, qs, ks, causal).view(np.uint16))
