@@ -297,6 +297,16 @@ void launch_append(const Launch& l, const AppendArgs& a) {
 // warps meet only at a unit's end, where each leaves its state in the ring
 // stage that it has just used up. Two CTAs to an SM keep about 130 KB of
 // loads in flight.
+//
+// Weights are taken over a warp's maximum less 7 binary places, so that they lie
+// below 2^8 and FP16 holds them to half a step of 2^-11 of themselves or 2^-32
+// of the largest (over the maximum itself those of 2^-25 were 0). The tensor
+// cores cut a product off at 2^-25 of the accumulator's power of two before they
+// add it, so every kAsideSteps steps a warp puts its accumulators aside, in FP32,
+// and starts from 0. They go to device memory: a second set of registers cost
+// 96/8 heads of 128 9%.
+constexpr float kLift = 7.f;
+constexpr int kAsideSteps = 128;
 constexpr int kUnitCost = 1;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
@@ -307,6 +317,7 @@ struct PagedArgs {
   __half* out;
   const uint32_t *lengths, *table;
   float* pieces;    // [C][2][16 * HD + 32]
+  float* aside;     // [C][kWarps][aside_floats][32]: accumulators, bases
   uint4* meta;      // [C]: of the unit that slot 1 begins: sequence, unit, last CTA, flag
   uint32_t* fault;
   int sequences, qh, kvh, table_width, page;
@@ -332,6 +343,8 @@ struct PagedShape {
   static constexpr int kBytes = kWarps * kStages * kStageBytes;
 };
 constexpr size_t piece_floats(int hd) { return kHeadsMax * hd + 2 * kHeadsMax; }
+// Of a thread's accumulators and bases of 8 nt heads.
+constexpr int aside_floats(int hd, int nt) { return nt * (hd / 16 * 4 + 2); }
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
@@ -589,12 +602,48 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
     uint32_t qf[NT][kK][2];
     load_q(comp, qf);
     float o[kK][NT][4] = {};
-    float m[NT][2], l[NT][2];
+    float m[NT][2], l[NT][2];  // m: maximum less kLift
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
       l[n][0] = l[n][1] = 0.f;
     }
+    int steps = 0;       // since the accumulators were 0
+    bool aside = false;  // some are put aside
+    // Adds what is aside to the accumulators.
+    auto take_back = [&](const float* at) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float* p = at + (n * 2 + e) * (HD / 16 * 2 + 1) * 32;
+          const float base = p[HD / 16 * 2 * 32];
+          const float g = base == m[n][e] ? 1.f : state_weight(base, m[n][e]);
+#pragma unroll
+          for (int kk = 0; kk < kK; ++kk) {
+            o[kk][n][e] += g * p[2 * kk * 32];
+            o[kk][n][e + 2] += g * p[(2 * kk + 1) * 32];
+          }
+        }
+    };
+    auto put_aside = [&](float* at) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float* p = at + (n * 2 + e) * (HD / 16 * 2 + 1) * 32;
+          p[HD / 16 * 2 * 32] = m[n][e];
+#pragma unroll
+          for (int kk = 0; kk < kK; ++kk) {
+            p[2 * kk * 32] = o[kk][n][e];
+            p[(2 * kk + 1) * 32] = o[kk][n][e + 2];
+            o[kk][n][e] = o[kk][n][e + 2] = 0.f;
+          }
+        }
+    };
+    auto place_aside = [&] {
+      return a.aside + ((size_t)blockIdx.x * kWarps + warp) * aside_floats(HD, NT) * 32 + lane;
+    };
     bool begins = comp.tile == 0;  // this segment holds its unit's first tile
     int stage = 0;
     const int key_k = lane & 15, chunk_k = lane >> 4;                       // K as rows of keys
@@ -641,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
           }
 #pragma unroll
           for (int sh = 4; sh < 32; sh <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, sh));
-          const float top = fmaxf(m[n][e], x);
+          const float top = fmaxf(m[n][e], x - kLift);
           f[n][e] = state_weight(m[n][e], top);
           moved |= top > m[n][e];
           m[n][e] = top;
@@ -691,12 +740,19 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
 
       const bool unit_done = comp.tile + 1 == comp.tiles;
       if (!unit_done && comp.place + 1 < end) {
+        if (++steps == kAsideSteps) {
+          if (aside) take_back(place_aside());
+          put_aside(place_aside());
+          steps = 0;
+          aside = true;
+        }
         ++comp.tile;
         ++comp.place;
         if (++stage == kStages) stage = 0;
         continue;
       }
       // ---- a segment ends: the four warps' states become one -----------------
+      if (aside) take_back(place_aside());
       const Cursor done = comp;
       advance(comp);
       const bool more = comp.place < end;
@@ -760,6 +816,8 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
       if (!more) break;
       __syncthreads();
       begins = true;
+      steps = 0;
+      aside = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         m[n][0] = m[n][1] = -INFINITY;
@@ -861,7 +919,8 @@ void paged_append(const Launch& l, const PagedAppend& p) {
 
 size_t paged_attention_workspace(int sm_count, int hd) {
   const size_t c = kCtasMax * sm_count;
-  return c * 2 * piece_floats(hd) * sizeof(float) + c * sizeof(uint4);
+  return c * (sizeof(uint4) + 2 * piece_floats(hd) * sizeof(float) +
+              (size_t)kThreads * aside_floats(hd, kHeadsMax / 8) * sizeof(float));
 }
 
 void paged_attention(const Launch& l, const PagedAttention& p, void* workspace) {
@@ -876,6 +935,7 @@ void paged_attention(const Launch& l, const PagedAttention& p, void* workspace) 
   a.table = p.table;
   a.meta = static_cast<uint4*>(workspace);
   a.pieces = reinterpret_cast<float*>(a.meta + c);
+  a.aside = a.pieces + c * 2 * piece_floats(p.hd);
   a.fault = p.fault;
   a.sequences = p.sequences;
   a.qh = p.qh;

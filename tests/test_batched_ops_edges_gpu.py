@@ -15,7 +15,7 @@ import numpy as np
 import pytest
 
 import metal_infer as mi
-from test_batched_ops_gpu import attention64, check, normal, run_packed, starts
+from test_batched_ops_gpu import attention64, check, normal, paged, rows_of, run_packed, run_paged, starts
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +94,43 @@ def test_packed_attention_rows_longer_than_an_accumulator_takes(ctx, hd, qh, kvh
                 big = np.abs(v[ks[s]:ks[s] + seen, g].astype(float)).max()
                 check(got[row:row + 1, h], want, tol + big * mean_bound(seen), (s, i, h))
     np.testing.assert_array_equal(got.view(np.uint16), run_packed(ctx, q, k, v, qs, ks, causal).view(np.uint16))
+
+
+@pytest.mark.parametrize("other", [1, -1])
+@pytest.mark.parametrize("exponent", [25.05, 24.5])
+@pytest.mark.parametrize("hd,qh", [(64, 1), (128, 1), (128, 12)])
+def test_paged_attention_sums_weights_far_below_the_largest(ctx, hd, qh, exponent, other):
+    # as many long sequences as leave a warp a quarter of one, all of the same pages
+    n, page, sequences = 262144, 256, 296
+    q, first, rest = small_weights(hd, exponent, n)
+    k, v = np.zeros((n // page, page, 1, hd), np.float16), np.full((n // page, page, 1, hd), other, np.float16)
+    k[0, 0, 0], v[0, 0] = first, 1
+    table = np.tile(np.arange(n // page, dtype=np.uint32), (sequences, 1))
+    got = run_paged(ctx, np.tile(q, (sequences, qh, 1)), k, v, [n] * sequences, table).astype(np.float64)
+    want = (1 + other * rest) / (1 + rest)
+    assert np.abs(got - want).max() <= mean_bound(n), (got.min(), got.max(), want)
+
+
+@pytest.mark.parametrize("hd,qh,page", [(64, 3, 16), (64, 20, 24), (128, 3, 24), (128, 20, 16)])
+def test_paged_attention_parts_longer_than_an_accumulator_takes(ctx, hd, qh, page):
+    # scores that grow along the keys, so that what was put aside is weighed
+    # down again and again; units that lie in one block, in two and in between
+    rng = np.random.default_rng(52)
+    n, sequences = 40000, 300
+    lengths = [n - 7 * s for s in range(sequences)]
+    table, pages = paged(rng, [n], page)
+    table = np.tile(table, (sequences, 1))
+    q = normal(rng, sequences, qh, hd) * np.float16(3)
+    kc, vc = np.full((pages, page, 1, hd), np.nan, np.float16), np.full((pages, page, 1, hd), np.nan, np.float16)
+    rows = rows_of(table, 0, n, page)
+    kc.reshape(-1, hd)[rows] = normal(rng, n, hd) * np.linspace(0.2, 1, n).astype(np.float16)[:, None]
+    vc.reshape(-1, hd)[rows] = normal(rng, n, hd)
+    got = run_paged(ctx, q, kc, vc, lengths, table)
+    assert np.all(np.isfinite(got))
+    k, v = kc.reshape(-1, hd)[rows], vc.reshape(-1, hd)[rows]
+    big = np.abs(v.astype(float)).max()
+    for s in (0, 1, 77, 148, 149, 298, 299):
+        for h in (0, qh - 1):
+            want, tol = attention64(q[s, h:h + 1], k, v, [lengths[s]])
+            check(got[s, h:h + 1], want, tol + big * mean_bound(n), (s, h))
+    np.testing.assert_array_equal(got.view(np.uint16), run_paged(ctx, q, kc, vc, lengths, table).view(np.uint16))
