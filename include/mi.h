@@ -135,9 +135,10 @@ mi_status mi_context_synchronize(mi_context* ctx);
 /* Synchronizes, then reports (and clears) the code of a bounded device wait
  * that expired since the last call: 0 = none; otherwise MI_ERR_TIMEOUT is
  * returned and *code names the wait (tensor-core GEMM pipeline: 1 producer,
- * 2 MMA issuer, 3 epilogue, 4 drain). Returns MI_ERR_INVALID_ARGUMENT or
- * MI_ERR_CONFIG when a kernel of this context refused a device-side argument
- * since then (see the ragged batches below). No reference counterpart: Metal
+ * 2 MMA issuer, 3 epilogue, 4 drain; 5 packed attention). Returns
+ * MI_ERR_INVALID_ARGUMENT or MI_ERR_CONFIG when a kernel of this context that
+ * no committed batch answers for refused a device-side argument since then (see
+ * the ragged batches below). No reference counterpart: Metal
  * command-buffer errors (context.rs:1058-1063) have no device-side waits. */
 mi_status mi_context_kernel_status(mi_context* ctx, uint32_t* code);
 /* The context's CUDA stream (cudaStream_t) for interop. */
@@ -204,7 +205,7 @@ void mi_batch_abandon(mi_batch* b);
 /* PendingBatch::wait: consumes the pending handle; stats may be NULL.
  * Returns MI_ERR_TIMEOUT when a kernel's bounded device wait expired (its
  * outputs are not valid), MI_ERR_INVALID_ARGUMENT or MI_ERR_CONFIG when one
- * refused a device-side argument, as mi_context_kernel_status reports it. */
+ * of this batch refused a device-side argument (see the ragged batches). */
 mi_status mi_pending_wait(mi_pending* p, mi_dispatch_stats* stats);
 /* Non-consuming completion query: 1 done, 0 running. */
 int mi_pending_is_complete(const mi_pending* p);
@@ -291,9 +292,11 @@ mi_status mi_batch_copy_into_cache(mi_batch* b, const mi_tensor* source, mi_tens
  * replays on the same addresses; starts, lengths, tables and options are read
  * on the device at run time. A start, length, page id or option outside of
  * its range is left out by the kernel (its rows' values are then unspecified,
- * nothing outside of the tensors is touched) and the next mi_pending_wait or
- * mi_context_kernel_status of the context returns MI_ERR_INVALID_ARGUMENT
- * (MI_ERR_CONFIG for sampling options).
+ * nothing outside of the tensors is touched), and mi_pending_wait of the batch
+ * returns MI_ERR_INVALID_ARGUMENT (MI_ERR_CONFIG for sampling options). Batches
+ * answer in the order of the stream: what a replayed graph refused before a
+ * commit, or an abandoned batch, comes with that commit's batch, or with
+ * mi_context_kernel_status where no commit follows.
  *
  * Every tensor must belong to the batch's context; data tensors start on a
  * 16-byte boundary; outputs do not overlap inputs (paged_append may rotate

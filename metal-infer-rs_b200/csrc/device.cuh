@@ -145,11 +145,9 @@ __device__ __forceinline__ void hist_add_rows(const uint16_t* logits, int first,
   __syncthreads();
 }
 
-// Says in a context's fault word (mapped host memory) that a device-side
-// argument was refused; the host reads it after a synchronization.
+// Says in a context's fault word that a device-side argument was refused.
 __device__ __forceinline__ void report_fault(uint32_t* fault, uint32_t code) {
-  *reinterpret_cast<volatile uint32_t*>(fault) = code;
-  __threadfence_system();
+  atomicOr(fault, 1u << code);
 }
 
 __device__ __forceinline__ uint32_t pos_of(const Pos& p) {

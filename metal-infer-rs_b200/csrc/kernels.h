@@ -224,7 +224,7 @@ constexpr int kMmaPrefillMinTokens = 512;
 bool attention_prefill_mma(const Launch& l, const AttnProblem& p);
 
 // ---- ragged batches --------------------------------------------------------------
-// Device-side arguments that a kernel refused (mi_context::fault).
+// Device-side arguments that a kernel refused (bits of mi_context::fault).
 enum Fault : uint32_t {
   kFaultStarts = 1,   // starts that do not rise, or leave the rows
   kFaultLength = 2,   // a length its page table cannot hold, or below the appended tokens

@@ -119,9 +119,14 @@ struct mi_context {
   // Reusable scratch of ops on the context's stream (grown on demand).
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
-  // Mapped host word that kernels write when they refuse a device-side
-  // argument (k::Fault), read after a synchronization.
+  // Device word in which kernels leave what they refused of their device-side
+  // arguments (a bit 1 << k::Fault for each), taken in stream order.
   uint32_t* fault = nullptr;
+  bool may_refuse = false;   // such kernels were launched since it was taken
+  bool may_replay = false;   // a captured graph holds such kernels
+  // Mapped host words that take its value: the free ones, and their memory.
+  std::vector<uint32_t*> fault_slots;
+  std::vector<void*> fault_memory;
 };
 
 struct mi_batch {
@@ -134,10 +139,26 @@ struct mi_pending {
   mi_context* ctx = nullptr;
   cudaEvent_t start = nullptr;
   cudaEvent_t stop = nullptr;
+  // What the batch's kernels refused, and when that is known (null: none can).
+  uint32_t* refused = nullptr;
+  cudaEvent_t taken = nullptr;
   std::chrono::steady_clock::time_point wall_start;
 };
 
 namespace mi {
+
+// Makes the context's device the calling thread's for one call.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(const mi_context* ctx) {
+    MI_CUDA(cudaGetDevice(&before));
+    if (before == ctx->device) before = -1;
+    else MI_CUDA(cudaSetDevice(ctx->device));
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
 
 // Allocates a tensor on the context stream (stream-ordered, zero-filled when
 // `zero`).
@@ -156,10 +177,9 @@ unsigned take_device_wait_status();
 // not valid and must not be reported as a result.
 void check_device_waits(const char* what);
 
-// Fails with MI_ERR_INVALID_ARGUMENT (MI_ERR_CONFIG for sampling options) when
-// a kernel refused a device-side argument of the context since the last check
-// (after a synchronization).
-void check_device_arguments(mi_context* ctx);
+// Notes that kernels are about to be launched that may refuse device-side
+// arguments (set the context's fault word).
+void note_refusals(mi_context* ctx);
 
 // Per-launch profiling hooks (CUDA events around a launch when enabled).
 struct ProfileScope {

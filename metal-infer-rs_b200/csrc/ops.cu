@@ -701,19 +701,6 @@ namespace {
 
 // ---- ragged batches ----------------------------------------------------------
 
-// Makes the context's device the calling thread's for one op.
-struct DeviceScope {
-  int before = -1;
-  explicit DeviceScope(const mi_context* ctx) {
-    MI_CUDA(cudaGetDevice(&before));
-    if (before == ctx->device) before = -1;
-    else MI_CUDA(cudaSetDevice(ctx->device));
-  }
-  ~DeviceScope() {
-    if (before >= 0) cudaSetDevice(before);
-  }
-};
-
 // A tensor of the batch's context with this dtype and rank.
 void require_tensor(const mi_context* ctx, const mi_tensor* t, mi_dtype dtype, size_t rank,
                     const char* what) {
@@ -882,6 +869,7 @@ mi_status mi_batch_paged_append(mi_batch* b, const mi_tensor* query, const mi_te
     p.lengths = lengths->u32();
     p.table = table->u32();
     p.fault = ctx->fault;
+    note_refusals(ctx);
     p.tokens = to_int(tokens, "tokens");
     p.sequences = (int)pg.sequences;
     p.kvh = to_int(kvh, "KV heads");
@@ -924,6 +912,7 @@ mi_status mi_batch_paged_attention(mi_batch* b, const mi_tensor* query,
     p.lengths = lengths->u32();
     p.table = table->u32();
     p.fault = ctx->fault;
+    note_refusals(ctx);
     p.sequences = (int)pg.sequences;
     p.qh = to_int(query->shape[1], "query heads");
     p.kvh = to_int(pg.kvh, "KV heads");
@@ -975,6 +964,7 @@ mi_status mi_batch_packed_attention(mi_batch* b, const mi_tensor* query, const m
     p.query_starts = query_starts->u32();
     p.key_starts = key_starts->u32();
     p.fault = ctx->fault;
+    note_refusals(ctx);
     p.causal = causal != 0;
     Out own;
     void* scratch = nullptr;
@@ -1020,6 +1010,7 @@ mi_status mi_batch_sample(mi_batch* b, const mi_tensor* logits, const mi_tensor*
     p.uniform = uniform->f32();
     p.tokens = tokens->u32();
     p.fault = ctx->fault;
+    note_refusals(ctx);
     p.rows = (int)rows;
     p.n = (int)n;
     ProfileScope ps(ctx, "sample_batch");

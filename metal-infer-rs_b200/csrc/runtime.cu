@@ -62,8 +62,9 @@ void context_release(mi_context* ctx) {
     cudaEventDestroy(p.stop);
   }
   if (ctx->scratch) cudaFreeAsync(ctx->scratch, ctx->stream);
+  if (ctx->fault) cudaFreeAsync(ctx->fault, ctx->stream);
   cudaStreamSynchronize(ctx->stream);
-  if (ctx->fault) cudaFreeHost(ctx->fault);
+  for (void* p : ctx->fault_memory) cudaFreeHost(p);
   cudaStreamDestroy(ctx->stream);
   delete ctx;
 }
@@ -146,28 +147,80 @@ void check_device_waits(const char* what) {
          what, code);
 }
 
-void check_device_arguments(mi_context* ctx) {
-  const uint32_t code = *reinterpret_cast<volatile uint32_t*>(ctx->fault);
-  if (!code) return;
-  *reinterpret_cast<volatile uint32_t*>(ctx->fault) = 0;
-  switch (code) {
-    case k::kFaultStarts:
-      fail(MI_ERR_INVALID_ARGUMENT,
-           "starts do not rise or leave their rows; the results are not valid");
-    case k::kFaultLength:
-      fail(MI_ERR_INVALID_ARGUMENT,
-           "a length does not fit its page table or its tokens; the results are not valid");
-    case k::kFaultPage:
-      fail(MI_ERR_INVALID_ARGUMENT,
-           "a page table names a page outside of the cache; the results are not valid");
-    case k::kFaultSampling:
-      fail(MI_ERR_CONFIG,
-           "invalid model configuration: sampling options outside of their ranges");
-    case k::kFaultTimeout:
-      fail(MI_ERR_TIMEOUT, "a bounded device wait expired; the results are not valid");
-    default:
-      fail(MI_ERR_COMMAND, "a kernel refused its arguments (code %u)", code);
+// ---- refused device-side arguments ------------------------------------------------
+// Kernels of several batches may be in flight, so the context's word is taken
+// in stream order: a commit lets the device move it into a host word of the
+// pending batch, behind the batch's kernels.
+
+namespace {
+
+__global__ void take_fault_kernel(uint32_t* fault, uint32_t* slot) {
+  *slot = atomicExch(fault, 0u);
+}
+
+bool is_capturing(mi_context* ctx) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  MI_CUDA(cudaStreamIsCapturing(ctx->stream, &status));
+  return status != cudaStreamCaptureStatusNone;
+}
+
+// Moves the context's word into a host word that the device writes when it comes
+// to it, null where there can be nothing.
+uint32_t* take_fault(mi_context* ctx) {
+  if ((!ctx->may_refuse && !ctx->may_replay) || is_capturing(ctx)) return nullptr;
+  if (ctx->fault_slots.empty()) {
+    constexpr int kSlots = 64;
+    uint32_t* memory = nullptr;
+    cudaError_t err = cudaHostAlloc(&memory, kSlots * sizeof(uint32_t),
+                                    cudaHostAllocMapped | cudaHostAllocPortable);
+    if (err != cudaSuccess)
+      fail(MI_ERR_RESOURCE, "host allocation failed: %s", cudaGetErrorString(err));
+    ctx->fault_memory.push_back(memory);
+    for (int i = 0; i < kSlots; ++i) ctx->fault_slots.push_back(memory + i);
   }
+  uint32_t* slot = ctx->fault_slots.back();
+  *slot = 0;
+  take_fault_kernel<<<1, 1, 0, ctx->stream>>>(ctx->fault, slot);
+  MI_CUDA(cudaGetLastError());
+  ctx->fault_slots.pop_back();
+  ctx->may_refuse = false;
+  return slot;
+}
+
+// What a host word holds (once the device has written it); frees it.
+uint32_t read_fault(mi_context* ctx, uint32_t* slot) {
+  if (!slot) return 0;
+  const uint32_t bits = *reinterpret_cast<volatile uint32_t*>(slot);
+  ctx->fault_slots.push_back(slot);
+  return bits;
+}
+
+constexpr uint32_t kWaitPacked = 5;  // mi_context_kernel_status's code of kFaultTimeout
+
+void check_fault(uint32_t bits) {
+  auto has = [&](k::Fault f) { return (bits >> f & 1u) != 0; };
+  if (has(k::kFaultTimeout))
+    fail(MI_ERR_TIMEOUT, "a bounded device wait expired (code %u); the results are not valid",
+         kWaitPacked);
+  if (has(k::kFaultStarts))
+    fail(MI_ERR_INVALID_ARGUMENT,
+         "starts do not rise or leave their rows; the results are not valid");
+  if (has(k::kFaultLength))
+    fail(MI_ERR_INVALID_ARGUMENT,
+         "a length does not fit its page table or its tokens; the results are not valid");
+  if (has(k::kFaultPage))
+    fail(MI_ERR_INVALID_ARGUMENT,
+         "a page table names a page outside of the cache; the results are not valid");
+  if (has(k::kFaultSampling))
+    fail(MI_ERR_CONFIG, "invalid model configuration: sampling options outside of their ranges");
+  if (bits) fail(MI_ERR_COMMAND, "a kernel refused its arguments (code 0x%x)", bits);
+}
+
+}  // namespace
+
+void note_refusals(mi_context* ctx) {
+  if (is_capturing(ctx)) ctx->may_replay = true;
+  else ctx->may_refuse = true;
 }
 
 ProfileScope::ProfileScope(mi_context* c, const char* n) : ctx(c), name(n) {
@@ -275,14 +328,13 @@ mi_status mi_context_create(int device, mi_context** out) {
       delete ctx;
       fail(MI_ERR_RESOURCE, "stream creation failed: %s", cudaGetErrorString(err));
     }
-    err = cudaHostAlloc(&ctx->fault, sizeof(uint32_t),
-                        cudaHostAllocMapped | cudaHostAllocPortable);
+    err = cudaMallocAsync(&ctx->fault, sizeof(uint32_t), ctx->stream);
+    if (err == cudaSuccess) err = cudaMemsetAsync(ctx->fault, 0, sizeof(uint32_t), ctx->stream);
     if (err != cudaSuccess) {
       cudaStreamDestroy(ctx->stream);
       delete ctx;
-      fail(MI_ERR_RESOURCE, "host allocation failed: %s", cudaGetErrorString(err));
+      fail(MI_ERR_RESOURCE, "device allocation failed: %s", cudaGetErrorString(err));
     }
-    *ctx->fault = 0;
     // Keep freed stream-ordered memory in the pool (no release to the OS
     // between steps).
     cudaMemPool_t pool;
@@ -364,7 +416,12 @@ mi_status mi_context_kernel_status(mi_context* ctx, uint32_t* code) {
     require_ctx(code, "code");
     sync_context(ctx);
     *code = take_device_wait_status();
-    if (*code == 0) check_device_arguments(ctx);
+    DeviceScope device(ctx);
+    uint32_t* slot = take_fault(ctx);
+    if (slot) sync_context(ctx);
+    const uint32_t refused = read_fault(ctx, slot);
+    if (*code == 0 && refused >> k::kFaultTimeout & 1u) *code = kWaitPacked;
+    if (*code == 0) check_fault(refused);
   });
   if (st == MI_OK && *code != 0) {
     set_error("a bounded device wait expired (code %u)", *code);
@@ -646,18 +703,28 @@ mi_status mi_batch_commit(mi_batch* b, mi_pending** out) {
     require_ctx(b, "batch");
     require_ctx(out, "out");
     auto* p = new mi_pending();
-    p->ctx = b->ctx;
+    mi_context* ctx = p->ctx = b->ctx;
     p->start = b->start;
     p->wall_start = b->wall_start;
     b->start = nullptr;
     delete b;
-    cudaError_t err = cudaEventCreate(&p->stop);
-    if (err == cudaSuccess) err = cudaEventRecord(p->stop, p->ctx->stream);
-    if (err != cudaSuccess) {
+    try {
+      DeviceScope device(ctx);
+      cudaError_t err = cudaEventCreate(&p->stop);
+      if (err == cudaSuccess) err = cudaEventRecord(p->stop, ctx->stream);
+      if (err == cudaSuccess && (p->refused = take_fault(ctx))) {
+        err = cudaEventCreateWithFlags(&p->taken, cudaEventDisableTiming);
+        if (err == cudaSuccess) err = cudaEventRecord(p->taken, ctx->stream);
+      }
+      if (err != cudaSuccess) fail(MI_ERR_COMMAND, "commit failed: %s", cudaGetErrorString(err));
+    } catch (...) {
+      // a host word that the device may still write is not used again
       cudaEventDestroy(p->start);
-      context_release(p->ctx);
+      if (p->stop) cudaEventDestroy(p->stop);
+      if (p->taken) cudaEventDestroy(p->taken);
+      context_release(ctx);
       delete p;
-      fail(MI_ERR_COMMAND, "commit failed: %s", cudaGetErrorString(err));
+      throw;
     }
     *out = p;
   });
@@ -666,21 +733,19 @@ mi_status mi_batch_commit(mi_batch* b, mi_pending** out) {
 mi_status mi_pending_wait(mi_pending* p, mi_dispatch_stats* stats) {
   return guard([&] {
     require_ctx(p, "pending");
-    cudaError_t err = cudaEventSynchronize(p->stop);
+    cudaError_t err = cudaEventSynchronize(p->taken ? p->taken : p->stop);
     float ms = 0.f;
     if (err == cudaSuccess) err = cudaEventElapsedTime(&ms, p->start, p->stop);
     auto wall = std::chrono::steady_clock::now() - p->wall_start;
     cudaEventDestroy(p->start);
     cudaEventDestroy(p->stop);
-    // the context stays until the checks below have read it
-    struct Release {
-      mi_context* ctx;
-      ~Release() { context_release(ctx); }
-    } release{p->ctx};
+    if (p->taken) cudaEventDestroy(p->taken);
+    const uint32_t refused = read_fault(p->ctx, p->refused);
+    context_release(p->ctx);
     delete p;
     if (err != cudaSuccess) fail(MI_ERR_COMMAND, "command failed: %s", cudaGetErrorString(err));
     check_device_waits("batch");
-    check_device_arguments(release.ctx);
+    check_fault(refused);
     if (stats) {
       stats->gpu_time = ms * 1e-3;
       stats->wall_time = std::chrono::duration<double>(wall).count();
@@ -689,7 +754,7 @@ mi_status mi_pending_wait(mi_pending* p, mi_dispatch_stats* stats) {
 }
 
 int mi_pending_is_complete(const mi_pending* p) {
-  return p && cudaEventQuery(p->stop) == cudaSuccess ? 1 : 0;
+  return p && cudaEventQuery(p->taken ? p->taken : p->stop) == cudaSuccess ? 1 : 0;
 }
 
 mi_status mi_batch_finish(mi_batch* b, mi_dispatch_stats* stats) {

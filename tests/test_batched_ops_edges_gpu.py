@@ -15,7 +15,7 @@ import numpy as np
 import pytest
 
 import metal_infer as mi
-from test_batched_ops_gpu import attention64, check, normal, paged, rows_of, run_packed, run_paged, starts
+from test_batched_ops_gpu import Graph, attention64, check, normal, paged, rows_of, run_packed, run_paged, starts, up
 
 pytestmark = pytest.mark.gpu
 
@@ -134,3 +134,99 @@ def test_paged_attention_parts_longer_than_an_accumulator_takes(ctx, hd, qh, pag
             want, tol = attention64(q[s, h:h + 1], k, v, [lengths[s]])
             check(got[s, h:h + 1], want, tol + big * mean_bound(n), (s, h))
     np.testing.assert_array_equal(got.view(np.uint16), run_paged(ctx, q, kc, vc, lengths, table).view(np.uint16))
+
+
+# ---- which batch answers for what a kernel refused ---------------------------------------
+
+
+class Decode:
+    """A small paged attention whose lengths may be bad."""
+
+    def __init__(self, ctx, lengths=(20, 9)):
+        rng = np.random.default_rng(61)
+        self.q, self.kc, self.vc = normal(rng, 2, 2, 64), normal(rng, 4, 16, 1, 64), normal(rng, 4, 16, 1, 64)
+        self.table, self.want = np.array([[0, 1], [2, 3]], np.uint32), None
+        self.tensors = [up(ctx, x) for x in (self.q, self.kc, self.vc, np.array(lengths, np.uint32), self.table)]
+        self.out = up(ctx, np.zeros_like(self.q))
+
+    def __call__(self, b):
+        b.paged_attention(*self.tensors, self.out)
+
+
+def sample_call(ctx, uniform):
+    rng = np.random.default_rng(62)
+    one_of = lambda x: up(ctx, np.full(2, x, np.float32))  # noqa: E731
+    t = [up(ctx, normal(rng, 2, 100)), one_of(1), up(ctx, np.zeros(2, np.uint32)), one_of(1), one_of(0), one_of(uniform),
+         up(ctx, np.zeros(2, np.uint32))]
+    return lambda b: b.sample(*t)
+
+
+def committed(ctx, *calls):
+    b = ctx.begin_batch()
+    for call in calls:
+        call(b)
+    return b.commit()
+
+
+def refused(status, word, call):
+    with pytest.raises(mi.CoreError) as e:
+        call()
+    assert e.value.status == status and word in e.value.message, e.value.message
+
+
+@pytest.mark.parametrize("first_waited", ["first", "last"])
+def test_each_of_several_open_batches_answers_for_itself(ctx, first_waited):
+    good, bad = Decode(ctx), Decode(ctx, (20, 33))
+    batches = [(committed(ctx, good), None), (committed(ctx, bad), (mi.ERR_INVALID_ARGUMENT, "length")),
+               (committed(ctx, good), None), (committed(ctx, sample_call(ctx, 1.0)), (mi.ERR_CONFIG, "sampling")),
+               (committed(ctx, bad, good), (mi.ERR_INVALID_ARGUMENT, "length")), (committed(ctx, good), None)]
+    ctx.synchronize()
+    for p, wrong in batches if first_waited == "first" else batches[::-1]:
+        if wrong:
+            refused(*wrong, p.wait)
+        else:
+            p.wait()
+    assert ctx.kernel_status() == 0
+
+
+def test_the_context_answers_for_what_no_batch_does(ctx):
+    # a committed batch keeps its answer; an abandoned one leaves it to the context
+    p = committed(ctx, Decode(ctx, (20, 33)))
+    assert ctx.kernel_status() == 0
+    refused(mi.ERR_INVALID_ARGUMENT, "length", p.wait)
+    b = ctx.begin_batch()
+    sample_call(ctx, -1.0)(b)
+    del b
+    refused(mi.ERR_CONFIG, "sampling", ctx.kernel_status)
+    assert ctx.kernel_status() == 0
+    committed(ctx, Decode(ctx)).wait()
+
+
+def test_a_replayed_refusal_comes_with_the_next_commit():
+    ctx = mi.MetalContext(0)
+    step, good = Decode(ctx), Decode(ctx)
+    graph = Graph().capture(ctx, step)
+    before = committed(ctx, good)
+    step.tensors[3].write(np.array([20, 33], np.uint32))
+    graph.replay(ctx.stream())
+    after = committed(ctx, good)
+    ctx.synchronize()
+    before.wait()
+    refused(mi.ERR_INVALID_ARGUMENT, "length", after.wait)
+    graph.replay(ctx.stream())
+    refused(mi.ERR_INVALID_ARGUMENT, "length", ctx.kernel_status)
+    step.tensors[3].write(np.array([20, 9], np.uint32))
+    graph.replay(ctx.stream())
+    assert ctx.kernel_status() == 0
+    graph.close()
+
+
+def test_many_open_batches(ctx):
+    # more than the context keeps words for at first
+    bad, good = Decode(ctx, (40, 9)), Decode(ctx)
+    pending = [committed(ctx, bad if i % 3 == 0 else good) for i in range(150)]
+    for i, p in enumerate(pending):
+        if i % 3 == 0:
+            refused(mi.ERR_INVALID_ARGUMENT, "length", p.wait)
+        else:
+            p.wait()
