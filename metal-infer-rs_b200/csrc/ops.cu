@@ -840,8 +840,9 @@ mi_status mi_batch_paged_append(mi_batch* b, const mi_tensor* query, const mi_te
       }
       if (query_out->base() != query->base()) require_apart(query_out, query, "query");
       for (const mi_tensor* t : {key, value, (const mi_tensor*)key_cache,
-                                 (const mi_tensor*)value_cache, starts, lengths, table})
-        require_apart(query_out, t, "another tensor of the call");
+                                 (const mi_tensor*)value_cache, query_weight, key_weight, starts,
+                                 lengths, table})
+        if (t) require_apart(query_out, t, "another tensor of the call");
     }
     MI_REQUIRE(std::isfinite(config.theta) && config.theta > 0.f, MI_ERR_INVALID_ARGUMENT,
                "theta must be positive and finite");

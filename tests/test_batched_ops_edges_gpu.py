@@ -230,3 +230,28 @@ def test_many_open_batches(ctx):
             refused(mi.ERR_INVALID_ARGUMENT, "length", p.wait)
         else:
             p.wait()
+
+
+# ---- refusals -------------------------------------------------------------------------------
+
+
+def test_paged_append_refuses_rotated_queries_over_a_tensor_that_it_reads(ctx):
+    e = lambda *shape: ctx.empty(list(shape), mi.DType.F16)  # noqa: E731
+    u = lambda *shape: ctx.empty(list(shape), mi.DType.U32)  # noqa: E731
+    # every input at the output's address in turn: only the queries themselves may be there
+    named = dict(query=e(3, 2, 64), key=e(3, 2, 64), value=e(3, 2, 64), query_weight=e(64), key_weight=e(64), starts=u(3),
+                 lengths=u(2), table=u(2, 2), key_cache=e(3, 16, 2, 64), value_cache=e(3, 16, 2, 64))
+    for name, t in named.items():
+        whole = ctx.empty([2 * int(np.prod(t.shape())) + 400], mi.DType.U32)
+        kind = t.dtype()
+        over = ctx.tensor_from_device(whole.data_ptr(), t.shape(), kind)
+        out = ctx.tensor_from_device(whole.data_ptr(), [3, 2, 64], mi.DType.F16)
+        args = dict(named, **{name: over})
+        b = ctx.begin_batch()
+        if name == "query":
+            b.paged_append(*args.values(), out, 1e4)
+        else:
+            with pytest.raises(mi.CoreError) as err:
+                b.paged_append(*args.values(), out, 1e4)
+            assert err.value.status == mi.ERR_INVALID_ARGUMENT and "overlaps" in err.value.message, name
+        b.finish()
