@@ -11,6 +11,10 @@ key, for the 8,240 keys at most that one accumulator takes. The weights are
 summed in FP32 by tiles of up to 128: (n / 80 + 128) 2^-24. Exponentials and
 joins add less than 2^-16, and the rounded output 2^-11.
 """
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -255,3 +259,67 @@ def test_paged_append_refuses_rotated_queries_over_a_tensor_that_it_reads(ctx):
                 b.paged_append(*args.values(), out, 1e4)
             assert err.value.status == mi.ERR_INVALID_ARGUMENT and "overlaps" in err.value.message, name
         b.finish()
+
+
+# ---- first calls inside a capture --------------------------------------------------------------
+
+
+FIRST_CALLS = '''
+import ctypes, sys
+import numpy as np
+import metal_infer as mi
+from test_batched_ops_gpu import Graph, down, normal, starts, up
+class Capture(Graph):
+    def call(self, name, *args):
+        if name == "cudaStreamBeginCapture":
+            args = (args[0], ctypes.c_int(int(sys.argv[1])))
+        super().call(name, *args)
+ctx = mi.MetalContext(0)
+rng = np.random.default_rng(71)
+u32 = lambda x: up(ctx, np.asarray(x, np.uint32))
+full = lambda *shape: up(ctx, np.zeros(shape, np.float16))
+f16 = lambda *shape: up(ctx, normal(rng, *shape))
+calls = {}
+for hd in (64, 128):
+    q, out = f16(3, 4, hd), full(3, 4, hd)
+    calls["append", hd] = ("paged_append", [q, f16(3, 2, hd), f16(3, 2, hd), f16(hd), f16(hd), u32([0, 3]), u32([5]), u32([[0]]),
+                                            full(1, 16, 2, hd), full(1, 16, 2, hd), out, 1e4], out)
+    for page in (16, 24):
+        out = full(3, 4, hd)
+        calls["paged", hd, page] = ("paged_attention", [q, f16(3 * 48 // page, page, 2, hd), f16(3 * 48 // page, page, 2, hd),
+                                                        u32([40, 0, 17]), u32(np.arange(3 * 48 // page).reshape(3, -1)), out], out)
+    for name, qh, queries, keys in (("own", 4, [30], [30]), ("planned", 64, [50] * 20, [50] * 20), ("split", 4, [9], [5000]),
+                                    ("long", 1, [37888], [9000]), ("long split", 4, [9], [90000])):
+        out = full(sum(queries), qh, hd)
+        kvh = 8 if qh == 64 else 1
+        calls[name, hd] = ("packed_attention", [f16(sum(queries), qh, hd), f16(sum(keys), kvh, hd), f16(sum(keys), kvh, hd),
+                                                u32(starts(queries)), u32(starts(keys)), False, out], out)
+for rows in (3, 20, 40, 90):
+    f = lambda x: up(ctx, np.full(rows, x, np.float32))
+    out = u32([0] * rows)
+    calls["sample", rows] = ("sample", [f16(rows, 999), f(0.8), u32([50] * rows), f(0.9), f(0), f(0.3), out], out)
+ctx.synchronize()
+graphs = {k: Capture().capture(ctx, lambda b: getattr(b, op)(*args)) for k, (op, args, _) in calls.items()}
+got = {}
+for k, g in graphs.items():
+    g.replay(ctx.stream())
+    got[k] = down(calls[k][2]).copy()
+assert ctx.kernel_status() == 0
+for k, (op, args, out) in calls.items():
+    out.write(np.zeros_like(got[k]))
+    b = ctx.begin_batch()
+    getattr(b, op)(*args)
+    b.finish()
+    assert np.any(got[k]) and np.array_equal(got[k].view(np.uint8), down(out).view(np.uint8)), k
+print("same:", len(calls))
+'''
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2])  # global, of the thread, relaxed
+def test_first_calls_inside_a_capture(mode):
+    # a process that has called none of the ops: captured, replayed, and then called
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    path = os.pathsep.join(os.path.join(root, d) for d in ("tests", "metal-infer-rs_b200", "oracle"))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS, str(mode)], env=dict(os.environ, PYTHONPATH=path), capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and "same:" in r.stdout, (r.stdout[-2000:], r.stderr[-2000:])
