@@ -19,7 +19,8 @@ import numpy as np
 import pytest
 
 import metal_infer as mi
-from test_batched_ops_gpu import Graph, attention64, check, normal, paged, rows_of, run_packed, run_paged, starts, up
+from test_batched_ops_gpu import (OPTIONS, UNIFORMS, Graph, attention64, check, check_packed, logits_of, normal, paged, rows_of,
+                                  run_packed, run_paged, run_sample, sample64, starts, up)
 
 pytestmark = pytest.mark.gpu
 
@@ -323,3 +324,53 @@ def test_first_calls_inside_a_capture(mode):
     r = subprocess.run([sys.executable, "-c", FIRST_CALLS, str(mode)], env=dict(os.environ, PYTHONPATH=path), capture_output=True, text=True,
                        timeout=300)
     assert r.returncode == 0 and "same:" in r.stdout, (r.stdout[-2000:], r.stderr[-2000:])
+
+
+# ---- kernels that large batches reach -------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n", [49153, 151936, 200003, 524224])
+@pytest.mark.parametrize("kind", ["normal", "equal", "two values", "masked", "lowest"])
+def test_sample_large_vocabularies_in_large_batches(ctx, kind, n):
+    # one CTA to a row (90 rows) and two (50): rows of several segments, after each
+    # of which counts near 2^16 move to a list; an odd n leaves rows unaligned
+    rng = np.random.default_rng(81)
+    options = [OPTIONS[0] + (0.37,), OPTIONS[1] + (0.9,), OPTIONS[2] + (0.1,), OPTIONS[3] + (0.999,),
+               OPTIONS[8] + (UNIFORMS[-1],), (1.0, n // 2, 0.9, 0.0, 0.99), (1.3, n - 1, 1.0, 0.0, 0.73)]
+    bits = np.stack([logits_of(kind, rng, n) for _ in options])
+    want = np.array([sample64(b, *o) for b, o in zip(bits, options)], np.uint32)
+    for rows in (90, 50, 25, 7):
+        pick = np.arange(rows) % len(options)
+        np.testing.assert_array_equal(run_sample(ctx, bits[pick], [options[i] for i in pick]), want[pick])
+
+
+@pytest.mark.parametrize("kind", ["normal", "equal", "two values"])
+def test_sample_the_largest_vocabulary_in_large_batches(ctx, kind):
+    # 86 segments to a CTA's row, and a count that moves to the list with most of them
+    n, rng = 2 ** 22, np.random.default_rng(83)
+    options = [OPTIONS[0] + (0.37,), (1.0, n // 2, 0.9, 0.0, 0.99)]
+    bits = np.stack([logits_of(kind, rng, n) for _ in options])
+    want = np.array([sample64(b, *o) for b, o in zip(bits, options)], np.uint32)
+    for rows in (80, 44):
+        pick = np.arange(rows) % 2
+        np.testing.assert_array_equal(run_sample(ctx, bits[pick], [options[i] for i in pick]), want[pick])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("queries,keys", [
+    ([700, 0, 333, 1200, 1, 81, 160, 80, 900], [700, 0, 333, 1200, 1, 81, 160, 80, 900]),
+    ([500, 640, 77, 300, 900, 129], [530, 700, 70, 0, 1000, 2129])])
+def test_packed_attention_ragged_prompts_in_a_planned_order(ctx, hd, queries, keys, causal):
+    # more than two items to an SM and no long prefix: the order from long to
+    # short; sequences without queries or keys, last tiles of every size, and NaN
+    # behind the last sequence
+    rng = np.random.default_rng(82)
+    qs, ks = starts(queries, 3), starts(keys, 5)
+    q, k, v = normal(rng, qs[-1] + 9, 32, hd), normal(rng, ks[-1] + 200, 8, hd), normal(rng, ks[-1] + 200, 8, hd)
+    q[qs[-1]:], k[ks[-1]:], v[ks[-1]:] = np.nan, np.nan, np.nan
+    k[:5], v[:5] = np.inf, np.nan
+    got = run_packed(ctx, q, k, v, qs, ks, causal)
+    check_packed(q, k, v, qs, ks, causal, got, heads=[0, 31])
+    assert np.all(np.isfinite(got[:qs[-1]])) and np.all(got[:3] == 7) and np.all(got[qs[-1]:] == 7)
+    np.testing.assert_array_equal(got.view(np.uint16), run_packed(ctx, q, k, v, qs, ks, causal).view(np.uint16))
