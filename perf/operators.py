@@ -126,6 +126,7 @@ def _logits(rows, vocabulary, generator):
 
 
 def prepare(case, seed):
+    engine = _engine() if own else None  # its stream is the inputs' too
     host = torch.Generator().manual_seed(seed)
     device = torch.Generator(device="cuda").manual_seed(seed)
 
@@ -176,26 +177,33 @@ def prepare(case, seed):
     if own:
         # what a program over the engine holds: its context, an open batch and
         # tensor handles over its device memory
-        state["handles"] = _handles(state)
-        torch.cuda.current_stream().synchronize()
+        mi, context, *_ = state["engine"] = engine
+        context.kernel_status()  # raises what the kernels of earlier passes refused
+        kinds = {torch.float16: mi.DType.F16, torch.float32: mi.DType.F32, torch.int32: mi.DType.U32}
+        state["handles"] = {k: context.tensor_from_device(t.data_ptr(), list(t.shape), kinds[t.dtype])
+                            for k, t in state.items() if isinstance(t, torch.Tensor)}
     return state
 
 
-_engine = None
+_engines = {}  # by device
 
 
-def _handles(state):
-    global _engine
-    if _engine is None:
+def _engine():
+    """The engine on torch's current device, with its stream made torch's current
+    one: what torch and the engine do then follows one another without a wait.
+    (A caller that leaves it for another stream orders the two itself.)"""
+    device = torch.cuda.current_device()
+    if device not in _engines:
         sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                                         "metal-infer-rs_b200"))
         import metal_infer as mi
-        context = mi.MetalContext(torch.cuda.current_device())
-        _engine = (mi, context, context.begin_batch())
-    mi, context, _ = _engine
-    kinds = {torch.float16: mi.DType.F16, torch.float32: mi.DType.F32, torch.int32: mi.DType.U32}
-    return {k: context.tensor_from_device(t.data_ptr(), list(t.shape), kinds[t.dtype])
-            for k, t in state.items() if isinstance(t, torch.Tensor)}
+        context = mi.MetalContext(device)
+        _engines[device] = (mi, context, context.begin_batch(), torch.cuda.ExternalStream(context.stream(), device))
+    stream = _engines[device][3]
+    if torch.cuda.current_stream() != stream:
+        stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(stream)
+    return _engines[device]
 
 
 def run(state):
@@ -203,8 +211,7 @@ def run(state):
 
 
 def _run_own(state):
-    mi, _, batch = _engine
-    case, h = state["case"], state["handles"]
+    case, h, batch = state["case"], state["handles"], state["engine"][2]
     if state["op"] == "sample":
         batch.sample(h["logits"], h["temperature"], h["top_k"], h["top_p"], h["min_p"], h["uniform"], h["tokens"])
         return state["tokens"]
