@@ -326,7 +326,8 @@ mi_status mi_batch_paged_append(mi_batch* b, const mi_tensor* query, const mi_te
                                 mi_tensor* query_out, mi_paged_rope config);
 /* Attention of one new token per sequence: query and out [sequences,
  * query_heads, head_dim]; token s sees positions [0, lengths[s]). A sequence of
- * length 0 gives zeros. Results do not depend on timing. */
+ * length 0 gives zeros; scores that are all -inf give NaN (0 / 0), as do +inf
+ * and NaN among them. Results do not depend on timing. */
 mi_status mi_batch_paged_attention(mi_batch* b, const mi_tensor* query,
                                    const mi_tensor* key_cache, const mi_tensor* value_cache,
                                    const mi_tensor* lengths, const mi_tensor* table,
@@ -335,7 +336,8 @@ mi_status mi_batch_paged_attention(mi_batch* b, const mi_tensor* query,
  * see keys [key_starts[s], ...) of the same sequence. With `causal` the last
  * query sees the last key, the one before it one key less: equal lengths are
  * the usual causal prompt, more keys than queries a prompt whose beginning was
- * computed before. Queries that see no key give zeros. */
+ * computed before. Queries that see no key give zeros; ones whose scores are
+ * all -inf give NaN, as in mi_batch_paged_attention. */
 mi_status mi_batch_packed_attention(mi_batch* b, const mi_tensor* query, const mi_tensor* key,
                                     const mi_tensor* value, const mi_tensor* query_starts,
                                     const mi_tensor* key_starts, int causal, mi_tensor* out);

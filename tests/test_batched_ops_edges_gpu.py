@@ -141,6 +141,30 @@ def test_paged_attention_parts_longer_than_an_accumulator_takes(ctx, hd, qh, pag
     np.testing.assert_array_equal(got.view(np.uint16), run_paged(ctx, q, kc, vc, lengths, table).view(np.uint16))
 
 
+@pytest.mark.parametrize("hd,n,sequences", [(64, 50, 2), (128, 3000, 2), (64, 30000, 300)])
+def test_attention_over_scores_of_minus_infinity(ctx, hd, n, sequences):
+    # keys of weight 0 in front leave the others' result alone; nothing but such
+    # keys is 0 / 0, in one piece, in joined pieces and in what was put aside
+    rng = np.random.default_rng(53)
+    q, k, v = normal(rng, sequences, 2, hd), normal(rng, n, 1, hd), normal(rng, n, 1, hd)
+    q[:, :, 0] = 1
+    k[:n - 7, :, 0] = -np.inf
+    page = 10
+    table = np.tile(np.arange(n // page, dtype=np.uint32), (sequences, 1))
+    lengths = [n if s % 2 == 0 else n - 7 for s in range(sequences)]
+    got = run_paged(ctx, q, k.reshape(-1, page, 1, hd), v.reshape(-1, page, 1, hd), lengths, table)
+    assert np.all(np.isnan(got[1::2]))
+    for s in (0, sequences - 2):
+        for h in (0, 1):
+            check(got[s, h:h + 1], *attention64(q[s, h:h + 1], k[n - 7:, 0], v[n - 7:, 0], [7]), (s, h))
+    for keys in (n, n - 7):
+        got = run_packed(ctx, q[:2], k, v, [0, 2], [0, keys], False)
+        if keys == n:
+            check_packed(q[:2], k[n - 7:], v[n - 7:], [0, 2], [0, 7], False, got)
+        else:
+            assert np.all(np.isnan(got))
+
+
 # ---- which batch answers for what a kernel refused ---------------------------------------
 
 
