@@ -317,7 +317,9 @@ typedef struct mi_paged_rope {
  * and RoPE, values are copied; queries are transformed the same way into
  * query_out (query, query_weight and query_out NULL: no queries). Same bits
  * as mi_batch_qk_norm_rope_cache / mi_batch_rope. Sequences must not share a
- * slot that is written. */
+ * slot that is written. mi_batch_packed_attention takes rotated keys end to end:
+ * a second append writes them, into [rows, 1, kv_heads, head_dim] (pages of one
+ * row) with a table that names each position's row. */
 mi_status mi_batch_paged_append(mi_batch* b, const mi_tensor* query, const mi_tensor* key,
                                 const mi_tensor* value, const mi_tensor* query_weight,
                                 const mi_tensor* key_weight, const mi_tensor* starts,
@@ -336,7 +338,8 @@ mi_status mi_batch_paged_attention(mi_batch* b, const mi_tensor* query,
  * see keys [key_starts[s], ...) of the same sequence. With `causal` the last
  * query sees the last key, the one before it one key less: equal lengths are
  * the usual causal prompt, more keys than queries a prompt whose beginning was
- * computed before. Queries that see no key give zeros; ones whose scores are
+ * computed before (its keys stand in the packed tensor too: it does not read
+ * pages of more than one row). Queries that see no key give zeros; ones whose scores are
  * all -inf give NaN, as in mi_batch_paged_attention. */
 mi_status mi_batch_packed_attention(mi_batch* b, const mi_tensor* query, const mi_tensor* key,
                                     const mi_tensor* value, const mi_tensor* query_starts,

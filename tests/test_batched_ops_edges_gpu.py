@@ -19,7 +19,7 @@ import numpy as np
 import pytest
 
 import metal_infer as mi
-from test_batched_ops_gpu import (OPTIONS, UNIFORMS, Graph, attention64, check, check_packed, logits_of, normal, paged, rows_of,
+from test_batched_ops_gpu import (OPTIONS, UNIFORMS, Graph, attention64, check, check_packed, down, logits_of, normal, paged, rows_of,
                                   run_packed, run_paged, run_sample, sample64, starts, up)
 
 pytestmark = pytest.mark.gpu
@@ -259,6 +259,74 @@ def test_many_open_batches(ctx):
             refused(mi.ERR_INVALID_ARGUMENT, "length", p.wait)
         else:
             p.wait()
+
+
+# ---- together, without the host -------------------------------------------------------------
+
+
+@pytest.mark.parametrize("norm", [True, False])
+def test_prompts_in_chunks_and_then_single_tokens(ctx, norm):
+    # each prompt's rotated keys and its values are appended twice: to the pages
+    # that decoding reads, and, as pages of one row, end to end for the attention
+    # of the prompt's chunks. One batch a step, nothing goes through the host.
+    rng = np.random.default_rng(91)
+    qh, kvh, hd, page, chunks = 8, 2, 64, 16, [[40, 7, 120], [33, 0, 81], [5, 90, 1]]
+    totals = np.sum(chunks, 0)
+    room = starts(totals + 3)  # of the packed rows of a prompt
+    width = int((totals.max() + 3 + page - 1) // page)
+    table = up(ctx, rng.permutation(3 * width).reshape(3, width).astype(np.uint32))
+    rows = np.full((3, totals.max() + 3), 0xFFFFFFF0, np.uint32)
+    for s in range(3):
+        rows[s, :totals[s] + 3] = room[s] + np.arange(totals[s] + 3)
+    rows = up(ctx, rows)
+    kc, vc = (up(ctx, np.full((3 * width, page, kvh, hd), np.nan, np.float16)) for _ in range(2))
+    kp, vp = (up(ctx, np.full((int(room[-1]), 1, kvh, hd), np.nan, np.float16)) for _ in range(2))
+    weights = [up(ctx, normal(rng, hd)) if norm else None for _ in range(2)]
+    keys, values, old = [np.zeros((0, kvh, hd), np.float16)] * 3, [np.zeros((0, kvh, hd), np.float16)] * 3, np.zeros(3, int)
+
+    def rotated(x, weight, first):
+        # the engine's contiguous ops, one sequence at a time
+        if not norm:
+            return down(ctx.rope(up(ctx, x), first, 1e4))
+        flat, other = ctx.empty([first + len(x), x.shape[1], hd], mi.DType.F16), up(ctx, x)
+        b = ctx.begin_batch()
+        b.qk_norm_rope_cache(other, up(ctx, x), weight, weight, flat, mi.QkNormRopeCacheConfig(first, 1e4, 1e-6))
+        b.finish()
+        return down(flat)[first:]
+
+    for counts in chunks + [[1, 1, 1]] * 3:
+        single, st = counts == [1, 1, 1], starts(counts)
+        q, k, v = (normal(rng, st[-1], h, hd) for h in (qh, kvh, kvh))
+        lengths = old + counts
+        tq, tk, tv, ts, tl = (up(ctx, x) for x in (q, k, v, st.astype(np.uint32), lengths.astype(np.uint32)))
+        turned, out = up(ctx, np.zeros_like(q)), up(ctx, np.zeros_like(q))
+        b = ctx.begin_batch()
+        b.paged_append(tq, tk, tv, *weights, ts, tl, table, kc, vc, turned, 1e4)
+        if single:
+            b.paged_attention(turned, kc, vc, tl, table, out)
+        else:
+            # the prompts so far, packed end to end: one call for each, as their
+            # rows have gaps between them
+            b.paged_append(None, tk, tv, None, weights[1], ts, tl, rows, kp, vp, None, 1e4)
+            flat_k, flat_v = kp.reshape([int(room[-1]), kvh, hd]), vp.reshape([int(room[-1]), kvh, hd])
+            for s in range(3):
+                b.packed_attention(turned, flat_k, flat_v, up(ctx, st[s:s + 2].astype(np.uint32)),
+                                   up(ctx, np.array([room[s], room[s] + lengths[s]], np.uint32)), True, out)
+        b.finish()
+        got, rq = down(out), down(turned)
+        for s, n in enumerate(counts):
+            if n == 0:
+                continue
+            a, e = st[s], st[s + 1]
+            np.testing.assert_array_equal(rq[a:e].view(np.uint16), rotated(q[a:e], weights[0], int(old[s])).view(np.uint16))
+            keys[s] = np.concatenate([keys[s], rotated(k[a:e], weights[1], int(old[s]))])
+            values[s] = np.concatenate([values[s], v[a:e]])
+            for h in range(qh):
+                g = h // (qh // kvh)
+                want, tol = attention64(rq[a:e, h], keys[s][:, g], values[s][:, g],
+                                        [lengths[s] - n + i + 1 for i in range(n)])
+                check(got[a:e, h], want, tol, (counts, s, h))
+        old = lengths
 
 
 # ---- refusals -------------------------------------------------------------------------------
