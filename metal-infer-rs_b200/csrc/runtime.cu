@@ -164,19 +164,26 @@ bool is_capturing(mi_context* ctx) {
   return status != cudaStreamCaptureStatusNone;
 }
 
+// More host words for a context.
+cudaError_t add_fault_slots(mi_context* ctx) {
+  constexpr int kSlots = 64;
+  uint32_t* memory = nullptr;
+  const cudaError_t err = cudaHostAlloc(&memory, kSlots * sizeof(uint32_t),
+                                        cudaHostAllocMapped | cudaHostAllocPortable);
+  if (err != cudaSuccess) return err;
+  ctx->fault_memory.push_back(memory);
+  for (int i = 0; i < kSlots; ++i) ctx->fault_slots.push_back(memory + i);
+  return cudaSuccess;
+}
+
 // Moves the context's word into a host word that the device writes when it comes
 // to it, null where there can be nothing.
 uint32_t* take_fault(mi_context* ctx) {
   if ((!ctx->may_refuse && !ctx->may_replay) || is_capturing(ctx)) return nullptr;
   if (ctx->fault_slots.empty()) {
-    constexpr int kSlots = 64;
-    uint32_t* memory = nullptr;
-    cudaError_t err = cudaHostAlloc(&memory, kSlots * sizeof(uint32_t),
-                                    cudaHostAllocMapped | cudaHostAllocPortable);
+    const cudaError_t err = add_fault_slots(ctx);
     if (err != cudaSuccess)
       fail(MI_ERR_RESOURCE, "host allocation failed: %s", cudaGetErrorString(err));
-    ctx->fault_memory.push_back(memory);
-    for (int i = 0; i < kSlots; ++i) ctx->fault_slots.push_back(memory + i);
   }
   uint32_t* slot = ctx->fault_slots.back();
   *slot = 0;
@@ -330,10 +337,13 @@ mi_status mi_context_create(int device, mi_context** out) {
     }
     err = cudaMallocAsync(&ctx->fault, sizeof(uint32_t), ctx->stream);
     if (err == cudaSuccess) err = cudaMemsetAsync(ctx->fault, 0, sizeof(uint32_t), ctx->stream);
+    // host words at once: allocated later they would end a capture elsewhere
+    if (err == cudaSuccess) err = add_fault_slots(ctx);
     if (err != cudaSuccess) {
+      if (ctx->fault) cudaFreeAsync(ctx->fault, ctx->stream);
       cudaStreamDestroy(ctx->stream);
       delete ctx;
-      fail(MI_ERR_RESOURCE, "device allocation failed: %s", cudaGetErrorString(err));
+      fail(MI_ERR_RESOURCE, "allocation failed: %s", cudaGetErrorString(err));
     }
     // Keep freed stream-ordered memory in the pool (no release to the OS
     // between steps).
