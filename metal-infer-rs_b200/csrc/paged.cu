@@ -302,9 +302,9 @@ void launch_append(const Launch& l, const AppendArgs& a) {
 // below 2^8 and FP16 holds them to half a step of 2^-11 of themselves or 2^-32
 // of the largest (over the maximum itself those of 2^-25 were 0). The tensor
 // cores cut a product off at 2^-25 of the accumulator's power of two before they
-// add it, so every kAsideSteps steps a warp puts its accumulators aside, in FP32,
-// and starts from 0. They go to device memory: a second set of registers cost
-// 96/8 heads of 128 9%.
+// add it, so every kAsideSteps steps a warp puts its accumulators and sums aside,
+// in FP32, and starts from 0. They go to device memory: a second set of registers
+// cost 96/8 heads of 128 9%.
 constexpr float kLift = 7.f;
 constexpr int kAsideSteps = 128;
 constexpr int kUnitCost = 1;
@@ -317,7 +317,7 @@ struct PagedArgs {
   __half* out;
   const uint32_t *lengths, *table;
   float* pieces;    // [C][2][16 * HD + 32]
-  float* aside;     // [C][kWarps][aside_floats][32]: accumulators, bases
+  float* aside;     // [C][kWarps][aside_floats][32]: accumulators, bases, sums
   uint4* meta;      // [C]: of the unit that slot 1 begins: sequence, unit, last CTA, flag
   uint32_t* fault;
   int sequences, qh, kvh, table_width, page;
@@ -343,8 +343,8 @@ struct PagedShape {
   static constexpr int kBytes = kWarps * kStages * kStageBytes;
 };
 constexpr size_t piece_floats(int hd) { return kHeadsMax * hd + 2 * kHeadsMax; }
-// Of a thread's accumulators and bases of 8 nt heads.
-constexpr int aside_floats(int hd, int nt) { return nt * (hd / 16 * 4 + 2); }
+// Of a thread's accumulators, bases and sums of 8 nt heads.
+constexpr int aside_floats(int hd, int nt) { return nt * (hd / 16 * 4 + 4); }
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
@@ -616,9 +616,10 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float* p = at + (n * 2 + e) * (HD / 16 * 2 + 1) * 32;
+          const float* p = at + (n * 2 + e) * (HD / 16 * 2 + 2) * 32;
           const float base = p[HD / 16 * 2 * 32];
           const float g = base == m[n][e] ? 1.f : state_weight(base, m[n][e]);
+          l[n][e] += g * p[(HD / 16 * 2 + 1) * 32];
 #pragma unroll
           for (int kk = 0; kk < kK; ++kk) {
             o[kk][n][e] += g * p[2 * kk * 32];
@@ -631,8 +632,10 @@ __global__ void __launch_bounds__(kThreads, PagedShape<HD, NT>::kCtas)
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float* p = at + (n * 2 + e) * (HD / 16 * 2 + 1) * 32;
+          float* p = at + (n * 2 + e) * (HD / 16 * 2 + 2) * 32;
           p[HD / 16 * 2 * 32] = m[n][e];
+          p[(HD / 16 * 2 + 1) * 32] = l[n][e];
+          l[n][e] = 0.f;
 #pragma unroll
           for (int kk = 0; kk < kK; ++kk) {
             p[2 * kk * 32] = o[kk][n][e];
