@@ -7,10 +7,12 @@ row's largest is 2^7 or more: it is off by at most 2^-11 of itself or 2^-32 of
 the largest, which is at most the sum, so a mean over n keys moves by at most
 2 (2^-11 + n 2^-32) max|v|. The tensor cores cut a product off at 2^-25 of the
 accumulator's power of two and the sum of 16 at 2^-23: (2^-25 + 2^-27) max|v| a
-key, for the 8,240 keys at most that one accumulator takes. The weights are
-summed in FP32 by tiles of up to 128: (n / 80 + 128) 2^-24. Exponentials and
-joins add less than 2^-16, and the rounded output 2^-11.
+key, for the 8,240 keys at most that one accumulator takes. The weights of as
+many are summed in FP32, every other one in one sum: 4,120 2^-24; adding up what
+several accumulators took is off by 2^-24 for each. Exponentials and joins add
+less than 2^-16, and the rounded output 2^-11.
 """
+import ctypes
 import os
 import subprocess
 import sys
@@ -40,7 +42,8 @@ def small_weights(hd, exponent, n):
 
 def mean_bound(n):
     """Of a mean over n keys whose values are at most 1."""
-    return (2 * (2.0 ** -11 + n * 2.0 ** -32) + min(n, 8240) * (2.0 ** -25 + 2.0 ** -27) + (n / 80 + 128) * 2.0 ** -24
+    taken = min(n, 8240)
+    return (2 * (2.0 ** -11 + n * 2.0 ** -32) + taken * (2.0 ** -25 + 2.0 ** -27) + (taken / 2 + 2 * n / 1024) * 2.0 ** -24
             + 2.0 ** -16 + 2.0 ** -11)
 
 
@@ -259,6 +262,27 @@ def test_many_open_batches(ctx):
             refused(mi.ERR_INVALID_ARGUMENT, "length", p.wait)
         else:
             p.wait()
+
+
+def test_a_commit_beside_a_capture_of_another_context(ctx):
+    # a capture that forbids the thread to allocate goes on beside another
+    # context's batch and its commit
+    other, rt = mi.MetalContext(0), ctypes.CDLL("libcudart.so.12")
+    step, beside = Decode(ctx), Decode(other, (20, 33))
+    b = other.begin_batch()
+    beside(b)
+    stream, graph = ctypes.c_void_p(ctx.stream()), ctypes.c_void_p()
+    mine = ctx.begin_batch()
+    ctx.synchronize()
+    assert rt.cudaStreamBeginCapture(stream, ctypes.c_int(0)) == 0  # global
+    try:
+        step(mine)
+        p = b.commit()
+    finally:
+        status = rt.cudaStreamEndCapture(stream, ctypes.byref(graph))
+    assert status == 0 and rt.cudaGraphDestroy(graph) == 0
+    refused(mi.ERR_INVALID_ARGUMENT, "length", p.wait)
+    mine.finish()
 
 
 # ---- together, without the host -------------------------------------------------------------
