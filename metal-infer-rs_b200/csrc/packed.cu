@@ -6,10 +6,11 @@
 //
 // Tensor-bound: 4 d operations per visible (query, key) pair and head on the
 // tcgen05 pipe, with the exponentials (16 per clock and SM) close behind at
-// head_dim 128 and ahead of it at 64. A long prompt runs at the board's power
-// limit (8192 tokens: 1.55 of 1.965 GHz), so instructions cost clock: a quarter
-// of the exponentials as polynomials on the FMA pipe shortened the softmax and
-// lost 3% all the same.
+// head_dim 128 and ahead of it at 64; each has 0.55 of its pipe, the rest is the
+// hand-over between the roles. Long prompts one after another also run at the
+// board's power limit (8192 tokens: 1.545 of 1.965 GHz), where instructions cost
+// clock: a quarter of the exponentials as polynomials on the FMA pipe shortened
+// the softmax and lost 3% all the same.
 //
 // A CTA takes two row tiles of one sequence and KV head. The rows of a tile
 // are the query heads of the group for up to 128 / group tokens, so a short
@@ -49,7 +50,7 @@
 // 8,240 keys (8,192 at head_dim 64) a row puts its output and its sum aside in
 // device memory, in FP32, and its accumulators start from 0: what products lose
 // then adds up to at most 2^-11.6 whatever the length (16,384 tokens of 32/8
-// heads of 128: 1,720 us without, 1,800 so).
+// heads of 128: 2.00 ms without, 2.10 so; 65,536: 31.0 and 32.8).
 
 #include <cuda.h>
 
@@ -462,8 +463,8 @@ static_assert(kPlanBins == 2 * kPlanThreads, "two bins to a thread");
 // into as many parts as there are places left in that wave (a part is work like
 // any other over keys of its own), which leave their rows' maxima, sums and
 // unnormalised outputs, and a last kernel joins them in order. With 32/8 heads
-// of 128, 64 queries over 65,536 keys take 855 us in one piece and 88 so, 1,300
-// over 9,300 (1.1 waves) 224 and 170, 1,200 over 5,200 120 and 94.
+// of 128, 64 queries over 65,536 keys take 906 us in one piece and 103 so, 1,300
+// over 9,300 (1.1 waves) 245 and 209, 1,200 over 5,200 122 and 108.
 constexpr int kPartLeast = 8;       // key tiles of a part at least
 constexpr int kSplitPlaces = 512;  // of a call that is split, at most (each is ranked among all)
 constexpr int kSplitRest = 512;    // SMs and one, at most
@@ -704,8 +705,8 @@ __device__ __noinline__ float take_back(uint32_t to, const float4* at, float m, 
 
 // How a CTA comes by its work: it looks for its place, it is in the plan's
 // order, or it is in a plan that splits it. kLong: rows may be long enough to be
-// put aside (a call of more keys than that; the others' softmax is shorter by
-// its registers: 8192 tokens in 452 us, 460 with it).
+// put aside (a call of more keys than that; the others' softmax is spared what
+// the registers for it cost: 8192 tokens, a call at a time, 452 us, 460 with it).
 enum Mode { kOwnPlace, kPlanned, kSplit };
 template <int HD, Mode kMode, bool kLong>
 __global__ void __launch_bounds__(kThreads, 1)
